@@ -380,6 +380,139 @@ typedef struct {
 int vrs_msda(vrs_ctx* ctx, const vrs_msda_desc* d, const float* value, const float* ref,
              const float* off, const float* attw, float* out, void* stream);
 
+/* ---- transformer layers -------------------------------------------------------
+ * The operators around the products of a transformer layer (a detector's
+ * backbone, an image encoder, a text decoder), whose products are 1x1
+ * vrs_conv2d calls over the rows.  No counterpart in the reference, whose one
+ * attention is vrs_psa_attention's.  A "row" is one token: elements of a row
+ * (of a head) are contiguous, rows (and heads) lie any stride apart. */
+
+/* RMS norm of rows, with the residual's addition:
+ *   s = x + res,  y = s * weight / sqrt(mean(s^2) + eps)
+ * all in float32, each output rounded once.  sum (NULL: not stored) receives
+ * s in `dtype`, the next layer's residual; it may be x or res itself.
+ * y_dtype == dtype: y has that type (it may be x or res where sum is not).
+ * y_dtype == VRS_FP8: y is e4m3, rne(clamp(y / scale)), with
+ *   group == 0:     scale = out_step (a power of two), as vrs_conv2d reads
+ *                   with x_e4m3 and in_scale = out_step; scales unused
+ *   group == cols:  one scale per row, max|y| / 448 (1 for a zero row)
+ *   32, 64 or 128:  one per that many columns (cols a multiple of it)
+ * stored in scales[rows][cols / group].  NaN elements do not count in a
+ * maximum and stay NaN.  cols <= 32768.  e4m3 needs 16-byte aligned rows
+ * (x, res, sum and y) and cols % 16 == 0; others take any alignment of their
+ * elements and are fastest at 16 bytes.  weight: float32 [cols]. */
+typedef struct {
+  int32_t rows, cols;
+  int32_t dtype;       /* VRS_BF16 or VRS_F32: x, res, sum */
+  int32_t y_dtype;     /* dtype or VRS_FP8 */
+  int32_t group;
+  float eps;           /* > 0 */
+  float out_step;      /* VRS_FP8 with group 0; else 0 */
+  int64_t x_ld, res_ld, sum_ld, y_ld;   /* elements between rows */
+} vrs_rms_desc;
+int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void* res, const float* weight, void* sum,
+                 void* y, float* scales, void* stream);
+
+/* Packed sequences: sequence i's queries are the rows q_start[i] ..
+ * q_start[i + 1] - 1 (q_start does not fall; a sequence may be empty; rows
+ * before the first and behind the last sequence belong to none and are left
+ * as they were), its keys the k_len[i] rows from k_start[i] of the key and
+ * value buffers, which may be a cache with room behind them.  The queries
+ * are the last of the sequence: query j has the place k_len - q_len + j
+ * among the keys.  k_start NULL: keys lie at the queries' rows; k_len NULL:
+ * as many keys as queries.  All three are DEVICE arrays, read by the kernels
+ * (so a captured graph follows their values); what they say outside the
+ * buffers is cut off, never read or written.
+ * max_q, max_k: the most queries and keys of a sequence, 0 if unknown; they
+ * choose among kernels, and any value gives right results. */
+typedef struct {
+  const int32_t* q_start;  /* [n + 1] */
+  const int32_t* k_start;  /* [n] or NULL */
+  const int32_t* k_len;    /* [n] or NULL */
+  int32_t n;
+  int32_t max_q, max_k;
+} vrs_seqs;
+
+/* Frequencies of rotary positions, in revolutions per position, for
+ * `pairs` pairs: f[i] = base^(-i / pairs) / (2 pi), then for long contexts
+ *   VRS_ROPE_LINEAR    f / factor
+ *   VRS_ROPE_BY_TURNS  pairs with over `high` turns in orig_len positions as
+ *                      they are, under `low` turns f / factor, linear in the
+ *                      turns between
+ *   VRS_ROPE_BY_INDEX  the same with a ramp linear in the pair's index, from
+ *                      floor(index of `high` turns) to ceil(index of `low`)
+ * Host arithmetic in 64 bits; out has `pairs` doubles (put them on the
+ * device for vrs_rope; several axes: one call for each, one after another). */
+#define VRS_ROPE_PLAIN 0
+#define VRS_ROPE_LINEAR 1
+#define VRS_ROPE_BY_TURNS 2
+#define VRS_ROPE_BY_INDEX 3
+int vrs_rope_freqs(int32_t pairs, double base, int32_t scaling, double factor, double low, double high,
+                   double orig_len, double* out);
+
+/* Rotary positions: the first `rot` elements of each head of q and k turn in
+ * pairs by pos * freq[i] revolutions and are multiplied by `scale`,
+ *   (a, b) -> scale * (a cos - b sin, a sin + b cos)
+ * VRS_ROPE_HALF pairs elements (i, i + rot/2), VRS_ROPE_PAIRS (2i, 2i + 1);
+ * the rest of the head is copied.  Angles are computed in 64 bits and reduced
+ * to a fraction of a turn, so far positions lose nothing.
+ * positions: int32 device [axes][pos_ld], pair i using the axis whose
+ * axis_pairs cover it (rows and columns of an image: axes 2); NULL (axes 1):
+ * the row's place among the keys of its sequence, or without seqs the row.
+ * Outputs: q_out row by row.  k_out, and v_out if v is given (copied as it
+ * is): row by row without seqs; with seqs, at the rows of the sequence's keys
+ * that vrs_attention with the same seqs reads, i.e. appended to the cache
+ * (rows whose place lies outside k_out are not written; sequences must not
+ * share rows of it).  q_out may be q and k_out may be k, with the same
+ * strides; k_out must not be k where rows move.  heads or kv_heads may be 0.
+ * rot even, <= 512, <= head_dim <= 4096. */
+#define VRS_ROPE_HALF 0
+#define VRS_ROPE_PAIRS 1
+typedef struct {
+  int32_t rows;              /* of q and k (and v) */
+  int32_t k_out_rows;        /* of k_out and v_out */
+  int32_t heads, kv_heads, head_dim, rot;
+  int32_t layout, dtype;
+  int32_t axes;              /* 1..4 */
+  int32_t axis_pairs[4];     /* pairs of each axis; they add up to rot / 2 */
+  float scale;
+  int64_t pos_ld;            /* >= rows, with positions */
+  /* elements between rows, between heads */
+  int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd;
+  int64_t qo_ld, qo_hd, ko_ld, ko_hd, vo_ld, vo_hd;
+} vrs_rope_desc;
+int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const double* freq, const int32_t* positions,
+             const void* q, const void* k, const void* v, void* q_out, void* k_out, void* v_out, void* stream);
+
+/* Attention over packed sequences, grouped heads:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, g]) v[j, g],
+ *   g = h / (heads / kv_heads)
+ * over the keys of the query's sequence: all of them, or with causal those at
+ * or before the query's own place (see vrs_seqs: the queries are the last of
+ * their sequence, so a prompt, a later piece of one over a cache, and a single
+ * new token are the same call).  A query that sees no key gets 0; keys it does
+ * not see, and whatever lies behind a sequence's keys, do not touch its result
+ * even where they hold NaN.  head_dim: a multiple of 8 up to 128; q, k, v, out
+ * and their strides 16-byte aligned, row strides under 4 M elements.  Scores,
+ * softmax and sums are float32; bfloat16 rounds the probabilities once.
+ * Results do not depend on the run (fixed order of every sum), but the kernel
+ * chosen from max_q, max_k, q_rows and k_rows decides that order.
+ * workspace: 16-byte aligned, of at least vrs_attention_workspace_size bytes
+ * for the same descriptor and seqs (0: none needed, may be NULL); a call uses
+ * it until its kernels end, so calls that may overlap need one each.  Only
+ * seqs' counts are read by vrs_attention_workspace_size. */
+typedef struct {
+  int32_t q_rows;              /* of q and out */
+  int32_t k_rows;              /* of k and v */
+  int32_t heads, kv_heads, head_dim, dtype;   /* VRS_BF16 or VRS_F32 */
+  int32_t causal;
+  float scale;                 /* > 0; 0: head_dim^-0.5 */
+  int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd;   /* elements between rows, between heads */
+} vrs_attention_desc;
+size_t vrs_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs* seqs);
+int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seqs, const void* q, const void* k,
+                  const void* v, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- models (layer closures + graph runtime) ------------------------------ */
 #define VRS_BLOCK_CONV 1        /* conv / conv_bn / dwconv / conv_plain (blocks/conv.rs) */
 #define VRS_BLOCK_C3K2 2        /* c3k2 (blocks/c3k2.rs:94-127) */

@@ -1,0 +1,346 @@
+// C-ABI entry points of the transformer-layer operators (include/vrs.h): RMS
+// norm, rotary positions, attention over packed sequences.  Each checks its
+// arguments, picks a kernel instance and launches it on the caller's stream.
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+#include <tuple>
+
+#include "vrs_internal.h"
+
+using namespace vrs;
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_type(int dtype, const char* what) {
+  if (dtype == VRS_BF16 || dtype == VRS_F32) return VRS_OK;
+  return fail(VRS_EUNSUPPORTED, "%s: dtype %d (VRS_BF16 or VRS_F32)", what, dtype);
+}
+
+// Element types need their own alignment whatever the kernel.
+int check_ptr(const void* p, size_t es, const char* what, const char* name) {
+  if (!p) return fail(VRS_EINVAL, "%s: null %s", what, name);
+  if (!aligned(p, es)) return fail(VRS_EBADSHAPE, "%s: %s is not aligned to its elements", what, name);
+  return VRS_OK;
+}
+
+int check_seqs(const vrs_seqs* s, const char* what) {
+  if (s->n < 0) return fail(VRS_EBADSHAPE, "%s: %d sequences", what, s->n);
+  if (!s->q_start) return fail(VRS_EINVAL, "%s: null q_start", what);
+  if (s->max_q < 0 || s->max_k < 0) return fail(VRS_EINVAL, "%s: negative max_q or max_k", what);
+  return VRS_OK;
+}
+
+int launch(vrs_ctx* ctx, const char* name, dim3 grid, dim3 block, uint32_t lds, void* args, void* stream) {
+  hipFunction_t f;
+  if (int rc = get_fn(ctx, name, &f)) return rc;
+  void* params[] = {args};
+  hipError_t e = hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, block.x, block.y, block.z, lds,
+                                       static_cast<hipStream_t>(stream), params, nullptr);
+  if (e != hipSuccess) return fail(VRS_EHIP, "launch %s: %s", name, hipGetErrorString(e));
+  return VRS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void* res, const float* weight, void* sum,
+                 void* y, float* scales, void* stream) {
+  const char* me = "vrs_rms_norm";
+  if (!ctx || !d) return fail(VRS_EINVAL, "%s: null argument", me);
+  int rc = check_type(d->dtype, me);
+  if (rc) return rc;
+  const bool f8 = d->y_dtype == VRS_FP8;
+  if (!f8 && d->y_dtype != d->dtype)
+    return fail(VRS_EUNSUPPORTED, "%s: y_dtype %d (dtype %d or VRS_FP8)", me, d->y_dtype, d->dtype);
+  if (d->rows < 0 || d->cols < 1) return fail(VRS_EBADSHAPE, "%s: %d rows of %d columns", me, d->rows, d->cols);
+  if (d->cols > 32768) return fail(VRS_EUNSUPPORTED, "%s: %d columns (up to 32768)", me, d->cols);
+  if (!(d->eps > 0.f) || std::isinf(d->eps)) return fail(VRS_EINVAL, "%s: eps %g", me, (double)d->eps);
+  const size_t es = elt_size(d->dtype);
+  if ((rc = check_ptr(x, es, me, "x")) || (rc = check_ptr(weight, 4, me, "weight")) ||
+      (rc = check_ptr(y, f8 ? 1 : es, me, "y")))
+    return rc;
+  if ((res && (rc = check_ptr(res, es, me, "res"))) || (sum && (rc = check_ptr(sum, es, me, "sum")))) return rc;
+  if (sum == y) return fail(VRS_EINVAL, "%s: sum and y are one buffer", me);
+  if (f8 && (x == y || res == y)) return fail(VRS_EINVAL, "%s: an e4m3 y over an input", me);
+  // outputs must not fold rows onto each other; inputs may (a stride of 0 repeats a row)
+  if (d->x_ld < 0 || (res && d->res_ld < 0) || d->y_ld < d->cols || (sum && d->sum_ld < d->cols))
+    return fail(VRS_EBADSHAPE, "%s: row strides", me);
+  for (const auto& [p, ld, name] : {std::tuple<const void*, int64_t, const char*>{x, d->x_ld, "x"}, {res, d->res_ld, "res"}})
+    if (p && ((p == y && ld != d->y_ld) || (p == sum && ld != d->sum_ld)))
+      return fail(VRS_EBADSHAPE, "%s: %s is an output with another row stride", me, name);
+  const int vec = 16 / (int)es;
+  auto fits = [&](const void* p, int64_t ld) { return !p || (aligned(p, 16) && ld % vec == 0); };
+  bool wide = d->cols % vec == 0 && fits(x, d->x_ld) && fits(res, d->res_ld) && fits(sum, d->sum_ld);
+  if (f8) {
+    if (d->group == 0) {
+      int e;
+      if (!(d->out_step >= 1e-30f && d->out_step <= 1e30f) || std::frexp(d->out_step, &e) != 0.5f)
+        return fail(VRS_EINVAL, "%s: out_step %g must be a positive power of two", me, (double)d->out_step);
+    } else {
+      if (d->group != d->cols && d->group != 32 && d->group != 64 && d->group != 128)
+        return fail(VRS_EUNSUPPORTED, "%s: group %d (0, 32, 64, 128 or all %d columns)", me, d->group, d->cols);
+      if (d->cols % d->group) return fail(VRS_EBADSHAPE, "%s: %d columns in groups of %d", me, d->cols, d->group);
+      if ((rc = check_ptr(scales, 4, me, "scales"))) return rc;
+    }
+    if (!wide || d->cols % 16 || !aligned(y, 16) || d->y_ld % 16)
+      return fail(VRS_EBADSHAPE, "%s: e4m3 needs 16-byte aligned rows and a multiple of 16 columns", me);
+  } else {
+    if (d->group) return fail(VRS_EINVAL, "%s: group %d without VRS_FP8", me, d->group);
+    wide = wide && fits(y, d->y_ld);
+  }
+  if (d->rows == 0) return VRS_OK;
+
+  // The fewest threads that hold a row in at most four vectors each: a row
+  // up to 256 vectors (bf16 2048, float32 1024 columns) in one wave, whose
+  // sums need no barrier.
+  struct Shape { int tpr, nv; };
+  static const Shape kWide[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}, {1024, 8}};
+  static const Shape kOne[] = {{64, 4}, {256, 4}, {256, 16}, {1024, 32}};
+  const int v = wide ? vec : 1, chunks = (d->cols + v - 1) / v;
+  const Shape* sh = wide ? kWide : kOne;
+  while (sh->tpr * sh->nv < chunks) ++sh;
+  char name[64];
+  snprintf(name, sizeof name, "vrs_rms_%s_%s_%dx%d_v%d", dsuffix(d->dtype), f8 ? "e4m3" : "same", sh->tpr, sh->nv, v);
+  vrs_rms_args a{};
+  a.x = x; a.res = res; a.weight = weight; a.sum = sum; a.y = y; a.scales = scales;
+  a.x_ld = d->x_ld; a.res_ld = d->res_ld; a.sum_ld = d->sum_ld; a.y_ld = d->y_ld;
+  a.rows = d->rows; a.cols = d->cols; a.eps = d->eps;
+  a.group = f8 ? d->group : 0;
+  a.inv_step = f8 && d->group == 0 ? 1.f / d->out_step : 1.f;
+  const int wg = std::max(sh->tpr, 256), rpw = wg / sh->tpr;
+  const int64_t steps = ((int64_t)d->rows + rpw - 1) / rpw;
+  const int64_t resident = 256ll * (2048 / wg);     // workgroups that fit the card at once
+  return launch(ctx, name, dim3((unsigned)std::min(steps, resident)), dim3(wg), 0, &a, stream);
+}
+
+int vrs_rope_freqs(int32_t pairs, double base, int32_t scaling, double factor, double low, double high,
+                   double orig_len, double* out) {
+  const char* me = "vrs_rope_freqs";
+  if (!out) return fail(VRS_EINVAL, "%s: null out", me);
+  if (pairs < 1 || pairs > 256) return fail(VRS_EBADSHAPE, "%s: %d pairs (1..256)", me, pairs);
+  if (!(base > 1.0) || std::isinf(base)) return fail(VRS_EINVAL, "%s: base %g", me, base);
+  if (scaling < VRS_ROPE_PLAIN || scaling > VRS_ROPE_BY_INDEX) return fail(VRS_EINVAL, "%s: scaling %d", me, scaling);
+  if (scaling != VRS_ROPE_PLAIN && (!(factor > 0.0) || std::isinf(factor)))
+    return fail(VRS_EINVAL, "%s: factor %g", me, factor);
+  if (scaling >= VRS_ROPE_BY_TURNS && (!(low > 0.0) || !(high > low) || std::isinf(high) || !(orig_len >= 1.0) || std::isinf(orig_len)))
+    return fail(VRS_EINVAL, "%s: turns %g .. %g over %g positions", me, low, high, orig_len);
+  // pair index whose frequency makes t turns over orig_len positions
+  auto index_of = [&](double t) { return pairs * std::log(orig_len / (t * 2.0 * M_PI)) / std::log(base); };
+  for (int i = 0; i < pairs; ++i) {
+    const double f = std::pow(base, -(double)i / pairs) / (2.0 * M_PI);
+    double keep = 1.0;      // share of the unscaled frequency
+    if (scaling == VRS_ROPE_LINEAR) keep = 0.0;
+    if (scaling == VRS_ROPE_BY_TURNS) keep = std::clamp((f * orig_len - low) / (high - low), 0.0, 1.0);
+    if (scaling == VRS_ROPE_BY_INDEX) {
+      const double from = std::max(std::floor(index_of(high)), 0.0);
+      const double to = std::max(std::min(std::ceil(index_of(low)), pairs - 1.0), from + 1e-3);
+      keep = 1.0 - std::clamp((i - from) / (to - from), 0.0, 1.0);
+    }
+    out[i] = f * keep + f / (scaling == VRS_ROPE_PLAIN ? 1.0 : factor) * (1.0 - keep);
+  }
+  return VRS_OK;
+}
+
+int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const double* freq, const int32_t* positions,
+             const void* q, const void* k, const void* v, void* q_out, void* k_out, void* v_out, void* stream) {
+  const char* me = "vrs_rope";
+  if (!ctx || !d) return fail(VRS_EINVAL, "%s: null argument", me);
+  int rc = check_type(d->dtype, me);
+  if (rc) return rc;
+  if (d->rows < 0 || d->heads < 0 || d->kv_heads < 0 || d->heads + (int64_t)d->kv_heads < 1 || d->k_out_rows < 0)
+    return fail(VRS_EBADSHAPE, "%s: %d rows, %d + %d heads", me, d->rows, d->heads, d->kv_heads);
+  if (d->head_dim < 1 || d->head_dim > 4096 || d->rot < 2 || d->rot % 2 || d->rot > d->head_dim || d->rot > 512)
+    return fail(VRS_EBADSHAPE, "%s: rot %d of head_dim %d", me, d->rot, d->head_dim);
+  if (d->layout != VRS_ROPE_HALF && d->layout != VRS_ROPE_PAIRS) return fail(VRS_EINVAL, "%s: layout %d", me, d->layout);
+  if (!std::isfinite(d->scale)) return fail(VRS_EINVAL, "%s: scale", me);
+  if (d->axes < 1 || d->axes > 4 || (d->axes > 1 && !positions))
+    return fail(VRS_EINVAL, "%s: %d axes%s", me, d->axes, positions ? "" : " without positions");
+  vrs_rope_args a{};
+  int64_t end = 0;
+  for (int i = 0; i < d->axes; ++i) {
+    if (d->axis_pairs[i] < 0) return fail(VRS_EBADSHAPE, "%s: axis_pairs", me);
+    end += d->axis_pairs[i];
+    a.axis_end[i] = (int32_t)std::min<int64_t>(end, d->rot);
+  }
+  if (end != d->rot / 2) return fail(VRS_EBADSHAPE, "%s: axes of %lld pairs, rot %d", me, (long long)end, d->rot);
+  const size_t es = elt_size(d->dtype);
+  if ((rc = check_ptr(freq, 8, me, "freq"))) return rc;
+  if (positions && (rc = check_ptr(positions, 4, me, "positions"))) return rc;
+  if (positions && d->pos_ld < d->rows) return fail(VRS_EBADSHAPE, "%s: pos_ld", me);
+  if (d->heads && ((rc = check_ptr(q, es, me, "q")) || (rc = check_ptr(q_out, es, me, "q_out")))) return rc;
+  if (d->kv_heads && ((rc = check_ptr(k, es, me, "k")) || (rc = check_ptr(k_out, es, me, "k_out")))) return rc;
+  if (v && (!d->kv_heads || (rc = check_ptr(v, es, me, "v")) || (rc = check_ptr(v_out, es, me, "v_out"))))
+    return rc ? rc : fail(VRS_EINVAL, "%s: v without kv_heads", me);
+  if (seqs && (rc = check_seqs(seqs, me))) return rc;
+  if (d->kv_heads && !seqs && d->k_out_rows < d->rows)
+    return fail(VRS_EBADSHAPE, "%s: %d rows into k_out's %d", me, d->rows, d->k_out_rows);
+  const int64_t in_ld[] = {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd};
+  for (int64_t s : in_ld)
+    if (s < 0) return fail(VRS_EBADSHAPE, "%s: negative stride", me);
+  auto out_ok = [&](int64_t ld, int64_t hd, int heads) {
+    return (ld >= d->head_dim || ld == 0) && (hd >= d->head_dim || heads == 1) && (ld > 0 || d->rows <= 1);
+  };
+  if ((d->heads && !out_ok(d->qo_ld, d->qo_hd, d->heads)) || (d->kv_heads && !out_ok(d->ko_ld, d->ko_hd, d->kv_heads)) ||
+      (v && !out_ok(d->vo_ld, d->vo_hd, d->kv_heads)))
+    return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
+  if (d->heads && q == q_out && (d->q_ld != d->qo_ld || d->q_hd != d->qo_hd))
+    return fail(VRS_EBADSHAPE, "%s: q_out is q with other strides", me);
+  const bool moves = seqs && (seqs->k_start || seqs->k_len);
+  if (d->kv_heads && k == k_out && (moves || d->k_ld != d->ko_ld || d->k_hd != d->ko_hd))
+    return fail(VRS_EBADSHAPE, "%s: k_out is k, but rows move or strides differ", me);
+  if (v && v == v_out) return fail(VRS_EINVAL, "%s: v_out is v", me);
+  if (d->rows == 0 || (seqs && seqs->n == 0)) return VRS_OK;
+
+  // the widest vector that divides the pairs, the head and every stride
+  int vec = 16 / (int)es;
+  auto fits = [&](int n) {
+    const size_t bytes = n * es;
+    bool ok = d->rot / 2 % n == 0 && d->head_dim % n == 0;
+    auto one = [&](const void* p, int64_t ld, int64_t hd) { ok = ok && aligned(p, bytes) && ld % n == 0 && hd % n == 0; };
+    if (d->heads) one(q, d->q_ld, d->q_hd), one(q_out, d->qo_ld, d->qo_hd);
+    if (d->kv_heads) one(k, d->k_ld, d->k_hd), one(k_out, d->ko_ld, d->ko_hd);
+    if (v) one(v, d->v_ld, d->v_hd), one(v_out, d->vo_ld, d->vo_hd);
+    return ok;
+  };
+  while (vec > 1 && !fits(vec)) vec = vec == 8 ? 4 : 1;
+  a.q = q; a.k = k; a.v = v; a.qo = q_out; a.ko = k_out; a.vo = v_out;
+  a.freq = freq; a.pos = positions;
+  if (seqs) a.s.q_start = seqs->q_start, a.s.k_start = seqs->k_start, a.s.k_len = seqs->k_len, a.s.n = seqs->n;
+  a.s.q_rows = d->rows; a.s.k_rows = d->kv_heads ? d->k_out_rows : 0x7fffffff;
+  a.q_ld = d->q_ld; a.q_hd = d->q_hd; a.k_ld = d->k_ld; a.k_hd = d->k_hd; a.v_ld = d->v_ld; a.v_hd = d->v_hd;
+  a.qo_ld = d->qo_ld; a.qo_hd = d->qo_hd; a.ko_ld = d->ko_ld; a.ko_hd = d->ko_hd; a.vo_ld = d->vo_ld; a.vo_hd = d->vo_hd;
+  a.pos_ld = d->pos_ld;
+  a.rows = d->rows; a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.rot = d->rot;
+  a.pairs_layout = d->layout == VRS_ROPE_PAIRS;
+  a.axes = d->axes; a.scale = d->scale;
+  const int64_t pc = d->rot / 2 / vec, tc = (d->head_dim - d->rot) / vec;
+  const int64_t qi = d->heads * pc, qt = q == q_out ? 0 : d->heads * tc, ki = d->kv_heads * pc,
+                kt = k == k_out ? 0 : d->kv_heads * tc, vi = v ? d->kv_heads * (int64_t)(d->head_dim / vec) : 0;
+  const int64_t items = qi + qt + ki + kt + vi;
+  if (items >= (1 << 22)) return fail(VRS_EUNSUPPORTED, "%s: %lld vectors in a row", me, (long long)items);
+  a.qi = (int32_t)qi; a.qt = (int32_t)qt; a.ki = (int32_t)ki; a.kt = (int32_t)kt; a.items = (int32_t)items;
+  a.inv_items = 1.f / (float)items;
+  // four rows to a workgroup (one wave computes a row's angles) once they fill the card twice
+  const int rpw = d->rows >= 2048 ? 4 : 1;
+  const int64_t blocks = ((int64_t)d->rows + rpw - 1) / rpw;
+  if (blocks >= (1ll << 32) / 256) return fail(VRS_EBADSHAPE, "%s: %d rows", me, d->rows);
+  char name[64];
+  snprintf(name, sizeof name, "vrs_rope_%s_v%d_r%d", dsuffix(d->dtype), vec, rpw);
+  return launch(ctx, name, dim3((unsigned)blocks), dim3(256), 0, &a, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
+  const char* me = "vrs_attention";
+  if (!d || !seqs) return fail(VRS_EINVAL, "%s: null argument", me);
+  int rc = check_type(d->dtype, me);
+  if (rc || (rc = check_seqs(seqs, me))) return rc;
+  if (d->q_rows < 0 || d->k_rows < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads)
+    return fail(VRS_EBADSHAPE, "%s: %d and %d rows, %d heads on %d", me, d->q_rows, d->k_rows, d->heads, d->kv_heads);
+  if (d->head_dim < 8 || d->head_dim % 8 || d->head_dim > 128)
+    return fail(VRS_EUNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 128)", me, d->head_dim);
+  if (!(d->scale >= 0.f && d->scale <= 1e30f)) return fail(VRS_EINVAL, "%s: scale %g", me, (double)d->scale);
+  const int vec = 16 / (int)elt_size(d->dtype);
+  for (int64_t s : {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd, d->o_ld, d->o_hd})
+    if (s < 0 || s % vec) return fail(VRS_EBADSHAPE, "%s: strides must be multiples of 16 bytes", me);
+  for (int64_t s : {d->q_ld, d->k_ld, d->v_ld, d->o_ld})
+    if (s >= (1 << 22)) return fail(VRS_EUNSUPPORTED, "%s: row stride %lld", me, (long long)s);
+  if ((d->o_ld < d->head_dim && d->q_rows > 1) || (d->o_hd < d->head_dim && d->heads > 1))
+    return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
+  return VRS_OK;
+}
+
+// Which kernel, and into how many parts the keys are split.
+struct AttentionPlan {
+  bool few;
+  int parts;
+  int64_t row_tiles;      // few: 32-row tiles of the longest sequence; prompts: ids of 128-query tiles
+};
+AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
+  const int64_t group = d->heads / d->kv_heads;
+  const int64_t mq = std::max<int64_t>(1, s->max_q > 0 ? std::min(s->max_q, d->q_rows) : d->q_rows);
+  const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : d->k_rows;
+  AttentionPlan p;
+  p.few = mq * group <= 64;
+  if (p.few) {
+    p.row_tiles = (mq * group + 31) / 32;
+    const int64_t wgs = std::max<int64_t>(1, s->n * d->kv_heads * p.row_tiles);
+    p.parts = (int)std::clamp<int64_t>(std::min(1024 / wgs, mk / 256), 1, 64);
+  } else {
+    p.row_tiles = d->q_rows / 128 + (int64_t)s->n;
+    const int64_t wgs = std::max<int64_t>(1, std::min(p.row_tiles, s->n * ((mq + 127) / 128)) * d->heads);
+    p.parts = (int)std::clamp<int64_t>(std::min(512 / wgs, mk / 512), 1, 16);
+  }
+  return p;
+}
+size_t attention_bytes(const vrs_attention_desc* d, const AttentionPlan& p) {
+  return p.parts == 1 ? 0 : (size_t)p.parts * d->q_rows * d->heads * (d->head_dim + 2) * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vrs_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs* seqs) {
+  if (check_attention(d, seqs) || d->q_rows == 0 || seqs->n == 0) return 0;
+  return attention_bytes(d, plan_attention(d, seqs));
+}
+
+int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seqs, const void* q, const void* k,
+                  const void* v, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* me = "vrs_attention";
+  if (!ctx) return fail(VRS_EINVAL, "%s: null ctx", me);
+  int rc = check_attention(d, seqs);
+  if (rc) return rc;
+  if (d->q_rows == 0 || seqs->n == 0) return VRS_OK;
+  for (const auto& [p, name] : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}}) {
+    if (!p) return fail(VRS_EINVAL, "%s: null %s", me, name);
+    if (!aligned(p, 16)) return fail(VRS_EBADSHAPE, "%s: %s must be 16-byte aligned", me, name);
+  }
+  if (out == k || out == v || (out == q && (d->o_ld != d->q_ld || d->o_hd != d->q_hd)))
+    return fail(VRS_EINVAL, "%s: out is an input", me);
+  const AttentionPlan p = plan_attention(d, seqs);
+  const size_t need = attention_bytes(d, p);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(VRS_EINVAL, "%s: workspace of %zu bytes, %zu needed", me, workspace ? workspace_bytes : (size_t)0, need);
+    if (!aligned(workspace, 16)) return fail(VRS_EINVAL, "%s: workspace alignment", me);
+  }
+  vrs_attention_args a{};
+  a.q = q; a.k = k; a.v = v; a.out = out;
+  a.s.q_start = seqs->q_start; a.s.k_start = seqs->k_start; a.s.k_len = seqs->k_len; a.s.n = seqs->n;
+  a.s.q_rows = d->q_rows; a.s.k_rows = d->k_rows;
+  a.q_ld = d->q_ld; a.q_hd = d->q_hd; a.k_ld = d->k_ld; a.k_hd = d->k_hd;
+  a.v_ld = d->v_ld; a.v_hd = d->v_hd; a.o_ld = d->o_ld; a.o_hd = d->o_hd;
+  a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.causal = d->causal != 0;
+  a.parts = p.parts;
+  a.tiles = (int32_t)p.row_tiles;
+  a.c = (float)((d->scale > 0.f ? (double)d->scale : 1.0 / std::sqrt((double)d->head_dim)) * 1.4426950408889634);
+  if (need) {
+    const int64_t rows = (int64_t)p.parts * d->q_rows * d->heads;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * d->head_dim);
+  }
+  const int64_t blocks = p.parts * (p.few ? (int64_t)seqs->n * d->kv_heads : p.row_tiles * d->heads);
+  const int64_t joins = ((int64_t)d->q_rows * d->heads + 3) / 4;
+  if (p.row_tiles >= (1ll << 31) || blocks >= (1ll << 32) / 256 || joins >= (1ll << 32) / 256)
+    return fail(VRS_EBADSHAPE, "%s: grid too large", me);
+  char name[64];
+  snprintf(name, sizeof name, "vrs_attention_%s_%s_d%d", p.few ? "few" : "prompt", dsuffix(d->dtype),
+           d->head_dim <= 64 ? 64 : 128);
+  if ((rc = launch(ctx, name, dim3((unsigned)blocks, p.few ? (unsigned)p.row_tiles : 1u), dim3(256), 0, &a, stream)))
+    return rc;
+  if (p.parts == 1) return VRS_OK;
+  snprintf(name, sizeof name, "vrs_attention_join_%s", dsuffix(d->dtype));
+  return launch(ctx, name, dim3((unsigned)joins), dim3(256), 0, &a, stream);
+}
+
+}  // extern "C"

@@ -333,4 +333,60 @@ typedef struct {
   int32_t total;        /* N * strips * sps */
 } vrs_stem_pair_args;
 
+/* RMS norm of rows (norm.hip): s = x (+ res), y = s * rsqrt(mean(s^2) + eps) * weight. */
+typedef struct {
+  const void* x;
+  const void* res;      /* NULL: no residual */
+  const float* weight;  /* [cols] */
+  void* sum;            /* NULL: the sum is not stored */
+  void* y;              /* element type, or e4m3 bytes */
+  float* scales;        /* e4m3 with a scale per group: [rows][cols / group] */
+  int64_t x_ld, res_ld, sum_ld, y_ld;   /* elements between rows */
+  int32_t rows, cols;
+  int32_t group;        /* e4m3: columns per scale; 0: the fixed step */
+  float eps;
+  float inv_step;       /* e4m3, group 0 */
+} vrs_rms_args;
+
+/* Packed sequences (vrs_seqs) with the bounds that keep every access inside
+ * the caller's buffers whatever the device arrays hold. */
+typedef struct {
+  const int32_t* q_start;  /* NULL: no sequences */
+  const int32_t* k_start;  /* NULL: q_start */
+  const int32_t* k_len;    /* NULL: as many keys as queries */
+  int32_t n, q_rows, k_rows;
+} vrs_seq_args;
+
+/* Rotary positions (rope.hip). */
+typedef struct {
+  const void *q, *k, *v;
+  void *qo, *ko, *vo;
+  const double* freq;      /* [rot / 2] revolutions per position */
+  const int32_t* pos;      /* [axes][pos_ld], NULL: the row's place in its sequence */
+  vrs_seq_args s;
+  int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd;       /* elements between rows, between heads */
+  int64_t qo_ld, qo_hd, ko_ld, ko_hd, vo_ld, vo_hd;
+  int64_t pos_ld;
+  int32_t rows, heads, kv, dim, rot, pairs_layout;
+  int32_t axes, axis_end[4];   /* pairs before the end of each axis */
+  int32_t items;               /* work items of a row */
+  int32_t qi, ki, qt, kt;      /* items of q and k turns, of the unturned tails */
+  float inv_items;
+  float scale;                 /* of cosine and sine */
+} vrs_rope_args;
+
+/* Attention over packed sequences and caches (attention.hip). */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  float* part_o;           /* parts > 1: [parts][q_rows][heads][dim] */
+  float2* part_ml;         /* parts > 1: [parts][q_rows][heads] running maximum (log2 units) and sum */
+  vrs_seq_args s;
+  int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd;   /* elements between rows, between heads */
+  int32_t heads, kv, dim, causal;
+  int32_t parts;           /* parts that a sequence's keys are split into */
+  int32_t tiles;           /* ids of query tiles (prompts) */
+  float c;                 /* scale * log2(e) */
+} vrs_attention_args;
+
 #endif

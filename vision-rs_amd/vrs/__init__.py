@@ -42,6 +42,8 @@ TILE_KW16 = 15
 TILE_SPLIT_1, TILE_SPLIT_4, TILE_SPLIT_8 = 0x1000, 0x2000, 0x3000   # OR: waves sharing K
 TILE_STEM_PAIR = 11   # model plans: the conv after a 64-channel stem, fused with it (bf16)
 TILE_BPAIR = 12   # model plans: a bottleneck's second 3x3 conv, fused with the first (bf16)
+ROPE_HALF, ROPE_PAIRS = 0, 1   # which elements of a head turn together: (i, i + rot/2) or (2i, 2i + 1)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_TURNS, ROPE_BY_INDEX = 0, 1, 2, 3   # scaling of rope_freqs for long contexts
 TILE_PWPAIR = 13   # model plans: a Detect class output conv fused with the 1x1 conv before it (bf16)
 
 ERRORS = {-1: "EINVAL", -2: "EBADSHAPE", -3: "EUNSUPPORTED", -4: "ENOMODULE", -5: "EHIP", -6: "ENOTFOUND",
@@ -79,6 +81,31 @@ class MsdaDesc(C.Structure):
     _fields_ = [("n", C.c_int32), ("q", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32),
                 ("levels", C.c_int32), ("points", C.c_int32), ("level_h", C.c_int32 * 8),
                 ("level_w", C.c_int32 * 8)]
+
+
+class RmsDesc(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("dtype", C.c_int32), ("y_dtype", C.c_int32),
+                ("group", C.c_int32), ("eps", C.c_float), ("out_step", C.c_float), ("x_ld", C.c_int64),
+                ("res_ld", C.c_int64), ("sum_ld", C.c_int64), ("y_ld", C.c_int64)]
+
+
+class Seqs(C.Structure):
+    _fields_ = [("q_start", C.c_void_p), ("k_start", C.c_void_p), ("k_len", C.c_void_p), ("n", C.c_int32),
+                ("max_q", C.c_int32), ("max_k", C.c_int32)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("k_out_rows", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("rot", C.c_int32), ("layout", C.c_int32), ("dtype", C.c_int32),
+                ("axes", C.c_int32), ("axis_pairs", C.c_int32 * 4), ("scale", C.c_float), ("pos_ld", C.c_int64),
+                *[(n, C.c_int64) for n in ("q_ld", "q_hd", "k_ld", "k_hd", "v_ld", "v_hd",
+                                           "qo_ld", "qo_hd", "ko_ld", "ko_hd", "vo_ld", "vo_hd")]]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("q_rows", C.c_int32), ("k_rows", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+                *[(n, C.c_int64) for n in ("q_ld", "q_hd", "k_ld", "k_hd", "v_ld", "v_hd", "o_ld", "o_hd")]]
 
 
 class BlockDesc(C.Structure):
@@ -133,6 +160,11 @@ SIGNATURES = {
     "vrs_detect_unletterbox": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "vrs_letterbox": (C.c_int, [_vp, _i32, _i32, _vp, _i64, _P(_i64), _P(_i32), _vp, _vp]),
     "vrs_msda": (C.c_int, [_vp, _P(MsdaDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_rms_norm": (C.c_int, [_vp, _P(RmsDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_rope_freqs": (C.c_int, [_i32, C.c_double, _i32, C.c_double, C.c_double, C.c_double, C.c_double, _vp]),
+    "vrs_rope": (C.c_int, [_vp, _P(RopeDesc), _P(Seqs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_attention_workspace_size": (_sz, [_P(AttentionDesc), _P(Seqs)]),
+    "vrs_attention": (C.c_int, [_vp, _P(AttentionDesc), _P(Seqs), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "vrs_model_create": (C.c_int, [_vp, _P(BlockDesc), _i32, _i32, _i32, _i32, _f32, _P(_vp)]),
     "vrs_model_set_autotune": (C.c_int, [_vp, _i32]),
     "vrs_model_num_params": (C.c_int, [_vp]),
@@ -234,6 +266,28 @@ def dtype_code(torch_dtype) -> int:
     if torch_dtype == torch.float32:
         return F32
     raise ValueError(f"unsupported dtype {torch_dtype}")
+
+
+def seqs(q_start, k_start=None, k_len=None, max_q=0, max_k=0):
+    """vrs_seqs: packed sequences from int32 device tensors q_start [n + 1] and, for keys in a cache,
+    k_start [n] and k_len [n].  Holds the tensors; their values are read when the kernels run."""
+    n = q_start.numel() - 1
+    for t, size in ((q_start, n + 1), (k_start, n), (k_len, n)):
+        if t is not None and (str(t.dtype) != "torch.int32" or t.numel() != size or not t.is_contiguous()):
+            raise ValueError("seqs: contiguous int32 tensors q_start [n + 1], k_start [n], k_len [n]")
+    if n < 0:
+        raise ValueError("seqs: q_start needs n + 1 elements")
+    s = Seqs(_ptr(q_start), _ptr(k_start), _ptr(k_len), n, max_q, max_k)
+    s.tensors = (q_start, k_start, k_len)
+    return s
+
+
+def rope_freqs(pairs, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, low=1.0, high=32.0, orig_len=0.0):
+    """vrs_rope_freqs: revolutions per position of each pair, a float64 torch tensor on the host."""
+    import torch
+    out = torch.empty(pairs, dtype=torch.float64)
+    check(lib().vrs_rope_freqs(pairs, base, scaling, factor, low, high, orig_len, out.data_ptr()))
+    return out
 
 
 class Context:
@@ -406,6 +460,143 @@ class Context:
         n, _, a = boxes.shape
         check(lib().vrs_detect_decode_grid(self.handle, _ptr(boxes), _ptr(ax), _ptr(ay), _ptr(strides), n, a,
                                            _ptr(out), _stream(stream)))
+
+    # ---- transformer layers ------------------------------------------------
+    def _rows(self, what, t, dims, dtype=None):
+        """A tensor of rows whose last dimension is contiguous, on this context's device."""
+        if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            raise ValueError(f"{what}: {dims} dimensions, the last one contiguous")
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{what}: on {t.device}, the context is on cuda:{self.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"{what}: {t.dtype}, not {dtype}")
+        return t
+
+    @staticmethod
+    def _ld(t, i):
+        """Elements between neighbours along i (of no account, then one row or head, where there is one)."""
+        return 0 if t is None else t.stride(i) if t.shape[i] > 1 else t.shape[-1]
+
+    def _stream(self, stream):
+        if stream is not None:
+            return stream
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def rms_norm(self, x, weight, eps=1e-6, res=None, sum=None, y=None, e4m3=False, group=0, out_step=0.0,
+                 scales=None, stream=None):
+        """vrs_rms_norm of x [rows, cols] (+ res): returns (y, sum, scales); sum None without res,
+        scales None unless e4m3 with a group.  e4m3: y is uint8, on the fixed out_step (group 0) or
+        with a scale for each `group` columns of a row.  y, sum, scales: outputs to write, else new."""
+        import torch
+        dt = dtype_code(x.dtype)
+        self._rows("rms_norm: x", x, 2)
+        rows, cols = x.shape
+        self._rows("rms_norm: weight", weight, 1, torch.float32)
+        if weight.shape[0] != cols:
+            raise ValueError(f"rms_norm: weight of {weight.shape[0]} for {cols} columns")
+        with _alloc_on(stream, x.device):
+            if y is None:
+                y = torch.empty(rows, cols, dtype=torch.uint8 if e4m3 else x.dtype, device=x.device)
+            if res is not None and sum is None:
+                sum = torch.empty(rows, cols, dtype=x.dtype, device=x.device)
+            if e4m3 and group > 0 and scales is None:
+                scales = torch.empty(rows, cols // group, dtype=torch.float32, device=x.device)
+        for what, t, want in (("res", res, x.dtype), ("sum", sum, x.dtype), ("y", y, torch.uint8 if e4m3 else x.dtype)):
+            if t is not None and self._rows("rms_norm: " + what, t, 2, want).shape != x.shape:
+                raise ValueError(f"rms_norm: {what} of {tuple(t.shape)} for x of {tuple(x.shape)}")
+        if scales is not None and (not e4m3 or group <= 0 or not scales.is_contiguous() or
+                                   self._rows("rms_norm: scales", scales, 2, torch.float32).shape != (rows, cols // group)):
+            raise ValueError("rms_norm: scales are [rows, cols / group], contiguous, for e4m3 with a group")
+        d = RmsDesc(rows, cols, dt, FP8 if e4m3 else dt, group, eps, out_step, self._ld(x, 0), self._ld(res, 0),
+                    self._ld(sum, 0), self._ld(y, 0))
+        check(lib().vrs_rms_norm(self.handle, C.byref(d), _ptr(x), _ptr(res), _ptr(weight), _ptr(sum), _ptr(y),
+                                 _ptr(scales), self._stream(stream)))
+        return y, sum, scales
+
+    def rope(self, q, k, freq, rot_dim=None, layout=ROPE_HALF, seqs=None, positions=None, axis_pairs=None, scale=1.0,
+             q_out=None, k_out=None, v=None, v_out=None, stream=None):
+        """vrs_rope: q [rows, heads, dim] and k [rows, kv_heads, dim] (either may be None) into q_out and
+        k_out, and v as it is into v_out; freq: float64 device tensor [rot_dim / 2] (rope_freqs).
+        positions: int32 [rows] or [axes, rows]; None: the place in the sequence, or the row.
+        With seqs, k_out and v_out [rows of the cache, kv_heads, dim] receive each sequence's rows at
+        its keys' places.  q_out, k_out None: new tensors.  Returns (q_out, k_out)."""
+        import torch
+        t0 = q if q is not None else k
+        dt = dtype_code(t0.dtype)
+        rows, _, dim = t0.shape
+        with _alloc_on(stream, t0.device):
+            if q is not None and q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            if k is not None and k_out is None:
+                if seqs is not None and (seqs.k_start or seqs.k_len):
+                    raise ValueError("rope: keys that move to a cache need k_out")
+                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        if (v is None) != (v_out is None) or (v is not None and k is None):
+            raise ValueError("rope: v, v_out and k go together")
+        ld = []
+        for what, t, n in (("q", q, rows), ("k", k, rows), ("v", v, rows), ("q_out", q_out, rows),
+                           ("k_out", k_out, None), ("v_out", v_out, None if k_out is None else k_out.shape[0])):
+            if t is None:
+                ld += [0, 0]
+                continue
+            like = q if what[0] == "q" else k
+            if like is None:
+                raise ValueError(f"rope: {what} without its input")
+            self._rows("rope: " + what, t, 3, t0.dtype)
+            if t.shape[1:] != (like.shape[1], dim) or (n is not None and t.shape[0] != n):
+                raise ValueError(f"rope: {what} of {tuple(t.shape)}")
+            ld += [self._ld(t, 0), self._ld(t, 1)]
+        rot = dim if rot_dim is None else rot_dim
+        pos_ld = 0
+        if positions is not None:
+            if positions.dim() == 1:
+                positions = positions[None]
+            self._rows("rope: positions", positions, 2, torch.int32)
+            if positions.shape[1] < rows:
+                raise ValueError(f"rope: {positions.shape[1]} positions for {rows} rows")
+            pos_ld = positions.stride(0) if positions.shape[0] > 1 else max(rows, 1)
+        axes = 1 if positions is None else positions.shape[0]
+        per = [rot // 2] if axis_pairs is None else list(axis_pairs)
+        if len(per) != axes or axes > 4:
+            raise ValueError(f"rope: axis_pairs {per} for {axes} axes")
+        self._rows("rope: freq", freq, 1, torch.float64)
+        if freq.shape[0] != rot // 2:
+            raise ValueError(f"rope: {freq.shape[0]} frequencies for rot_dim {rot}")
+        d = RopeDesc(rows, 0 if k_out is None else k_out.shape[0], 0 if q is None else q.shape[1],
+                     0 if k is None else k.shape[1], dim, rot, layout, dt, axes,
+                     (C.c_int32 * 4)(*per), scale, pos_ld, *ld)
+        check(lib().vrs_rope(self.handle, C.byref(d), C.byref(seqs) if seqs is not None else None, _ptr(freq),
+                             _ptr(positions), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out),
+                             self._stream(stream)))
+        return q_out, k_out
+
+    def attention(self, q, k, v, seqs, causal=True, scale=0.0, out=None, workspace=None, stream=None):
+        """vrs_attention: q [rows, heads, dim], k and v [key rows, kv_heads, dim] (a cache as one run of
+        rows), seqs from vrs.seqs; scale 0: dim^-0.5.  workspace: a uint8 device tensor of at least
+        vrs_attention_workspace_size bytes, else allocated.  Returns out (rows of no sequence: as they
+        were, or unset where out is new)."""
+        import torch
+        dt = dtype_code(q.dtype)
+        with _alloc_on(stream, q.device):
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            for what, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+                self._rows("attention: " + what, t, 3, q.dtype)
+            if k.shape != v.shape or q.shape != out.shape or k.shape[2] != q.shape[2]:
+                raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
+                                 f"out {tuple(out.shape)}")
+            d = AttentionDesc(q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], dt, int(causal), scale,
+                              *[self._ld(t, i) for t in (q, k, v, out) for i in (0, 1)])
+            need = lib().vrs_attention_workspace_size(C.byref(d), C.byref(seqs))
+            if workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+                have = need
+            else:
+                have = workspace.numel() * workspace.element_size()
+            check(lib().vrs_attention(self.handle, C.byref(d), C.byref(seqs), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                                      _ptr(workspace), have, self._stream(stream)))
+        return out
 
     def msda(self, value, shapes, ref, off, attw, out, stream=None):
         n, s, heads, dh = value.shape
