@@ -166,7 +166,7 @@ def test_wrappers_check_tensors():
     c = object.__new__(vrs.Context)
     c.handle, c.device = None, 0
     x = torch.zeros(4, 64)
-    with pytest.raises(ValueError, match="context is on"):
+    with pytest.raises(ValueError, match="context's device"):
         c.rms_norm(x, torch.ones(64))
     with pytest.raises(ValueError, match="contiguous"):
         c.rms_norm(torch.zeros(64, 4).t(), torch.ones(64))
@@ -177,3 +177,13 @@ def test_wrappers_check_tensors():
     for bad in ((i.long(),), (i[:0],), (i, i), (i, i[:2], i), (torch.zeros(6, dtype=torch.int32)[::2],)):
         with pytest.raises(ValueError):
             vrs.seqs(*bad)
+
+
+def test_packed_descriptors_have_the_structures_layout():
+    """The binding packs descriptors as bytes: every field at its place in the C structure."""
+    rms_d = vrs.RmsDesc(1, 2, 3, 4, 5, 0.5, 0.25, 6, 7, 8, 9)
+    assert vrs._RMS(1, 2, 3, 4, 5, 0.5, 0.25, 6, 7, 8, 9) == bytes(rms_d)
+    rope_d = vrs.RopeDesc(1, 2, 3, 4, 5, 6, 7, 8, 9, (C.c_int32 * 4)(10, 11, 12, 13), 0.5, *range(14, 27))
+    assert vrs._ROPE(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 0.5, *range(14, 27)) == bytes(rope_d)
+    att_d = vrs.AttentionDesc(1, 2, 3, 4, 5, 6, 7, 0.5, *range(8, 16))
+    assert vrs._ATTENTION(1, 2, 3, 4, 5, 6, 7, 0.5, *range(8, 16)) == bytes(att_d)

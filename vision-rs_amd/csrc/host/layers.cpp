@@ -261,22 +261,30 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
 // Which kernel, and into how many parts the keys are split.
 struct AttentionPlan {
   bool few;
+  int qt;                 // prompts: 32-row tiles of a wave; its workgroup takes 128 * qt rows
   int parts;
-  int64_t row_tiles;      // few: 32-row tiles of the longest sequence; prompts: ids of 128-query tiles
+  int64_t row_tiles;      // few: 32-row tiles of the longest sequence; prompts: ids of row tiles
 };
 AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   const int64_t group = d->heads / d->kv_heads;
   const int64_t mq = std::max<int64_t>(1, s->max_q > 0 ? std::min(s->max_q, d->q_rows) : d->q_rows);
   const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : d->k_rows;
   AttentionPlan p;
+  p.qt = 1;
   p.few = mq * group <= 64;
   if (p.few) {
     p.row_tiles = (mq * group + 31) / 32;
     const int64_t wgs = std::max<int64_t>(1, s->n * d->kv_heads * p.row_tiles);
     p.parts = (int)std::clamp<int64_t>(std::min(1024 / wgs, mk / 256), 1, 64);
   } else {
-    p.row_tiles = d->q_rows / 128 + (int64_t)s->n;
-    const int64_t wgs = std::max<int64_t>(1, std::min(p.row_tiles, s->n * ((mq + 127) / 128)) * d->heads);
+    // row tiles at most: whole ones of all rows and a part of one to each sequence
+    auto count = [&](int64_t bm) {
+      return std::min(d->q_rows * group / bm + s->n, s->n * ((mq * group + bm - 1) / bm));
+    };
+    if (d->head_dim <= 64 && d->dtype == VRS_BF16 && count(256) * d->kv_heads >= 512) p.qt = 2;
+    const int64_t bm = 128 * p.qt;
+    p.row_tiles = d->q_rows * group / bm + (int64_t)s->n;
+    const int64_t wgs = std::max<int64_t>(1, count(bm) * d->kv_heads);
     p.parts = (int)std::clamp<int64_t>(std::min(512 / wgs, mk / 512), 1, 16);
   }
   return p;
@@ -329,15 +337,20 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * d->head_dim);
   }
-  const int64_t blocks = p.parts * (p.few ? (int64_t)seqs->n * d->kv_heads : p.row_tiles * d->heads);
+  const int64_t blocks = p.parts * (p.few ? (int64_t)seqs->n : p.row_tiles) * d->kv_heads;
   const int64_t joins = ((int64_t)d->q_rows * d->heads + 3) / 4;
   if (p.row_tiles >= (1ll << 31) || blocks >= (1ll << 32) / 256 || joins >= (1ll << 32) / 256)
     return fail(VRS_EBADSHAPE, "%s: grid too large", me);
+  const int D = d->head_dim <= 64 ? 64 : 128;
   char name[64];
-  snprintf(name, sizeof name, "vrs_attention_%s_%s_d%d", p.few ? "few" : "prompt", dsuffix(d->dtype),
-           d->head_dim <= 64 ? 64 : 128);
-  if ((rc = launch(ctx, name, dim3((unsigned)blocks, p.few ? (unsigned)p.row_tiles : 1u), dim3(256), 0, &a, stream)))
-    return rc;
+  if (p.few) {
+    snprintf(name, sizeof name, "vrs_attention_few_%s_d%d", dsuffix(d->dtype), D);
+    rc = launch(ctx, name, dim3((unsigned)blocks, (unsigned)p.row_tiles), dim3(256), 0, &a, stream);
+  } else {
+    snprintf(name, sizeof name, "vrs_attention_prompt_%s_d%d_q%d", dsuffix(d->dtype), D, p.qt);
+    rc = launch(ctx, name, dim3((unsigned)blocks), dim3(256), 0, &a, stream);
+  }
+  if (rc) return rc;
   if (p.parts == 1) return VRS_OK;
   snprintf(name, sizeof name, "vrs_attention_join_%s", dsuffix(d->dtype));
   return launch(ctx, name, dim3((unsigned)joins), dim3(256), 0, &a, stream);

@@ -22,6 +22,8 @@
 // keys, values that are not finite are staged as 0, and if there were any,
 // products of indicators add them to the queries that see them
 // (add_specials).  Keys behind a sequence's last are not read at all.
+#include <type_traits>
+
 #include "seqs.h"
 
 namespace {
@@ -74,76 +76,101 @@ __device__ __forceinline__ bool clean(u32x4_t& u) {
   return bad;
 }
 
-template <typename T, int D>
+// One wave's QT tiles of 32 queries.
+template <typename T, int D, int QT>
 struct Wave {
   using E = Elt<T>;
   using G = typename E::group;
   static constexpr int PER = 16 / (int)sizeof(T);   // elements of a chunk
-  G qf[D / 16];
-  f32x16_t o[D / 32];
-  float m, l;          // running maximum (raw scores) and this lane's share of the sum
+  G qf[QT][D / 16];
+  f32x16_t o[QT][D / 32];
+  float m[QT], l[QT];   // running maximum (raw scores) and this lane's share of the sum
+  int lim[QT];          // keys that the lane's query sees
   int l32, hh;
 
   __device__ __forceinline__ void init() {
     l32 = threadIdx.x & 31;
     hh = (threadIdx.x >> 5) & 1;
-    m = -INFINITY;
-    l = 0.f;
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
+    for (int q = 0; q < QT; ++q) {
+      m[q] = -INFINITY;
+      l[q] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[q][t][r] = 0.f;
+    }
   }
   // Q^T operand: 8 elements at s * 16 + hh * 8 of the lane's query
-  __device__ __forceinline__ void load_q(const T* q, int dim, bool ok) {
+  __device__ __forceinline__ void load_q(int t, const T* q, int dim, bool ok) {
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       const int d = s * 16 + hh * 8;
-      qf[s] = ok && d < dim ? E::load(q + d) : E::zero();
+      qf[t][s] = ok && d < dim ? E::load(q + d) : E::zero();
     }
   }
   // register r of an S^T accumulator: key of the 32
   __device__ __forceinline__ int key_of(int r) const { return (r >> 2) * 8 + hh * 4 + (r & 3); }
 
-  // running maximum and sum over NS * 32 keys starting at kc, those from lim on masked; s becomes p
-  template <int NS>
-  __device__ __forceinline__ void softmax(f32x16_t (&s)[NS], int kc, int lim, bool masked, float c) {
-    if (masked) {
+  // scores of keys from lim on become -inf
+  __device__ __forceinline__ void mask(int q, f32x16_t& s, int kc) const {
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
+    for (int r = 0; r < 16; ++r) s[r] = kc + key_of(r) < lim[q] ? s[r] : -INFINITY;
+  }
+  static __device__ __forceinline__ float top(const f32x16_t& s) {
+    float t = s[0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = kc + n * 32 + key_of(r) < lim ? s[n][r] : -INFINITY;
-    }
-    float t = -INFINITY;
+    for (int r = 1; r < 16; ++r) t = fmaxf(t, s[r]);
+    return max32(t);
+  }
+  // the running maxima follow the tile maxima t where one is exceeded by more than 2^kTau
+  __device__ __forceinline__ void follow(const float (&t)[QT], float c) {
+    bool far = false;
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t = fmaxf(t, s[n][r]);
-    t = max32(t);
-    if (__any((t - m) * c > kTau)) {
+    for (int q = 0; q < QT; ++q) far |= (t[q] - m[q]) * c > kTau;
+    if (__any(far)) {
       // (a first maximum: t - -inf; lanes without any key yet keep -inf and factor 1)
-      const float mn = fmaxf(m, t);
-      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
-      m = mn;
-      l *= alpha;
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) o[d] *= alpha;
+      for (int q = 0; q < QT; ++q) {
+        const float mn = fmaxf(m[q], t[q]);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[q] - mn) * c);
+        m[q] = mn;
+        l[q] *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) o[q][d] *= alpha;
+      }
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
+  }
+  // scores -> probabilities: packed pairs (bfloat16, l summing the rounded ones) or float32
+  struct P { uint32_t u[sizeof(T) == 2 ? 8 : 16]; };
+  __device__ __forceinline__ P probs(int q, const f32x16_t& s, float c) {
+    const float mc = m[q] == -INFINITY ? 0.f : m[q] * c;
+    P p;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+      for (int i = 0; i < 8; ++i) {
+        p.u[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, -mc)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, -mc)));
+        l[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v_t, p.u[i]),
+                                               __builtin_bit_cast(bf16x2v_t, 0x3f803f80u), l[q], false);
+      }
+    } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], c, -mc));
-        if constexpr (sizeof(T) == 4) l += s[n][r];
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mc));
+        p.u[r] = __float_as_uint(e);
+        l[q] += e;
       }
+    }
+    return p;
   }
 
   // S^T of the 32 keys from `row` of a K tile in LDS
-  __device__ __forceinline__ f32x16_t scores(const T* sK, int row) const {
-    f32x16_t s;
+  __device__ __forceinline__ void scores(const T* sK, int row, f32x16_t (&s)[QT]) const {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[q][r] = 0.f;
     const int key = row + l32, z = Lds<T, D>::kswz(key);
     const T* base = sK + key * D;
 #pragma unroll
@@ -155,9 +182,9 @@ struct Wave {
         kf.lo = *reinterpret_cast<const u32x4_t*>(base + ((4 * i + 2 * hh) ^ z) * PER);
         kf.hi = *reinterpret_cast<const u32x4_t*>(base + ((4 * i + 2 * hh + 1) ^ z) * PER);
       }
-      s = mfma32_k16(kf, qf[i], s);
+#pragma unroll
+      for (int q = 0; q < QT; ++q) s[q] = mfma32_k16(kf, qf[q][i], s[q]);
     }
-    return s;
   }
 
   // This lane's V^T operand (bfloat16) for the 16 keys from `row`, channels d * 32 + 0..31
@@ -175,68 +202,66 @@ struct Wave {
     const int key = row + key_of(r), e = d * 32 + l32;
     return sV[key * D + (((e >> 2) ^ Lds<T, D>::vswz(key)) << 2) + (e & 3)];
   }
-  // Adds what the infinities and NaN among 32 keys (rows of v, n of them, dim elements) give the
-  // queries that see them (bit r of seen: key_of(r)): for each sign, indicators of such values times
-  // indicators of seen keys.  A NaN counts as an infinity of either sign (inf - inf).  Reads memory
-  // again: rare, so small code rather than fast.
-  __device__ __forceinline__ void add_specials(const T* v, int64_t ld, int n, int dim, uint32_t seen) {
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-#pragma unroll 1
-      for (int sign = 0; sign < 2; ++sign) {
-        const float inf = sign ? -INFINITY : INFINITY;
-        f32x16_t count;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) count[r] = 0.f;
-#pragma unroll 1
-        for (int r = 0; r < 16; ++r) {
-          const int key = (r >> 2) * 8 + hh * 4 + (r & 3), e = d * 32 + l32;
-          const float x = key < n && e < dim ? E::to_f(v[key * ld + e]) : 0.f;
-          count = __builtin_amdgcn_mfma_f32_32x32x2f32(x != x || x == inf ? 1.f : 0.f, (seen >> r) & 1 ? 1.f : 0.f, count, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] += count[r] > 0.f ? inf : 0.f;
-      }
-    }
-  }
-  // registers of the 32 keys from kc that lie before lim
-  __device__ __forceinline__ uint32_t seen_mask(int kc, int lim) const {
-    uint32_t m = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) m |= kc + key_of(r) < lim ? 1u << r : 0u;
-    return m;
-  }
 
-  // O^T += V^T P^T over the 32 keys from `row` of a V tile, p their probabilities
-  __device__ __forceinline__ void pv(const T* sV, int row, const f32x16_t& p) {
+  // O^T += V^T P^T over the 32 keys from `row` of a V tile
+  __device__ __forceinline__ void pv(const T* sV, int row, const P (&p)[QT]) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        G pf;
-        pf.v = (u32x4_t){pack_bf16x2(p[8 * ks], p[8 * ks + 1]), pack_bf16x2(p[8 * ks + 2], p[8 * ks + 3]),
-                         pack_bf16x2(p[8 * ks + 4], p[8 * ks + 5]), pack_bf16x2(p[8 * ks + 6], p[8 * ks + 7])};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)    // sum of the rounded pairs
-          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v_t, (uint32_t)pf.v[j]),
-                                              __builtin_bit_cast(bf16x2v_t, 0x3f803f80u), l, false);
+      for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const G vf = vt(sV, row + ks * 16, d);
-          o[d] = mfma32_k16(vf, pf, o[d]);
+#pragma unroll
+          for (int q = 0; q < QT; ++q) {
+            G pf;
+            pf.v = (u32x4_t){p[q].u[4 * ks], p[q].u[4 * ks + 1], p[q].u[4 * ks + 2], p[q].u[4 * ks + 3]};
+            o[q][d] = mfma32_k16(vf, pf, o[q][d]);
+          }
         }
-      }
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v1(sV, row, r, d), p[r], o[d], 0, 0, 0);
+        for (int d = 0; d < D / 32; ++d) {
+          const float v = v1(sV, row, r, d);
+#pragma unroll
+          for (int q = 0; q < QT; ++q)
+            o[q][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, __uint_as_float(p[q].u[r]), o[q][d], 0, 0, 0);
+        }
     }
   }
 
+  // Adds what the infinities and NaN among the 32 keys from kc (rows of v, n of them, dim elements)
+  // give the queries that see them: for each sign, indicators of such values times indicators of
+  // seen keys.  A NaN counts as an infinity of either sign (inf - inf).  Reads memory again: rare,
+  // so small code rather than fast.
+  __device__ __forceinline__ void add_specials(const T* v, int64_t ld, int n, int dim, int kc) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+#pragma unroll 1
+        for (int sign = 0; sign < 2; ++sign) {
+          const float inf = sign ? -INFINITY : INFINITY;
+          f32x16_t count;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) count[r] = 0.f;
+#pragma unroll 1
+          for (int r = 0; r < 16; ++r) {
+            const int key = key_of(r), e = d * 32 + l32;
+            const float x = key < n && e < dim ? E::to_f(v[key * ld + e]) : 0.f;
+            count = __builtin_amdgcn_mfma_f32_32x32x2f32(x != x || x == inf ? 1.f : 0.f, kc + key < lim[q] ? 1.f : 0.f,
+                                                         count, 0, 0, 0);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[q][d][r] += count[r] > 0.f ? inf : 0.f;
+        }
+      }
+  }
+
   // O / l of the lane's query to `out` (element type), `dim` elements; no key seen: zeros
-  __device__ __forceinline__ void store(T* out, int dim, bool ok) {
-    const float lt = sum32(l);
+  __device__ __forceinline__ void store(int q, T* out, int dim, bool ok) const {
+    const float lt = sum32(l[q]);
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
@@ -244,17 +269,17 @@ struct Wave {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int e = d * 32 + g * 8 + hh * 4;
-          const f32x4_t v = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+          const f32x4_t v = {o[q][d][4 * g] * inv, o[q][d][4 * g + 1] * inv, o[q][d][4 * g + 2] * inv, o[q][d][4 * g + 3] * inv};
           if (ok && e < dim) *reinterpret_cast<f32x4_t*>(out + e) = v;
         }
       } else {
         // two quads of 4: the halves swapped so that each lane has 8 elements in a row
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
-          u32x2_t a = {pack_bf16x2(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
-                       pack_bf16x2(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv)};
-          u32x2_t b = {pack_bf16x2(o[d][4 * g + 4] * inv, o[d][4 * g + 5] * inv),
-                       pack_bf16x2(o[d][4 * g + 6] * inv, o[d][4 * g + 7] * inv)};
+          u32x2_t a = {pack_bf16x2(o[q][d][4 * g] * inv, o[q][d][4 * g + 1] * inv),
+                       pack_bf16x2(o[q][d][4 * g + 2] * inv, o[q][d][4 * g + 3] * inv)};
+          u32x2_t b = {pack_bf16x2(o[q][d][4 * g + 4] * inv, o[q][d][4 * g + 5] * inv),
+                       pack_bf16x2(o[q][d][4 * g + 6] * inv, o[q][d][4 * g + 7] * inv)};
           const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
           const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
           const int e = d * 32 + g * 8 + hh * 8;
@@ -265,15 +290,15 @@ struct Wave {
   }
 
   // the unfinished query to a workspace: O (float32), running maximum in log2 units, sum
-  __device__ __forceinline__ void store_part(float* po, float2* pml, int dim, float c, bool ok) {
-    const float lt = sum32(l);
-    if (ok && hh == 0) *pml = make_float2(m == -INFINITY ? -INFINITY : m * c, lt);
+  __device__ __forceinline__ void store_part(int q, float* po, float2* pml, int dim, float c, bool ok) const {
+    const float lt = sum32(l[q]);
+    if (ok && hh == 0) *pml = make_float2(m[q] == -INFINITY ? -INFINITY : m[q] * c, lt);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int e = d * 32 + g * 8 + hh * 4;
-        const f32x4_t v = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        const f32x4_t v = {o[q][d][4 * g], o[q][d][4 * g + 1], o[q][d][4 * g + 2], o[q][d][4 * g + 3]};
         if (ok && e < dim) *reinterpret_cast<f32x4_t*>(po + e) = v;
       }
   }
@@ -291,63 +316,109 @@ __device__ __forceinline__ void part_of(int keys, int i, int parts, int unit, in
   ke = min(keys, (int)((int64_t)tiles * (i + 1) / parts) * unit);
 }
 
+// Place of a row tile: which sequence, and which of its tiles (of BM rows; a
+// query has `group` rows, one for each head of a key head).
+struct TilePlace { int seq, tile; };
+// Up to 64 sequences: those with the most keys first, so that the last
+// workgroups to run are short ones; lane i holds sequence i, and its first id is
+// the sum of the tiles of those before it.  More: in order, sequence i's ids
+// from floor(first row / BM) + i, enough for each whatever the lengths.
+// tile < 0: the id is none's.
+template <int BM>
+__device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group, int id) {
+  if (s.n <= 64) {
+    const int i = min((int)(threadIdx.x & 63), s.n - 1);
+    const SeqSpan sp = seq_span(s, i);
+    const int tiles = (int)(((int64_t)sp.q_len * group + BM - 1) / BM), keys = sp.k_len;
+    int before = 0;
+    for (int k = 0; k < s.n; ++k) {
+      const int kk = __builtin_amdgcn_readlane(keys, k), kt = __builtin_amdgcn_readlane(tiles, k);
+      if (kk > keys || (kk == keys && k < i)) before += kt;
+    }
+    const uint64_t hit = __ballot(id >= before && id < before + tiles && (int)(threadIdx.x & 63) < s.n);
+    if (!hit) return {0, -1};
+    const int at = __builtin_ctzll(hit);
+    return {at, id - __builtin_amdgcn_readlane(before, at)};
+  }
+  auto first = [&](int i) { return (int)((int64_t)min(max(s.q_start[i], 0), s.q_rows) * group / BM) + i; };
+  if (id < first(0)) return {0, -1};
+  const int sq = find_seq(s.n, id, first);
+  return {sq, id - first(sq)};
+}
+
 // ---------------------------------------------------------------------------
-// Prompts: a workgroup of 4 waves takes 128 queries of one head, a wave 32;
-// K and V tiles are shared through LDS, double buffered, the next tile's loads
-// in flight in registers while this one is computed.
-template <typename T, int D, int KT>
+// Prompts: a workgroup of 4 waves takes 128 * QT rows, the queries of all heads
+// of one key head (neighbouring rows share a query, so causal tiles waste
+// little and the keys serve the whole group), a wave 32 * QT of them; K and V
+// tiles of KT keys are shared through LDS.
+//
+// Per 32 keys x 32 queries at D = 128 the matrix cores are busy for 512 cycles
+// of a SIMD, its exponentials and the rest of the softmax take about 300 and
+// the operand reads from LDS 512 / QT (K and V fragments serve QT query
+// tiles).  So the loop is a software pipeline: the next 32 keys' scores are
+// multiplied while these 32 keys' exponentials are taken, and P V while the
+// next maximum is.
+//
+// LDS holds three tiles: tile i + 1 is written from registers while tile i is
+// read, one barrier before tile i's last 32 keys (whose step reads tile
+// i + 1's first scores) orders both, and tile i + 2's loads are in flight.
+template <typename T, int D, int KT, int QT>
 __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
-  constexpr int NT = 256, BM = 128;
+  constexpr int NT = 256, BM = 128 * QT, NS = KT / 32;
   constexpr int CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T);
   constexpr int IT = KT * CH / NT;                 // chunks a thread stages of K, and of V
-  __shared__ __attribute__((aligned(16))) T smem[2][2][KT * D];
-  __shared__ int odd_tile[2];     // first key of the tile that a buffer holds, if it had values not finite
+  constexpr int TILE = KT * D;
+  __shared__ __attribute__((aligned(16))) T smem[3 * 2 * TILE];    // three times K, V
+  __shared__ int odd_tile[3];     // first key of the tile that a buffer holds, if it had values not finite
   const int tid = threadIdx.x, wave = tid >> 6;
-  // heads outermost: an XCD's workgroups read few heads' keys; a head's late
-  // query tiles (the longest, when causal) first
+  // key heads outermost: an XCD's workgroups read few heads' keys
   const int logical = xcd_remap(blockIdx.x, gridDim.x);
   const int part = logical % a.parts;
   const int rest = logical / a.parts;
-  const int tile_id = a.tiles - 1 - rest % a.tiles, h = rest / a.tiles;
-  // sequence i's query tiles are ids floor(q_start[i] / BM) + i + 0, 1, ...: enough
-  // ids for each whatever the lengths, so no table of tiles is needed
-  auto first = [&](int i) { return min(max(a.s.q_start[i], 0), a.s.q_rows) / BM + i; };
-  if (tile_id < first(0)) return;
-  const int sq = find_seq(a.s.n, tile_id, first);
-  const SeqSpan sp = seq_span(a.s, sq);
-  const int j0 = (tile_id - first(sq)) * BM;
-  if (j0 < 0 || j0 >= sp.q_len) return;
-  const int hk = h / (a.heads / a.kv);
+  const int hk = rest / a.tiles, group = a.heads / a.kv;
+  TilePlace at = place_tile<BM>(a.s, group, rest % a.tiles);
+  if (at.tile < 0) return;
+  const SeqSpan sp = seq_span(a.s, at.seq);
+  const int64_t rows = (int64_t)sp.q_len * group;
+  const int tiles = (int)((rows + BM - 1) / BM);
+  if (at.tile >= tiles) return;
+  const int64_t r0 = (int64_t)(tiles - 1 - at.tile) * BM;     // late rows (causal: the most keys) first
 
-  Wave<T, D> w;
+  Wave<T, D, QT> w;
   w.init();
-  const int j = j0 + wave * 32 + w.l32;
-  const bool ok = j < sp.q_len;
-  const int lim = visible(sp, min(j, sp.q_len - 1), a.causal);
-  w.load_q(static_cast<const T*>(a.q) + (int64_t)(sp.q0 + j) * a.q_ld + h * a.q_hd, a.dim, ok);
-
+  int64_t qrow[QT];
+  int head[QT];
+  bool ok[QT];
+#pragma unroll
+  for (int q = 0; q < QT; ++q) {
+    const int64_t r = r0 + wave * 32 * QT + q * 32 + w.l32;
+    ok[q] = r < rows;
+    const int j = (int)(min(r, rows - 1) / group);
+    head[q] = hk * group + (int)(min(r, rows - 1) - (int64_t)j * group);
+    qrow[q] = sp.q0 + j;
+    w.lim[q] = visible(sp, j, a.causal);
+    w.load_q(q, static_cast<const T*>(a.q) + qrow[q] * a.q_ld + head[q] * a.q_hd, a.dim, ok[q]);
+  }
   int kb, ke;
-  part_of(visible(sp, min(j0 + BM, sp.q_len) - 1, a.causal), part, a.parts, KT, kb, ke);
-  const int lim_min = __builtin_amdgcn_readfirstlane(lim), lim_max = __builtin_amdgcn_readlane(lim, 31);
+  part_of(visible(sp, (int)((min(r0 + BM, rows) - 1) / group), a.causal), part, a.parts, KT, kb, ke);
+  const int all = visible(sp, (int)(r0 / group), a.causal);   // keys that every row of the workgroup sees
 
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
   u32x4_t kr[IT], vr[IT];
   // keys past the sequence's last and elements past the head read 0
   auto load = [&](int kc) {
-    const int rows = min(KT, sp.k_lim - kc);
-    const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((rows - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
-    const auto rv = make_rsrc(vp + (int64_t)kc * a.v_ld, (int)(((rows - 1) * a.v_ld + a.dim) * (int)sizeof(T)));
+    const int n = min(KT, sp.k_lim - kc);
+    const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
+    const auto rv = make_rsrc(vp + (int64_t)kc * a.v_ld, (int)(((n - 1) * a.v_ld + a.dim) * (int)sizeof(T)));
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int it = tid + i * NT, row = it / CH, ch = it % CH;
-      const bool in = ch * PER < a.dim && row < rows;
+      const bool in = ch * PER < a.dim && row < n;
       kr[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, in ? (uint32_t)(row * (int)a.k_ld + ch * PER) * sizeof(T) : kOOB, 0, 0);
       vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, in ? (uint32_t)(row * (int)a.v_ld + ch * PER) * sizeof(T) : kOOB, 0, 0);
     }
   };
-  // keys that every query of the workgroup sees
-  const int all = visible(sp, j0, a.causal);
   auto stage = [&](int buf, int kc) {
     if (kc + KT > all) {
       bool bad = false;
@@ -355,46 +426,78 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       for (int i = 0; i < IT; ++i) bad |= clean<T>(vr[i]);
       if (bad) odd_tile[buf] = kc;
     }
+    T* sK = smem + buf * 2 * TILE;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int it = tid + i * NT, row = it / CH, ch = it % CH;
-      *reinterpret_cast<u32x4_t*>(&smem[buf][0][row * D + (ch ^ Lds<T, D>::kswz(row)) * PER]) = kr[i];
-      *reinterpret_cast<u32x4_t*>(&smem[buf][1][row * D + (ch ^ Lds<T, D>::vswz(row)) * PER]) = vr[i];
+      *reinterpret_cast<u32x4_t*>(sK + row * D + (ch ^ Lds<T, D>::kswz(row)) * PER) = kr[i];
+      *reinterpret_cast<u32x4_t*>(sK + TILE + row * D + (ch ^ Lds<T, D>::vswz(row)) * PER) = vr[i];
     }
   };
   if (kb < ke) {
+    if (tid < 3) odd_tile[tid] = -1;
     load(kb);
-    if (tid < 2) odd_tile[tid] = -1;
     __syncthreads();
     stage(0, kb);
+    if (kb + KT < ke) load(kb + KT);
     __syncthreads();
-    int buf = 0;
-    for (int kc = kb; kc < ke; kc += KT, buf ^= 1) {
-      const bool more = kc + KT < ke;
-      if (more) load(kc + KT);
-      if (kc < lim_max) {
-        const T* sK = smem[buf][0];
-        const T* sV = smem[buf][1];
-        f32x16_t s[KT / 32];
+    f32x16_t s[QT];
+    float t[QT];
+    int buf = 0, kc = kb;
+    // maximum of 32 keys' scores, of which those a query does not see are masked first
+    auto look = [&](bool masked, int key) {
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n) s[n] = w.scores(sK, n * 32);
-        w.softmax(s, kc, lim, kc + KT > lim_min, a.c);
-#pragma unroll
-        for (int n = 0; n < KT / 32; ++n) w.pv(sV, n * 32, s[n]);
-        if (odd_tile[buf] == kc)
-          for (int n = 0; n < KT; n += 32)
-            w.add_specials(vp + (int64_t)(kc + n) * a.v_ld, a.v_ld, sp.k_lim - kc - n, a.dim, w.seen_mask(kc + n, lim));
+      for (int q = 0; q < QT; ++q) {
+        if (masked) w.mask(q, s[q], key);
+        t[q] = w.top(s[q]);
       }
-      if (more) stage(buf ^ 1, kc + KT);
-      __syncthreads();
-    }
+    };
+    w.scores(smem, 0, s);
+    look(kb + KT > all, kb);
+    // TAIL: some row does not see the whole tile, or no tile follows
+    auto tile = [&](auto tail, bool more, bool next_masked) {
+      constexpr bool TAIL = decltype(tail)::value;
+      const int nbuf = buf == 2 ? 0 : buf + 1;
+      const T* sK = smem + buf * 2 * TILE;
+      if (!TAIL || more) {
+        stage(nbuf, kc + KT);
+        if (kc + 2 * KT < ke) load(kc + 2 * KT);
+      }
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const bool last = n == NS - 1;
+        w.follow(t, a.c);
+        if (last) __syncthreads();
+        f32x16_t s1[QT];
+        const bool ahead = !TAIL || !last || more;
+        if (ahead) w.scores(last ? smem + nbuf * 2 * TILE : sK, last ? 0 : (n + 1) * 32, s1);
+        typename Wave<T, D, QT>::P p[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], a.c);
+        w.pv(sK + TILE, n * 32, p);
+        if (ahead) {
+#pragma unroll
+          for (int q = 0; q < QT; ++q) s[q] = s1[q];
+          look(last ? next_masked : TAIL, kc + (n + 1) * 32);
+        }
+      }
+      if (TAIL && odd_tile[buf] == kc)
+        for (int n = 0; n < NS; ++n)
+          w.add_specials(vp + (int64_t)(kc + n * 32) * a.v_ld, a.v_ld, sp.k_lim - kc - n * 32, a.dim, kc + n * 32);
+      buf = nbuf;
+      kc += KT;
+    };
+    while (kc + 2 * KT <= all && kc + KT < ke) tile(std::false_type{}, true, false);
+    while (kc < ke) tile(std::true_type{}, kc + KT < ke, kc + 2 * KT > all);
   }
-  const int64_t row = sp.q0 + j;
-  if (a.parts == 1) {
-    w.store(static_cast<T*>(a.out) + row * a.o_ld + h * a.o_hd, a.dim, ok);
-  } else {
-    const int64_t at = ((int64_t)part * a.s.q_rows + row) * a.heads + h;
-    w.store_part(a.part_o + at * a.dim, a.part_ml + at, a.dim, a.c, ok);
+#pragma unroll
+  for (int q = 0; q < QT; ++q) {
+    if (a.parts == 1) {
+      w.store(q, static_cast<T*>(a.out) + qrow[q] * a.o_ld + head[q] * a.o_hd, a.dim, ok[q]);
+    } else {
+      const int64_t i = ((int64_t)part * a.s.q_rows + qrow[q]) * a.heads + head[q];
+      w.store_part(q, a.part_o + i * a.dim, a.part_ml + i, a.dim, a.c, ok[q]);
+    }
   }
 }
 
@@ -417,9 +520,10 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   __shared__ __attribute__((aligned(16))) char mem[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
   __shared__ float sm[4][32], sl[4][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int logical = xcd_remap(blockIdx.x, gridDim.x);
-  const int part = logical % a.parts;
-  const int rest = logical / a.parts;
+  // in the order of launch, i.e. round the XCDs: no two workgroups share keys, and
+  // sequences of different lengths spread evenly
+  const int part = blockIdx.x % a.parts;
+  const int rest = blockIdx.x / a.parts;
   const int hk = rest % a.kv, sq = rest / a.kv;
   const SeqSpan sp = seq_span(a.s, sq);
   const int G_ = a.heads / a.kv;
@@ -429,14 +533,15 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
 
   // row tiles of the sequence, one workgroup each (and more than were counted on, in turn)
   for (int64_t r0 = blockIdx.y * 32; r0 < rows; r0 += gridDim.y * 32) {
-    Wave<T, D> w;
+    Wave<T, D, 1> w;
     w.init();
     const int64_t pr = min(r0 + w.l32, rows - 1);
     const bool ok = r0 + w.l32 < rows;
     const int j = (int)(pr / G_), h = hk * G_ + (int)(pr - (int64_t)j * G_);
     const int64_t row = sp.q0 + j;
     const int lim = visible(sp, j, a.causal);
-    w.load_q(static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd, a.dim, ok);
+    w.lim[0] = lim;
+    w.load_q(0, static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd, a.dim, ok);
     const int lim_min = __builtin_amdgcn_readfirstlane(lim), lim_max = __builtin_amdgcn_readlane(lim, 31);
     int kb, ke;
     part_of(lim_max, part, a.parts, 32, kb, ke);
@@ -468,7 +573,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) s[0] = mfma32_k16(kr[i], w.qf[i], s[0]);
+      for (int i = 0; i < D / 16; ++i) s[0] = mfma32_k16(kr[i], w.qf[0][i], s[0]);
       const int at = kc;
       const bool masked = at + 32 > lim_min;
       bool bad = false;
@@ -484,16 +589,19 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
       __builtin_amdgcn_wave_barrier();     // the wave's own tile: order alone is needed
       kc += 128;
       if (kc < ke) load(kc);
-      w.softmax(s, at, lim, masked, a.c);
-      w.pv(sV, 0, s[0]);
-      if (__any(bad)) w.add_specials(vp + (int64_t)at * a.v_ld, a.v_ld, sp.k_lim - at, a.dim, w.seen_mask(at, lim));
+      if (masked) w.mask(0, s[0], at);
+      const float t[1] = {w.top(s[0])};
+      w.follow(t, a.c);
+      const typename Wave<T, D, 1>::P p[1] = {w.probs(0, s[0], a.c)};
+      w.pv(sV, 0, p);
+      if (__any(bad)) w.add_specials(vp + (int64_t)at * a.v_ld, a.v_ld, sp.k_lim - at, a.dim, at);
       __builtin_amdgcn_wave_barrier();
     }
     // join the four waves: the largest maximum, sums and O scaled to it
-    const float lt = sum32(w.l);
+    const float lt = sum32(w.l[0]);
     __syncthreads();                       // every wave is done with its V tile
     if (w.hh == 0) {
-      sm[wave][w.l32] = w.m;
+      sm[wave][w.l32] = w.m[0];
       sl[wave][w.l32] = lt;
     }
 #pragma unroll
@@ -501,7 +609,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4_t*>(&sO[(wave * 32 + w.l32) * OL + d * 32 + g * 8 + w.hh * 4]) =
-            (f32x4_t){w.o[d][4 * g], w.o[d][4 * g + 1], w.o[d][4 * g + 2], w.o[d][4 * g + 3]};
+            (f32x4_t){w.o[0][d][4 * g], w.o[0][d][4 * g + 1], w.o[0][d][4 * g + 2], w.o[0][d][4 * g + 3]};
     __syncthreads();
     // 8 threads to a row, 4 elements at a time
     const int rr = threadIdx.x >> 3, e0 = (threadIdx.x & 7) * 4;
@@ -569,16 +677,23 @@ __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
 }
 }  // namespace
 
-#define VRS_ATTENTION(TN, T, D, KT)                                                                          \
-  extern "C" __global__ __launch_bounds__(256, 2) void vrs_attention_prompt_##TN##_d##D(vrs_attention_args a) { \
-    prompt_body<T, D, KT>(a);                                                                                \
-  }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void vrs_attention_few_##TN##_d##D(vrs_attention_args a) { \
-    few_body<T, D>(a);                                                                                       \
+#define VRS_ATTENTION_PROMPT(TN, T, D, KT, QT, WGS)                                                                        \
+  extern "C" __global__ __launch_bounds__(256, WGS) void vrs_attention_prompt_##TN##_d##D##_q##QT(vrs_attention_args a) { \
+    prompt_body<T, D, KT, QT>(a);                                                                                         \
   }
-VRS_ATTENTION(bf16, bf16_t, 64, 64)
-VRS_ATTENTION(bf16, bf16_t, 128, 64)
-VRS_ATTENTION(f32, float, 64, 32)
-VRS_ATTENTION(f32, float, 128, 32)
+#define VRS_ATTENTION_FEW(TN, T, D)                                                                                           \
+  extern "C" __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void vrs_attention_few_##TN##_d##D(vrs_attention_args a) { \
+    few_body<T, D>(a);                                                                                                        \
+  }
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 1, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 1, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 2, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 2, 1)
+VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 2)
+VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 1)
+VRS_ATTENTION_FEW(bf16, bf16_t, 64)
+VRS_ATTENTION_FEW(bf16, bf16_t, 128)
+VRS_ATTENTION_FEW(f32, float, 64)
+VRS_ATTENTION_FEW(f32, float, 128)
 extern "C" __global__ __launch_bounds__(256) void vrs_attention_join_bf16(vrs_attention_args a) { join_body<bf16_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_attention_join_f32(vrs_attention_args a) { join_body<float>(a); }

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_DIR = os.path.join(PKG, "lib")
@@ -128,6 +129,12 @@ class ConvIo(C.Structure):
 
 PLAN_FP8 = 0x10000
 
+# The descriptors above as packed bytes (native alignment, the same layout).
+_RMS = struct.Struct("5i2f4q").pack
+_ROPE = struct.Struct("9i4if13q").pack
+_ATTENTION = struct.Struct("7if8q").pack
+_NONE = (0, 0, 0, 0)
+
 # Every exported symbol of include/vrs.h with its ctypes signature.
 _vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 _P = C.POINTER
@@ -160,11 +167,11 @@ SIGNATURES = {
     "vrs_detect_unletterbox": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "vrs_letterbox": (C.c_int, [_vp, _i32, _i32, _vp, _i64, _P(_i64), _P(_i32), _vp, _vp]),
     "vrs_msda": (C.c_int, [_vp, _P(MsdaDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
-    "vrs_rms_norm": (C.c_int, [_vp, _P(RmsDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_rms_norm": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vrs_rope_freqs": (C.c_int, [_i32, C.c_double, _i32, C.c_double, C.c_double, C.c_double, C.c_double, _vp]),
-    "vrs_rope": (C.c_int, [_vp, _P(RopeDesc), _P(Seqs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "vrs_attention_workspace_size": (_sz, [_P(AttentionDesc), _P(Seqs)]),
-    "vrs_attention": (C.c_int, [_vp, _P(AttentionDesc), _P(Seqs), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vrs_rope": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_attention_workspace_size": (_sz, [_vp, _vp]),
+    "vrs_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "vrs_model_create": (C.c_int, [_vp, _P(BlockDesc), _i32, _i32, _i32, _i32, _f32, _P(_vp)]),
     "vrs_model_set_autotune": (C.c_int, [_vp, _i32]),
     "vrs_model_num_params": (C.c_int, [_vp]),
@@ -279,6 +286,7 @@ def seqs(q_start, k_start=None, k_len=None, max_q=0, max_k=0):
         raise ValueError("seqs: q_start needs n + 1 elements")
     s = Seqs(_ptr(q_start), _ptr(k_start), _ptr(k_len), n, max_q, max_k)
     s.tensors = (q_start, k_start, k_len)
+    s.address = C.addressof(s)
     return s
 
 
@@ -462,22 +470,19 @@ class Context:
                                            _ptr(out), _stream(stream)))
 
     # ---- transformer layers ------------------------------------------------
-    def _rows(self, what, t, dims, dtype=None):
-        """A tensor of rows whose last dimension is contiguous, on this context's device."""
-        if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
-            raise ValueError(f"{what}: {dims} dimensions, the last one contiguous")
-        if t.device.type != "cuda" or t.device.index != self.device:
-            raise ValueError(f"{what}: on {t.device}, the context is on cuda:{self.device}")
-        if dtype is not None and t.dtype != dtype:
-            raise ValueError(f"{what}: {t.dtype}, not {dtype}")
-        return t
+    # A call's host time counts where its kernel takes a few microseconds: each
+    # tensor is looked at once, and a descriptor is packed as bytes (a fifth of
+    # the time of a ctypes structure).
+    def _strides(self, what, t, shape, dtype):
+        """Strides of a tensor that has this shape and type, lies on this context's device, and whose
+        last dimension is contiguous."""
+        st = t.stride()
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != self.device or (st[-1] != 1 and shape[-1] > 1):
+            raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} with strides {st}; needs {tuple(shape)} "
+                             f"{dtype} on cuda:{self.device} (the context's device), the last dimension contiguous")
+        return st
 
-    @staticmethod
-    def _ld(t, i):
-        """Elements between neighbours along i (of no account, then one row or head, where there is one)."""
-        return 0 if t is None else t.stride(i) if t.shape[i] > 1 else t.shape[-1]
-
-    def _stream(self, stream):
+    def _launch_stream(self, stream):
         if stream is not None:
             return stream
         import torch
@@ -489,86 +494,97 @@ class Context:
         scales None unless e4m3 with a group.  e4m3: y is uint8, on the fixed out_step (group 0) or
         with a scale for each `group` columns of a row.  y, sum, scales: outputs to write, else new."""
         import torch
-        dt = dtype_code(x.dtype)
-        self._rows("rms_norm: x", x, 2)
-        rows, cols = x.shape
-        self._rows("rms_norm: weight", weight, 1, torch.float32)
-        if weight.shape[0] != cols:
-            raise ValueError(f"rms_norm: weight of {weight.shape[0]} for {cols} columns")
-        with _alloc_on(stream, x.device):
-            if y is None:
-                y = torch.empty(rows, cols, dtype=torch.uint8 if e4m3 else x.dtype, device=x.device)
-            if res is not None and sum is None:
-                sum = torch.empty(rows, cols, dtype=x.dtype, device=x.device)
-            if e4m3 and group > 0 and scales is None:
-                scales = torch.empty(rows, cols // group, dtype=torch.float32, device=x.device)
-        for what, t, want in (("res", res, x.dtype), ("sum", sum, x.dtype), ("y", y, torch.uint8 if e4m3 else x.dtype)):
-            if t is not None and self._rows("rms_norm: " + what, t, 2, want).shape != x.shape:
-                raise ValueError(f"rms_norm: {what} of {tuple(t.shape)} for x of {tuple(x.shape)}")
-        if scales is not None and (not e4m3 or group <= 0 or not scales.is_contiguous() or
-                                   self._rows("rms_norm: scales", scales, 2, torch.float32).shape != (rows, cols // group)):
+        shape, dt, dev = x.shape, x.dtype, x.device
+        code = dtype_code(dt)
+        if len(shape) != 2:
+            raise ValueError(f"rms_norm: x of {tuple(shape)}, needs [rows, cols]")
+        rows, cols = shape
+        x_ld = self._strides("rms_norm: x", x, shape, dt)[0]
+        self._strides("rms_norm: weight", weight, shape[1:], torch.float32)
+        res_ld = 0 if res is None else self._strides("rms_norm: res", res, shape, dt)[0]
+        y_dt = torch.uint8 if e4m3 else dt
+        sum_ld = y_ld = cols
+        scaled = e4m3 and group > 0
+        if sum is not None:
+            sum_ld = self._strides("rms_norm: sum", sum, shape, dt)[0]
+        if y is not None:
+            y_ld = self._strides("rms_norm: y", y, shape, y_dt)[0]
+        if scales is not None and (not scaled or not scales.is_contiguous() or
+                                   not self._strides("rms_norm: scales", scales, (rows, cols // group), torch.float32)):
             raise ValueError("rms_norm: scales are [rows, cols / group], contiguous, for e4m3 with a group")
-        d = RmsDesc(rows, cols, dt, FP8 if e4m3 else dt, group, eps, out_step, self._ld(x, 0), self._ld(res, 0),
-                    self._ld(sum, 0), self._ld(y, 0))
-        check(lib().vrs_rms_norm(self.handle, C.byref(d), _ptr(x), _ptr(res), _ptr(weight), _ptr(sum), _ptr(y),
-                                 _ptr(scales), self._stream(stream)))
+        if rows == 1:
+            x_ld = res_ld = sum_ld = y_ld = cols     # a single row's stride is of no account
+        with _alloc_on(stream, dev):
+            if y is None:
+                y = torch.empty(shape, dtype=y_dt, device=dev)
+            if sum is None and res is not None:
+                sum = torch.empty(shape, dtype=dt, device=dev)
+            if scaled and scales is None:
+                scales = torch.empty((rows, cols // group), dtype=torch.float32, device=dev)
+        d = _RMS(rows, cols, code, FP8 if e4m3 else code, group, eps, out_step, x_ld, res_ld, sum_ld, y_ld)
+        check(lib().vrs_rms_norm(self.handle, d, _ptr(x), _ptr(res), _ptr(weight), _ptr(sum), _ptr(y), _ptr(scales),
+                                 self._launch_stream(stream)))
         return y, sum, scales
 
     def rope(self, q, k, freq, rot_dim=None, layout=ROPE_HALF, seqs=None, positions=None, axis_pairs=None, scale=1.0,
              q_out=None, k_out=None, v=None, v_out=None, stream=None):
         """vrs_rope: q [rows, heads, dim] and k [rows, kv_heads, dim] (either may be None) into q_out and
         k_out, and v as it is into v_out; freq: float64 device tensor [rot_dim / 2] (rope_freqs).
-        positions: int32 [rows] or [axes, rows]; None: the place in the sequence, or the row.
-        With seqs, k_out and v_out [rows of the cache, kv_heads, dim] receive each sequence's rows at
-        its keys' places.  q_out, k_out None: new tensors.  Returns (q_out, k_out)."""
+        positions: int32 [rows] or [axes, rows] (or more columns); None: the place in the sequence, or
+        the row.  With seqs, k_out and v_out [rows of the cache, kv_heads, dim] receive each sequence's
+        rows at its keys' places.  q_out, k_out None: new tensors.  Returns (q_out, k_out)."""
         import torch
         t0 = q if q is not None else k
-        dt = dtype_code(t0.dtype)
+        dt, dev = t0.dtype, t0.device
+        code = dtype_code(dt)
+        if t0.ndim != 3 or (k is not None and k.ndim != 3):
+            raise ValueError("rope: q and k are [rows, heads, dim]")
+        if (v is None) != (v_out is None) or (v is not None and k is None) or (q is None and q_out is not None) or \
+                (k is None and k_out is not None):
+            raise ValueError("rope: q_out goes with q, k_out with k, and v with both v_out and k")
         rows, _, dim = t0.shape
-        with _alloc_on(stream, t0.device):
-            if q is not None and q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            if k is not None and k_out is None:
-                if seqs is not None and (seqs.k_start or seqs.k_len):
-                    raise ValueError("rope: keys that move to a cache need k_out")
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        if (v is None) != (v_out is None) or (v is not None and k is None):
-            raise ValueError("rope: v, v_out and k go together")
-        ld = []
-        for what, t, n in (("q", q, rows), ("k", k, rows), ("v", v, rows), ("q_out", q_out, rows),
-                           ("k_out", k_out, None), ("v_out", v_out, None if k_out is None else k_out.shape[0])):
-            if t is None:
-                ld += [0, 0]
-                continue
-            like = q if what[0] == "q" else k
-            if like is None:
-                raise ValueError(f"rope: {what} without its input")
-            self._rows("rope: " + what, t, 3, t0.dtype)
-            if t.shape[1:] != (like.shape[1], dim) or (n is not None and t.shape[0] != n):
-                raise ValueError(f"rope: {what} of {tuple(t.shape)}")
-            ld += [self._ld(t, 0), self._ld(t, 1)]
         rot = dim if rot_dim is None else rot_dim
-        pos_ld = 0
+        heads = kv = k_out_rows = 0
+        q_ld = k_ld = v_ld = qo_ld = ko_ld = vo_ld = (dim, dim)
+        with _alloc_on(stream, dev):
+            if q is not None:
+                heads = q.shape[1]
+                q_ld = self._strides("rope: q", q, q.shape, dt)
+                if q_out is None:
+                    q_out = torch.empty(q.shape, dtype=dt, device=dev)
+                qo_ld = self._strides("rope: q_out", q_out, q.shape, dt)
+            if k is not None:
+                kv = k.shape[1]
+                k_ld = self._strides("rope: k", k, (rows, kv, dim), dt)
+                if k_out is None:
+                    if seqs is not None and (seqs.k_start or seqs.k_len):
+                        raise ValueError("rope: keys that move to a cache need k_out")
+                    k_out = torch.empty(k.shape, dtype=dt, device=dev)
+                k_out_rows = k_out.shape[0]
+                ko_ld = self._strides("rope: k_out", k_out, (k_out_rows, kv, dim), dt)
+                if v is not None:
+                    v_ld = self._strides("rope: v", v, (rows, kv, dim), dt)
+                    vo_ld = self._strides("rope: v_out", v_out, (k_out_rows, kv, dim), dt)
+        self._strides("rope: freq", freq, (rot // 2,), torch.float64)
+        axes, pos_ld = 1, 0
         if positions is not None:
-            if positions.dim() == 1:
+            if positions.ndim == 1:
                 positions = positions[None]
-            self._rows("rope: positions", positions, 2, torch.int32)
-            if positions.shape[1] < rows:
-                raise ValueError(f"rope: {positions.shape[1]} positions for {rows} rows")
-            pos_ld = positions.stride(0) if positions.shape[0] > 1 else max(rows, 1)
-        axes = 1 if positions is None else positions.shape[0]
+            axes, pos_ld = positions.shape[0], positions.stride(0)
+            self._strides("rope: positions", positions, (axes, max(rows, positions.shape[1])), torch.int32)
         per = [rot // 2] if axis_pairs is None else list(axis_pairs)
         if len(per) != axes or axes > 4:
             raise ValueError(f"rope: axis_pairs {per} for {axes} axes")
-        self._rows("rope: freq", freq, 1, torch.float64)
-        if freq.shape[0] != rot // 2:
-            raise ValueError(f"rope: {freq.shape[0]} frequencies for rot_dim {rot}")
-        d = RopeDesc(rows, 0 if k_out is None else k_out.shape[0], 0 if q is None else q.shape[1],
-                     0 if k is None else k.shape[1], dim, rot, layout, dt, axes,
-                     (C.c_int32 * 4)(*per), scale, pos_ld, *ld)
-        check(lib().vrs_rope(self.handle, C.byref(d), C.byref(seqs) if seqs is not None else None, _ptr(freq),
-                             _ptr(positions), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out),
-                             self._stream(stream)))
+        if axes == 1:
+            pos_ld = rows
+        ld = [s[i] for s in (q_ld, k_ld, v_ld, qo_ld, ko_ld, vo_ld) for i in (0, 1)]
+        if rows == 1 or heads == 1 or kv == 1 or k_out_rows == 1:     # strides along a single one are of no account
+            for i, n in enumerate((rows, heads, rows, kv, rows, kv, rows, heads, k_out_rows, kv, k_out_rows, kv)):
+                if n == 1:
+                    ld[i] = dim
+        d = _ROPE(rows, k_out_rows, heads, kv, dim, rot, layout, code, axes, *per, *_NONE[axes:], scale, pos_ld, *ld)
+        check(lib().vrs_rope(self.handle, d, None if seqs is None else seqs.address, _ptr(freq), _ptr(positions), _ptr(q),
+                             _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out), self._launch_stream(stream)))
         return q_out, k_out
 
     def attention(self, q, k, v, seqs, causal=True, scale=0.0, out=None, workspace=None, stream=None):
@@ -577,25 +593,37 @@ class Context:
         vrs_attention_workspace_size bytes, else allocated.  Returns out (rows of no sequence: as they
         were, or unset where out is new)."""
         import torch
-        dt = dtype_code(q.dtype)
-        with _alloc_on(stream, q.device):
+        dt, dev, sq, sk = q.dtype, q.device, q.shape, k.shape
+        code = dtype_code(dt)
+        if len(sq) != 3 or len(sk) != 3:
+            raise ValueError(f"attention: q {tuple(sq)}, k {tuple(sk)}; needs [rows, heads, dim]")
+        rows, heads, dim = sq
+        k_rows, kv, _ = sk
+        q_ld, q_hd, _ = self._strides("attention: q", q, sq, dt)
+        k_ld, k_hd, _ = self._strides("attention: k", k, (k_rows, kv, dim), dt)
+        v_ld, v_hd, _ = self._strides("attention: v", v, sk, dt)
+        with _alloc_on(stream, dev):
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            for what, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-                self._rows("attention: " + what, t, 3, q.dtype)
-            if k.shape != v.shape or q.shape != out.shape or k.shape[2] != q.shape[2]:
-                raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
-                                 f"out {tuple(out.shape)}")
-            d = AttentionDesc(q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], dt, int(causal), scale,
-                              *[self._ld(t, i) for t in (q, k, v, out) for i in (0, 1)])
-            need = lib().vrs_attention_workspace_size(C.byref(d), C.byref(seqs))
+                out = torch.empty(sq, dtype=dt, device=dev)
+            o_ld, o_hd, _ = self._strides("attention: out", out, sq, dt)
+            if rows == 1:           # strides along a single row or head are of no account
+                q_ld = o_ld = dim
+            if k_rows == 1:
+                k_ld = v_ld = dim
+            if heads == 1:
+                q_hd = o_hd = dim
+            if kv == 1:
+                k_hd = v_hd = dim
+            d = _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd)
+            L, s = lib(), seqs.address
             if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-                have = need
+                have = L.vrs_attention_workspace_size(d, s)
+                if have:
+                    workspace = torch.empty(have, dtype=torch.uint8, device=dev)
             else:
                 have = workspace.numel() * workspace.element_size()
-            check(lib().vrs_attention(self.handle, C.byref(d), C.byref(seqs), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                      _ptr(workspace), have, self._stream(stream)))
+            check(L.vrs_attention(self.handle, d, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                  _ptr(workspace), have, self._launch_stream(stream)))
         return out
 
     def msda(self, value, shapes, ref, off, attw, out, stream=None):
