@@ -261,7 +261,7 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
 // Which kernel, and into how many parts the keys are split.
 struct AttentionPlan {
   bool few;
-  int qt;                 // prompts: 32-row tiles of a wave; its workgroup takes 128 * qt rows
+  int qt, waves;          // prompts: 32-row tiles of a wave, waves of a workgroup
   int parts;
   int64_t row_tiles;      // few: 32-row tiles of the longest sequence; prompts: ids of row tiles
 };
@@ -271,21 +271,47 @@ AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : d->k_rows;
   AttentionPlan p;
   p.qt = 1;
+  p.waves = 4;
   p.few = mq * group <= 64;
   if (p.few) {
     p.row_tiles = (mq * group + 31) / 32;
+    // eight workgroups to a CU (two at once), of at least 256 keys each (64 tokens over 500 .. 8000 keys,
+    // 512 workgroups: 1 part 278 us, 2 246, 4 236, 8 254)
     const int64_t wgs = std::max<int64_t>(1, s->n * d->kv_heads * p.row_tiles);
-    p.parts = (int)std::clamp<int64_t>(std::min(1024 / wgs, mk / 256), 1, 64);
+    p.parts = (int)std::clamp<int64_t>(std::min(2048 / wgs, mk / 256), 1, 64);
   } else {
     // row tiles at most: whole ones of all rows and a part of one to each sequence
     auto count = [&](int64_t bm) {
       return std::min(d->q_rows * group / bm + s->n, s->n * ((mq * group + bm - 1) / bm));
     };
-    if (d->head_dim <= 64 && d->dtype == VRS_BF16 && count(256) * d->kv_heads >= 512) p.qt = 2;
-    const int64_t bm = 128 * p.qt;
+    // 256 rows to a workgroup where key tiles are many (fewer reads of them; measured at head_dim 128,
+    // causal 8192 keys: 516 us against 545; causal up to 2800 keys, where more of a tile is masked:
+    // 198 against 189) and there are such workgroups for every CU.
+    const int64_t keys = std::max<int64_t>(1, d->causal ? mk - mq / 2 : mk);    // of a row, in the mean
+    const bool f32 = d->dtype == VRS_F32, small = d->head_dim <= 64;
+    if (keys >= 2048 && count(256) * d->kv_heads >= (small ? 512 : 256)) {
+      if (!f32 && small) p.qt = 2;
+      else p.waves = 8;
+    }
+    const int64_t bm = 32 * p.qt * p.waves;
     p.row_tiles = d->q_rows * group / bm + (int64_t)s->n;
-    const int64_t wgs = std::max<int64_t>(1, count(bm) * d->kv_heads);
-    p.parts = (int)std::clamp<int64_t>(std::min(512 / wgs, mk / 512), 1, 16);
+    // Parts: CUs take whole workgroups, so few of them leave CUs idle in the last round; a CU with one
+    // workgroup of 4 waves is slower than its share of two (bfloat16: 0.6, where a wave waits for
+    // itself; float32, bound by its matrix instructions, 0.95); each part more costs its unfinished
+    // rows' way through memory, and the first a second launch.  Times in us: 32 keys of a workgroup at
+    // the rates measured, 4 TB/s, 4 us.  Measured, four pieces of 100 .. 300 queries over 2000 .. 9000
+    // keys: 1 part 207, 2 165, 3 192, 4 175; two maps of 1369 in float32: 1 101, 2 107, 3 84, 4 92.
+    const double wgs = std::max(1.0, (double)count(bm) * (double)d->kv_heads);
+    const double step = bm / 128.0 * (f32 ? (small ? 2.1 : 4.1) : (small ? 0.32 : 0.51));
+    const double alone = p.waves * p.qt > 4 ? 1.0 : f32 ? 0.95 : 0.6;
+    const double rows = (double)std::min((int64_t)d->q_rows, s->n * mq) * d->heads;
+    double best = 0;
+    for (int i = 1; i <= 16 && (i == 1 || keys / i >= 128); ++i) {
+      const double on_cu = std::ceil(wgs * i / 256.0), odd = std::fmod(on_cu, 2.0);
+      const double t = (on_cu - odd + odd / alone) * std::ceil((double)keys / i / 32.0) * step +
+                       (i > 1 ? 4.0 + 2.0 * i * rows * (d->head_dim + 2) * 4 / 4e6 : 0.0);
+      if (i == 1 || t < best) best = t, p.parts = i;
+    }
   }
   return p;
 }
@@ -347,8 +373,8 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
     snprintf(name, sizeof name, "vrs_attention_few_%s_d%d", dsuffix(d->dtype), D);
     rc = launch(ctx, name, dim3((unsigned)blocks, (unsigned)p.row_tiles), dim3(256), 0, &a, stream);
   } else {
-    snprintf(name, sizeof name, "vrs_attention_prompt_%s_d%d_q%d", dsuffix(d->dtype), D, p.qt);
-    rc = launch(ctx, name, dim3((unsigned)blocks), dim3(256), 0, &a, stream);
+    snprintf(name, sizeof name, "vrs_attention_prompt_%s_d%d_q%d_w%d", dsuffix(d->dtype), D, p.qt, p.waves);
+    rc = launch(ctx, name, dim3((unsigned)blocks), dim3(64 * p.waves), 0, &a, stream);
   }
   if (rc) return rc;
   if (p.parts == 1) return VRS_OK;

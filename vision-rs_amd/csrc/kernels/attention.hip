@@ -47,6 +47,17 @@ __device__ __forceinline__ float sum32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A buffer resource in scalar registers, and a 16-byte load of each lane straight to LDS: lane i's
+// at `to` + 16 i.  Nothing waits for it by itself: the vmcnt waits below do.
+__device__ __forceinline__ i32x4_hw lds_rsrc(const void* base, int bytes) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  return (i32x4_hw){__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff),
+                    __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+__device__ __forceinline__ void load_lds(const i32x4_hw& r, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r) : "memory", "m0");
+}
+
 // Layout of a K or V tile in LDS: rows of D elements, 16-byte chunks XORed
 // with bits of the row so that one instruction's lanes meet distinct banks
 // (64 banks of 4 bytes): K's 16-byte reads take 16 rows at one chunk; V's
@@ -316,6 +327,18 @@ __device__ __forceinline__ void part_of(int keys, int i, int parts, int unit, in
   ke = min(keys, (int)((int64_t)tiles * (i + 1) / parts) * unit);
 }
 
+// The r-th sequence by number of keys, the most first (over 64: the r-th).
+__device__ __forceinline__ int ranked_seq(const vrs_seq_args& s, int r) {
+  if (s.n == 1 || s.n > 64) return r;
+  const int i = threadIdx.x & 63;
+  const int keys = i < s.n ? seq_span(s, i).k_len : -1;
+  int rank = 0;
+  for (int k = 0; k < s.n; ++k) {
+    const int kk = __builtin_amdgcn_readlane(keys, k);
+    rank += kk > keys || (kk == keys && k < i);
+  }
+  return __builtin_ctzll(__ballot(rank == r));
+}
 // Place of a row tile: which sequence, and which of its tiles (of BM rows; a
 // query has `group` rows, one for each head of a key head).
 struct TilePlace { int seq, tile; };
@@ -362,21 +385,21 @@ __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group
 // LDS holds three tiles: tile i + 1 is written from registers while tile i is
 // read, one barrier before tile i's last 32 keys (whose step reads tile
 // i + 1's first scores) orders both, and tile i + 2's loads are in flight.
-template <typename T, int D, int KT, int QT>
+template <typename T, int D, int KT, int QT, int NW>
 __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
-  constexpr int NT = 256, BM = 128 * QT, NS = KT / 32;
+  constexpr int NT = 64 * NW, BM = 32 * NW * QT, NS = KT / 32;
   constexpr int CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T);
   constexpr int IT = KT * CH / NT;                 // chunks a thread stages of K, and of V
   constexpr int TILE = KT * D;
   __shared__ __attribute__((aligned(16))) T smem[3 * 2 * TILE];    // three times K, V
   __shared__ int odd_tile[3];     // first key of the tile that a buffer holds, if it had values not finite
   const int tid = threadIdx.x, wave = tid >> 6;
-  // key heads outermost: an XCD's workgroups read few heads' keys
-  const int logical = xcd_remap(blockIdx.x, gridDim.x);
-  const int part = logical % a.parts;
-  const int rest = logical / a.parts;
-  const int hk = rest / a.tiles, group = a.heads / a.kv;
-  TilePlace at = place_tile<BM>(a.s, group, rest % a.tiles);
+  // Key heads innermost, so that workgroups dealt round the 8 XCDs give each XCD
+  // few heads' keys (one of 8, three of 12) and as many long tiles as any other.
+  const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv;
+  const int part = rest % a.parts;
+  const int group = a.heads / a.kv;
+  const TilePlace at = place_tile<BM>(a.s, group, rest / a.parts);
   if (at.tile < 0) return;
   const SeqSpan sp = seq_span(a.s, at.seq);
   const int64_t rows = (int64_t)sp.q_len * group;
@@ -405,41 +428,55 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
 
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
-  u32x4_t kr[IT], vr[IT];
-  // keys past the sequence's last and elements past the head read 0
-  auto load = [&](int kc) {
+  // A thread's chunks of a tile, straight to LDS: one instruction of a wave fills 1 KiB in lane
+  // order, so the swizzle is in what each lane loads.  Elements past the head read nothing (they
+  // stay 0 in LDS); keys past the sequence's last leave what was there, masked and, for V, cleaned.
+  uint32_t ko[IT], vo[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int slot = (i * NW + wave) * 64 + (tid & 63), row = slot / CH, at = slot % CH;
+    const int kc = (at ^ Lds<T, D>::kswz(row)) * PER, vc = (at ^ Lds<T, D>::vswz(row)) * PER;
+    ko[i] = kc < a.dim ? (uint32_t)(row * (int)a.k_ld + kc) * (uint32_t)sizeof(T) : kOOB;
+    vo[i] = vc < a.dim ? (uint32_t)(row * (int)a.v_ld + vc) * (uint32_t)sizeof(T) : kOOB;
+  }
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem + wave * 1024);
+  auto load = [&](int buf, int kc) {
     const int n = min(KT, sp.k_lim - kc);
-    const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
-    const auto rv = make_rsrc(vp + (int64_t)kc * a.v_ld, (int)(((n - 1) * a.v_ld + a.dim) * (int)sizeof(T)));
+    const i32x4_hw rk = lds_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
+    const i32x4_hw rv = lds_rsrc(vp + (int64_t)kc * a.v_ld, (int)(((n - 1) * a.v_ld + a.dim) * (int)sizeof(T)));
+    const uint32_t to = lds0 + buf * 2 * TILE * (uint32_t)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int it = tid + i * NT, row = it / CH, ch = it % CH;
-      const bool in = ch * PER < a.dim && row < n;
-      kr[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, in ? (uint32_t)(row * (int)a.k_ld + ch * PER) * sizeof(T) : kOOB, 0, 0);
-      vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, in ? (uint32_t)(row * (int)a.v_ld + ch * PER) * sizeof(T) : kOOB, 0, 0);
-    }
+    for (int i = 0; i < IT; ++i) load_lds(rk, ko[i], to + i * NW * 1024);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) load_lds(rv, vo[i], to + TILE * (uint32_t)sizeof(T) + i * NW * 1024);
   };
-  auto stage = [&](int buf, int kc) {
-    if (kc + KT > all) {
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < IT; ++i) bad |= clean<T>(vr[i]);
-      if (bad) odd_tile[buf] = kc;
-    }
-    T* sK = smem + buf * 2 * TILE;
+  // V of a tile that some row does not see whole: values that are not finite become 0
+  auto clean_tile = [&](int buf, int kc) {
+    bool bad = false;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int it = tid + i * NT, row = it / CH, ch = it % CH;
-      *reinterpret_cast<u32x4_t*>(sK + row * D + (ch ^ Lds<T, D>::kswz(row)) * PER) = kr[i];
-      *reinterpret_cast<u32x4_t*>(sK + TILE + row * D + (ch ^ Lds<T, D>::vswz(row)) * PER) = vr[i];
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(smem + (buf * 2 + 1) * TILE) + (i * NW + wave) * 64 + (tid & 63);
+      u32x4_t u = *at;
+      if (clean<T>(u)) {
+        *at = u;
+        bad = true;
+      }
     }
+    if (bad) odd_tile[buf] = kc;
   };
   if (kb < ke) {
     if (tid < 3) odd_tile[tid] = -1;
-    load(kb);
-    __syncthreads();
-    stage(0, kb);
-    if (kb + KT < ke) load(kb + KT);
+    if (a.dim < D) {
+      for (int i = tid; i < 3 * 2 * TILE / PER; i += NT) reinterpret_cast<u32x4_t*>(smem)[i] = (u32x4_t){0, 0, 0, 0};
+      __syncthreads();
+    }
+    load(0, kb);
+    if (kb + KT < ke) {
+      load(1, kb + KT);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * IT) : "memory");   // the first tile is there
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
     __syncthreads();
     f32x16_t s[QT];
     float t[QT];
@@ -453,32 +490,33 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       }
     };
     w.scores(smem, 0, s);
-    look(kb + KT > all, kb);
-    // TAIL: some row does not see the whole tile, or no tile follows
-    auto tile = [&](auto tail, bool more, bool next_masked) {
+    look(kb + 32 > all, kb);
+    // TAIL: some row does not see the whole of this or the next tile, or no tile follows
+    auto tile = [&](auto tail, bool more) {
       constexpr bool TAIL = decltype(tail)::value;
       const int nbuf = buf == 2 ? 0 : buf + 1;
       const T* sK = smem + buf * 2 * TILE;
-      if (!TAIL || more) {
-        stage(nbuf, kc + KT);
-        if (kc + 2 * KT < ke) load(kc + 2 * KT);
-      }
+      if (TAIL && kc + KT > all) clean_tile(buf, kc);
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const bool last = n == NS - 1;
         w.follow(t, a.c);
-        if (last) __syncthreads();
+        if (last) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the next tile
+        if (last || (TAIL && kc + KT > all)) __syncthreads();
+        if (last && kc + 2 * KT < ke) load(buf == 0 ? 2 : buf - 1, kc + 2 * KT);
         f32x16_t s1[QT];
         const bool ahead = !TAIL || !last || more;
+        __builtin_amdgcn_s_setprio(1);
         if (ahead) w.scores(last ? smem + nbuf * 2 * TILE : sK, last ? 0 : (n + 1) * 32, s1);
         typename Wave<T, D, QT>::P p[QT];
 #pragma unroll
         for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], a.c);
         w.pv(sK + TILE, n * 32, p);
+        __builtin_amdgcn_s_setprio(0);
         if (ahead) {
 #pragma unroll
           for (int q = 0; q < QT; ++q) s[q] = s1[q];
-          look(last ? next_masked : TAIL, kc + (n + 1) * 32);
+          look(TAIL && kc + (n + 2) * 32 > all, kc + (n + 1) * 32);
         }
       }
       if (TAIL && odd_tile[buf] == kc)
@@ -487,8 +525,8 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       buf = nbuf;
       kc += KT;
     };
-    while (kc + 2 * KT <= all && kc + KT < ke) tile(std::false_type{}, true, false);
-    while (kc < ke) tile(std::true_type{}, kc + KT < ke, kc + 2 * KT > all);
+    while (kc + 2 * KT <= all && kc + KT < ke) tile(std::false_type{}, true);
+    while (kc < ke) tile(std::true_type{}, kc + KT < ke);
   }
 #pragma unroll
   for (int q = 0; q < QT; ++q) {
@@ -520,11 +558,10 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   __shared__ __attribute__((aligned(16))) char mem[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
   __shared__ float sm[4][32], sl[4][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // in the order of launch, i.e. round the XCDs: no two workgroups share keys, and
-  // sequences of different lengths spread evenly
-  const int part = blockIdx.x % a.parts;
-  const int rest = blockIdx.x / a.parts;
-  const int hk = rest % a.kv, sq = rest / a.kv;
+  // no two workgroups share keys: in the order of launch, round the XCDs, the
+  // sequences with the most keys first
+  const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv;
+  const int part = rest % a.parts, sq = ranked_seq(a.s, rest / a.parts);
   const SeqSpan sp = seq_span(a.s, sq);
   const int G_ = a.heads / a.kv;
   const int64_t rows = (int64_t)sp.q_len * G_;
@@ -550,21 +587,25 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
     const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
     G kr[D / 16];
     u32x4_t vr[IT];
-    auto load = [&](int kc) {
+    uint32_t ko[D / 16], vo[IT];           // offsets in a tile; elements past the head read 0
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int d = i * 16 + w.hh * 8;
+      ko[i] = d < a.dim ? (uint32_t)(w.l32 * (int)a.k_ld + d) * (uint32_t)sizeof(T) : kOOB;
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int it = lane + i * 64, r = it / CH, ch = it % CH;
+      vo[i] = ch * PER < a.dim ? (uint32_t)(r * (int)a.v_ld + ch * PER) * (uint32_t)sizeof(T) : kOOB;
+    }
+    auto load = [&](int kc) {              // keys past the sequence's last are masked, whatever they read
       const int n = min(32, sp.k_lim - kc);
       const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
       const auto rv = make_rsrc(vp + (int64_t)kc * a.v_ld, (int)(((n - 1) * a.v_ld + a.dim) * (int)sizeof(T)));
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const int d = i * 16 + w.hh * 8;
-        kr[i] = E::bload(rk, d < a.dim && w.l32 < n ? (uint32_t)(w.l32 * (int)a.k_ld + d) * sizeof(T) : kOOB, 0);
-      }
+      for (int i = 0; i < D / 16; ++i) kr[i] = E::bload(rk, ko[i], 0);
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int it = lane + i * 64, r = it / CH, ch = it % CH;
-        vr[i] = __builtin_amdgcn_raw_buffer_load_b128(
-            rv, ch * PER < a.dim && r < n ? (uint32_t)(r * (int)a.v_ld + ch * PER) * sizeof(T) : kOOB, 0, 0);
-      }
+      for (int i = 0; i < IT; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, vo[i], 0, 0);
     };
     int kc = kb + wave * 32;
     if (kc < ke) load(kc);
@@ -677,20 +718,22 @@ __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
 }
 }  // namespace
 
-#define VRS_ATTENTION_PROMPT(TN, T, D, KT, QT, WGS)                                                                        \
-  extern "C" __global__ __launch_bounds__(256, WGS) void vrs_attention_prompt_##TN##_d##D##_q##QT(vrs_attention_args a) { \
-    prompt_body<T, D, KT, QT>(a);                                                                                         \
+#define VRS_ATTENTION_PROMPT(TN, T, D, KT, QT, NW, WPS)                                                                      \
+  extern "C" __global__ __launch_bounds__(64 * NW, WPS) void vrs_attention_prompt_##TN##_d##D##_q##QT##_w##NW(vrs_attention_args a) { \
+    prompt_body<T, D, KT, QT, NW>(a);                                                                                         \
   }
 #define VRS_ATTENTION_FEW(TN, T, D)                                                                                           \
   extern "C" __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void vrs_attention_few_##TN##_d##D(vrs_attention_args a) { \
     few_body<T, D>(a);                                                                                                        \
   }
-VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 1, 2)
-VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 1, 2)
-VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 2, 2)
-VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 2, 1)
-VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 2)
-VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 1)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 1, 4, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 2, 4, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 1, 4, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 64, 1, 8, 2)
+VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 4, 2)
+VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 8, 2)
+VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 4, 2)
+VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 8, 2)
 VRS_ATTENTION_FEW(bf16, bf16_t, 64)
 VRS_ATTENTION_FEW(bf16, bf16_t, 128)
 VRS_ATTENTION_FEW(f32, float, 64)
