@@ -261,7 +261,7 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
 // Which kernel, and into how many parts the keys are split.
 struct AttentionPlan {
   bool few;
-  int qt, waves;          // prompts: 32-row tiles of a wave, waves of a workgroup
+  int qt, waves;          // 32-row tiles of a wave (prompts), waves of a workgroup
   int parts;
   int64_t row_tiles;      // few: 32-row tiles of the longest sequence; prompts: ids of row tiles
 };
@@ -275,10 +275,15 @@ AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   p.few = mq * group <= 64;
   if (p.few) {
     p.row_tiles = (mq * group + 31) / 32;
-    // eight workgroups to a CU (two at once), of at least 256 keys each (64 tokens over 500 .. 8000 keys,
-    // 512 workgroups: 1 part 278 us, 2 246, 4 236, 8 254)
+    // Workgroups of four waves, two on a CU at once: two of each wherever there are enough keys for 192
+    // a part, four parts at most beyond that, so that long and short sequences even out.  Measured in
+    // bfloat16 at head_dim 128: 64 tokens over 500 .. 8000 keys, 512 workgroups: 1 part 278 us, 2 246,
+    // 4 236, 8 254; one token, 8 key heads, 4000 keys: 192 keys a part 14.5 us, 256 16.5, 384 16.8.
     const int64_t wgs = std::max<int64_t>(1, s->n * d->kv_heads * p.row_tiles);
-    p.parts = (int)std::clamp<int64_t>(std::min(2048 / wgs, mk / 256), 1, 64);
+    p.parts = (int)std::clamp<int64_t>(std::min(std::max<int64_t>(4, 512 / wgs), mk / 192), 1, 64);
+    // short ones: eight waves and no second launch (head_dim 128, 300 keys: 9.6 us against 10.2, 700:
+    // 13.7 against 12.6; head_dim 64, 700: 8.5 against 9.5)
+    if (d->dtype == VRS_BF16 && wgs <= 256 && mk * (d->head_dim <= 64 ? 64 : 128) <= 1 << 16) p.waves = 8, p.parts = 1;
   } else {
     // row tiles at most: whole ones of all rows and a part of one to each sequence
     auto count = [&](int64_t bm) {
@@ -364,14 +369,14 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * d->head_dim);
   }
   const int64_t blocks = p.parts * (p.few ? (int64_t)seqs->n : p.row_tiles) * d->kv_heads;
-  const int64_t joins = ((int64_t)d->q_rows * d->heads + 3) / 4;
-  if (p.row_tiles >= (1ll << 31) || blocks >= (1ll << 32) / 256 || joins >= (1ll << 32) / 256)
+  const int64_t joins = ((int64_t)d->q_rows * d->heads * (d->head_dim / 4) + 255) / 256;
+  if (p.row_tiles >= (1ll << 31) || blocks >= (1ll << 32) / 512 || joins >= (1ll << 32) / 256)
     return fail(VRS_EBADSHAPE, "%s: grid too large", me);
   const int D = d->head_dim <= 64 ? 64 : 128;
   char name[64];
   if (p.few) {
-    snprintf(name, sizeof name, "vrs_attention_few_%s_d%d", dsuffix(d->dtype), D);
-    rc = launch(ctx, name, dim3((unsigned)blocks, (unsigned)p.row_tiles), dim3(256), 0, &a, stream);
+    snprintf(name, sizeof name, "vrs_attention_few_%s_d%d_w%d", dsuffix(d->dtype), D, p.waves);
+    rc = launch(ctx, name, dim3((unsigned)blocks, (unsigned)p.row_tiles), dim3(64 * p.waves), 0, &a, stream);
   } else {
     snprintf(name, sizeof name, "vrs_attention_prompt_%s_d%d_q%d_w%d", dsuffix(d->dtype), D, p.qt, p.waves);
     rc = launch(ctx, name, dim3((unsigned)blocks), dim3(64 * p.waves), 0, &a, stream);

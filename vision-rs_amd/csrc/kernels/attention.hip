@@ -480,7 +480,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
     __syncthreads();
     f32x16_t s[QT];
     float t[QT];
-    int buf = 0, kc = kb;
+    int kc = kb;
     // maximum of 32 keys' scores, of which those a query does not see are masked first
     auto look = [&](bool masked, int key) {
 #pragma unroll
@@ -492,7 +492,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
     w.scores(smem, 0, s);
     look(kb + 32 > all, kb);
     // TAIL: some row does not see the whole of this or the next tile, or no tile follows
-    auto tile = [&](auto tail, bool more) {
+    auto tile = [&](auto tail, int buf, bool more) {
       constexpr bool TAIL = decltype(tail)::value;
       const int nbuf = buf == 2 ? 0 : buf + 1;
       const T* sK = smem + buf * 2 * TILE;
@@ -522,11 +522,14 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       if (TAIL && odd_tile[buf] == kc)
         for (int n = 0; n < NS; ++n)
           w.add_specials(vp + (int64_t)(kc + n * 32) * a.v_ld, a.v_ld, sp.k_lim - kc - n * 32, a.dim, kc + n * 32);
-      buf = nbuf;
       kc += KT;
     };
-    while (kc + 2 * KT <= all && kc + KT < ke) tile(std::false_type{}, true);
-    while (kc < ke) tile(std::true_type{}, kc + KT < ke);
+    while (kc + 4 * KT <= all && kc + 3 * KT < ke) {     // three at a time: LDS addresses are constants
+      tile(std::false_type{}, 0, true);
+      tile(std::false_type{}, 1, true);
+      tile(std::false_type{}, 2, true);
+    }
+    for (int buf = 0; kc < ke; buf = buf == 2 ? 0 : buf + 1) tile(std::true_type{}, buf, kc + KT < ke);
   }
 #pragma unroll
   for (int q = 0; q < QT; ++q) {
@@ -542,21 +545,21 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
 // ---------------------------------------------------------------------------
 // Few queries to a sequence (single tokens): a workgroup takes 32 rows, the
 // queries of all heads of one key head, so that the keys are read once for
-// the group; its 4 waves take different tiles of 32 keys, each on its own (no
+// the group; its NW waves take different tiles of 32 keys, each on its own (no
 // barrier inside the loop), and join their O, m and l through LDS at the end.
 // Memory bound: K goes straight to registers in operand layout (16 bytes of a
 // row to a lane), V through a wave's own LDS tile for the transposed reads,
 // the next tile's loads in flight meanwhile.
-template <typename T, int D>
+template <typename T, int D, int NW>
 __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   using E = Elt<T>;
   using G = typename E::group;
   constexpr int CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T);
   constexpr int IT = 32 * CH / 64;                 // V chunks of a lane
   constexpr int OL = D + 4;                        // O row in LDS (float32)
-  constexpr int V_BYTES = 4 * 32 * D * (int)sizeof(T), O_BYTES = 4 * 32 * OL * 4;
+  constexpr int V_BYTES = NW * 32 * D * (int)sizeof(T), O_BYTES = NW * 32 * OL * 4;
   __shared__ __attribute__((aligned(16))) char mem[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
-  __shared__ float sm[4][32], sl[4][32];
+  __shared__ float sm[NW][32], sl[NW][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // no two workgroups share keys: in the order of launch, round the XCDs, the
   // sequences with the most keys first
@@ -628,7 +631,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
         *reinterpret_cast<u32x4_t*>(sV + r * D + (ch ^ Lds<T, D>::vswz(r)) * PER) = vr[i];
       }
       __builtin_amdgcn_wave_barrier();     // the wave's own tile: order alone is needed
-      kc += 128;
+      kc += NW * 32;
       if (kc < ke) load(kc);
       if (masked) w.mask(0, s[0], at);
       const float t[1] = {w.top(s[0])};
@@ -638,7 +641,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
       if (__any(bad)) w.add_specials(vp + (int64_t)at * a.v_ld, a.v_ld, sp.k_lim - at, a.dim, at);
       __builtin_amdgcn_wave_barrier();
     }
-    // join the four waves: the largest maximum, sums and O scaled to it
+    // join the waves: the largest maximum, sums and O scaled to it
     const float lt = sum32(w.l[0]);
     __syncthreads();                       // every wave is done with its V tile
     if (w.hh == 0) {
@@ -652,26 +655,28 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
         *reinterpret_cast<f32x4_t*>(&sO[(wave * 32 + w.l32) * OL + d * 32 + g * 8 + w.hh * 4]) =
             (f32x4_t){w.o[0][d][4 * g], w.o[0][d][4 * g + 1], w.o[0][d][4 * g + 2], w.o[0][d][4 * g + 3]};
     __syncthreads();
-    // 8 threads to a row, 4 elements at a time
-    const int rr = threadIdx.x >> 3, e0 = (threadIdx.x & 7) * 4;
+    // 2 NW threads to a row, 4 elements at a time
+    const int rr = threadIdx.x / (2 * NW), e0 = threadIdx.x % (2 * NW) * 4;
     if (r0 + rr < rows) {
       const int jj = (int)((r0 + rr) / G_), ho = hk * G_ + (int)(r0 + rr - (int64_t)jj * G_);
       const int64_t orow = sp.q0 + jj;
-      const float mx = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
-      float f[4], lsum = 0.f;
+      float mx = sm[0][rr];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {        // a wave without keys has l = 0, O = 0
+      for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sm[i][rr]);
+      float f[NW], lsum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {       // a wave without keys has l = 0, O = 0
         f[i] = sm[i][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[i][rr] - mx) * a.c);
         lsum += f[i] * sl[i][rr];
       }
       const float inv = a.parts > 1 ? 1.f : lsum == 0.f ? 0.f : 1.f / lsum;
       const int64_t at = ((int64_t)part * a.s.q_rows + orow) * a.heads + ho;
-      if (a.parts > 1 && (threadIdx.x & 7) == 0) a.part_ml[at] = make_float2(mx == -INFINITY ? mx : mx * a.c, lsum);
+      if (a.parts > 1 && e0 == 0) a.part_ml[at] = make_float2(mx == -INFINITY ? mx : mx * a.c, lsum);
       T* out = static_cast<T*>(a.out) + orow * a.o_ld + ho * a.o_hd;
-      for (int e = e0; e < a.dim; e += 32) {
+      for (int e = e0; e < a.dim; e += 8 * NW) {
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v += f[i] * *reinterpret_cast<const f32x4_t*>(&sO[(i * 32 + rr) * OL + e]);
+        for (int i = 0; i < NW; ++i) v += f[i] * *reinterpret_cast<const f32x4_t*>(&sO[(i * 32 + rr) * OL + e]);
         v *= inv;
         if (a.parts > 1) {
           *reinterpret_cast<f32x4_t*>(a.part_o + at * a.dim + e) = v;
@@ -687,31 +692,39 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
 }
 
 // ---------------------------------------------------------------------------
-// Joins the parts of the keys: a wave takes one (row, head).
+// Joins the parts of the keys: a thread takes 4 elements of one (row, head).
 template <typename T>
 __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int per = a.dim / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = t / per;
+  const int e = (int)(t - id * per) * 4;
   const int64_t row = id / a.heads;
   const int h = (int)(id - row * a.heads);
   if (row >= a.s.q_rows || row < a.s.q_start[0]) return;
-  const int sq = find_seq(a.s.n, (int)row, [&](int i) { return a.s.q_start[i]; });
+  int sq = 0;
+  for (int n = a.s.n; n > 1;) {          // the last sequence that starts at or before the row
+    const int half = n / 2;
+    if (a.s.q_start[sq + half] <= row) sq += half, n -= half;
+    else n = half;
+  }
   const SeqSpan sp = seq_span(a.s, sq);
   if (row < sp.q0 || row >= sp.q0 + sp.q_len) return;
   const int64_t step = (int64_t)a.s.q_rows * a.heads;
   float mx = -INFINITY;
+#pragma unroll 4
   for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.part_ml[p * step + id].x);
   float l = 0.f;
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-  const int e = lane * 4;
+#pragma unroll 4
   for (int p = 0; p < a.parts; ++p) {
     const float2 ml = a.part_ml[p * step + id];
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (p * step + id) * a.dim + e);
+    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);   // no key seen: l, O are 0
     l += f * ml.y;
-    if (e < a.dim) v += f * *reinterpret_cast<const f32x4_t*>(a.part_o + (p * step + id) * a.dim + e);
+    v += f * o;
   }
   v *= l == 0.f ? 0.f : 1.f / l;
-  if (e >= a.dim) return;
   T* out = static_cast<T*>(a.out) + row * a.o_ld + h * a.o_hd + e;
   if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4_t*>(out) = v;
   else *reinterpret_cast<u32x2_t*>(out) = (u32x2_t){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
@@ -722,21 +735,23 @@ __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
   extern "C" __global__ __launch_bounds__(64 * NW, WPS) void vrs_attention_prompt_##TN##_d##D##_q##QT##_w##NW(vrs_attention_args a) { \
     prompt_body<T, D, KT, QT, NW>(a);                                                                                         \
   }
-#define VRS_ATTENTION_FEW(TN, T, D)                                                                                           \
-  extern "C" __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void vrs_attention_few_##TN##_d##D(vrs_attention_args a) { \
-    few_body<T, D>(a);                                                                                                        \
+#define VRS_ATTENTION_FEW(TN, T, D, NW, WPS)                                                                               \
+  extern "C" __global__ __launch_bounds__(64 * NW, WPS) void vrs_attention_few_##TN##_d##D##_w##NW(vrs_attention_args a) { \
+    few_body<T, D, NW>(a);                                                                                                 \
   }
-VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 1, 4, 2)
+VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 32, 1, 4, 4)
 VRS_ATTENTION_PROMPT(bf16, bf16_t, 64, 64, 2, 4, 2)
 VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 32, 1, 4, 2)
 VRS_ATTENTION_PROMPT(bf16, bf16_t, 128, 64, 1, 8, 2)
-VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 4, 2)
+VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 4, 3)
 VRS_ATTENTION_PROMPT(f32, float, 64, 32, 1, 8, 2)
 VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 4, 2)
 VRS_ATTENTION_PROMPT(f32, float, 128, 32, 1, 8, 2)
-VRS_ATTENTION_FEW(bf16, bf16_t, 64)
-VRS_ATTENTION_FEW(bf16, bf16_t, 128)
-VRS_ATTENTION_FEW(f32, float, 64)
-VRS_ATTENTION_FEW(f32, float, 128)
+VRS_ATTENTION_FEW(bf16, bf16_t, 64, 4, 2)
+VRS_ATTENTION_FEW(bf16, bf16_t, 128, 4, 2)
+VRS_ATTENTION_FEW(bf16, bf16_t, 64, 8, 2)
+VRS_ATTENTION_FEW(bf16, bf16_t, 128, 8, 2)
+VRS_ATTENTION_FEW(f32, float, 64, 4, 1)
+VRS_ATTENTION_FEW(f32, float, 128, 4, 1)
 extern "C" __global__ __launch_bounds__(256) void vrs_attention_join_bf16(vrs_attention_args a) { join_body<bf16_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_attention_join_f32(vrs_attention_args a) { join_body<float>(a); }

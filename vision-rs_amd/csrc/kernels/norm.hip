@@ -101,15 +101,36 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
   const T* res = static_cast<const T*>(a.res);
   T* sum = static_cast<T*>(a.sum);
 
-  float w[NV][VEC];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  // The next row's loads are in flight while this one is reduced and stored (8192 rows of 4096 in
+  // bfloat16 with the residual: 50 us, 5.3 TB/s, against 58 without); not where 1024 threads hold a
+  // row, whose registers are full.
+  constexpr bool kAhead = TPR <= 256;
+  float w[NV][VEC];      // the weights of this thread's columns, held likewise
+  auto weight = [&](int i) {
     const int c = (i * TPR + t) * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) w[i][e] = c < a.cols ? a.weight[c + e] : 0.f;
+  };
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) weight(i);
   }
+  float nx[NV][VEC], nr[NV][VEC];
+  auto fetch = [&](int64_t r0) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (row < a.rows && c < a.cols) {
+        load_vec<T, VEC>(x + row * a.x_ld + c, nx[i]);
+        if (res) load_vec<T, VEC>(res + row * a.res_ld + c, nr[i]);
+      }
+    }
+  };
+  if constexpr (kAhead) fetch((int64_t)blockIdx.x * RPW);
   // every thread of a workgroup makes every step (the reductions of wide rows have barriers)
   for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < a.rows; r0 += (int64_t)gridDim.x * RPW) {
+    if constexpr (!kAhead) fetch(r0);
     const int64_t row = r0 + threadIdx.x / TPR;
     const bool ok = row < a.rows;
     float s[NV][VEC];
@@ -117,22 +138,14 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * VEC;
-      if (ok && c < a.cols) {
-        load_vec<T, VEC>(x + row * a.x_ld + c, s[i]);
-        if (res) {
-          float q[VEC];
-          load_vec<T, VEC>(res + row * a.res_ld + c, q);
+      const bool in = ok && c < a.cols;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) s[i][e] += q[e];
-        }
-        if (sum) store_vec<T, VEC>(sum + row * a.sum_ld + c, s[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[i][e] = 0.f;
-      }
+      for (int e = 0; e < VEC; ++e) s[i][e] = !in ? 0.f : res ? nx[i][e] + nr[i][e] : nx[i][e];
+      if (in && sum) store_vec<T, VEC>(sum + row * a.sum_ld + c, s[i]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) ss += s[i][e] * s[i][e];
     }
+    if constexpr (kAhead) fetch(r0 + (int64_t)gridDim.x * RPW);
     ss = row_reduce<float, TPR, false>(ss, lds);
     float r;
     if (ss > 1e-25f && ss < INFINITY) {
@@ -149,12 +162,14 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
     }
     float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (!kAhead) weight(i);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         s[i][e] = s[i][e] * r * w[i][e];
         if constexpr (OUT == kFp8) amax = fmaxf(amax, fabsf(s[i][e]));
       }
+    }
     if constexpr (OUT == kSame) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {

@@ -488,6 +488,14 @@ class Context:
         import torch
         return torch._C._cuda_getCurrentRawStream(self.device)
 
+    def _empty(self, stream, shape, dtype, device):
+        """A new tensor, allocated on the launch stream (see _alloc_on)."""
+        import torch
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=device)
+        with _alloc_on(stream, device):
+            return torch.empty(shape, dtype=dtype, device=device)
+
     def rms_norm(self, x, weight, eps=1e-6, res=None, sum=None, y=None, e4m3=False, group=0, out_step=0.0,
                  scales=None, stream=None):
         """vrs_rms_norm of x [rows, cols] (+ res): returns (y, sum, scales); sum None without res,
@@ -514,13 +522,12 @@ class Context:
             raise ValueError("rms_norm: scales are [rows, cols / group], contiguous, for e4m3 with a group")
         if rows == 1:
             x_ld = res_ld = sum_ld = y_ld = cols     # a single row's stride is of no account
-        with _alloc_on(stream, dev):
-            if y is None:
-                y = torch.empty(shape, dtype=y_dt, device=dev)
-            if sum is None and res is not None:
-                sum = torch.empty(shape, dtype=dt, device=dev)
-            if scaled and scales is None:
-                scales = torch.empty((rows, cols // group), dtype=torch.float32, device=dev)
+        if y is None:
+            y = self._empty(stream, shape, y_dt, dev)
+        if sum is None and res is not None:
+            sum = self._empty(stream, shape, dt, dev)
+        if scaled and scales is None:
+            scales = self._empty(stream, (rows, cols // group), torch.float32, dev)
         d = _RMS(rows, cols, code, FP8 if e4m3 else code, group, eps, out_step, x_ld, res_ld, sum_ld, y_ld)
         check(lib().vrs_rms_norm(self.handle, d, _ptr(x), _ptr(res), _ptr(weight), _ptr(sum), _ptr(y), _ptr(scales),
                                  self._launch_stream(stream)))
@@ -546,25 +553,29 @@ class Context:
         rot = dim if rot_dim is None else rot_dim
         heads = kv = k_out_rows = 0
         q_ld = k_ld = v_ld = qo_ld = ko_ld = vo_ld = (dim, dim)
-        with _alloc_on(stream, dev):
-            if q is not None:
-                heads = q.shape[1]
-                q_ld = self._strides("rope: q", q, q.shape, dt)
-                if q_out is None:
-                    q_out = torch.empty(q.shape, dtype=dt, device=dev)
-                qo_ld = self._strides("rope: q_out", q_out, q.shape, dt)
-            if k is not None:
-                kv = k.shape[1]
-                k_ld = self._strides("rope: k", k, (rows, kv, dim), dt)
-                if k_out is None:
-                    if seqs is not None and (seqs.k_start or seqs.k_len):
-                        raise ValueError("rope: keys that move to a cache need k_out")
-                    k_out = torch.empty(k.shape, dtype=dt, device=dev)
-                k_out_rows = k_out.shape[0]
-                ko_ld = self._strides("rope: k_out", k_out, (k_out_rows, kv, dim), dt)
-                if v is not None:
-                    v_ld = self._strides("rope: v", v, (rows, kv, dim), dt)
-                    vo_ld = self._strides("rope: v_out", v_out, (k_out_rows, kv, dim), dt)
+        if q is not None:
+            shape = q.shape
+            heads = shape[1]
+            q_ld = self._strides("rope: q", q, shape, dt)
+            if q_out is None:
+                q_out = self._empty(stream, shape, dt, dev)
+            qo_ld = self._strides("rope: q_out", q_out, shape, dt)
+        if k is not None:
+            kv = k.shape[1]
+            shape = (rows, kv, dim)
+            k_ld = self._strides("rope: k", k, shape, dt)
+            if k_out is None:
+                if seqs is not None and (seqs.k_start or seqs.k_len):
+                    raise ValueError("rope: keys that move to a cache need k_out")
+                k_out = self._empty(stream, shape, dt, dev)
+            out_shape = k_out.shape
+            if out_shape[1:] != shape[1:]:
+                raise ValueError(f"rope: k_out of {tuple(out_shape)} for k of {shape}")
+            k_out_rows = out_shape[0]
+            ko_ld = self._strides("rope: k_out", k_out, out_shape, dt)
+            if v is not None:
+                v_ld = self._strides("rope: v", v, shape, dt)
+                vo_ld = self._strides("rope: v_out", v_out, out_shape, dt)
         self._strides("rope: freq", freq, (rot // 2,), torch.float64)
         axes, pos_ld = 1, 0
         if positions is not None:
@@ -577,7 +588,7 @@ class Context:
             raise ValueError(f"rope: axis_pairs {per} for {axes} axes")
         if axes == 1:
             pos_ld = rows
-        ld = [s[i] for s in (q_ld, k_ld, v_ld, qo_ld, ko_ld, vo_ld) for i in (0, 1)]
+        ld = [*q_ld[:2], *k_ld[:2], *v_ld[:2], *qo_ld[:2], *ko_ld[:2], *vo_ld[:2]]
         if rows == 1 or heads == 1 or kv == 1 or k_out_rows == 1:     # strides along a single one are of no account
             for i, n in enumerate((rows, heads, rows, kv, rows, kv, rows, heads, k_out_rows, kv, k_out_rows, kv)):
                 if n == 1:
@@ -602,28 +613,27 @@ class Context:
         q_ld, q_hd, _ = self._strides("attention: q", q, sq, dt)
         k_ld, k_hd, _ = self._strides("attention: k", k, (k_rows, kv, dim), dt)
         v_ld, v_hd, _ = self._strides("attention: v", v, sk, dt)
-        with _alloc_on(stream, dev):
-            if out is None:
-                out = torch.empty(sq, dtype=dt, device=dev)
-            o_ld, o_hd, _ = self._strides("attention: out", out, sq, dt)
-            if rows == 1:           # strides along a single row or head are of no account
-                q_ld = o_ld = dim
-            if k_rows == 1:
-                k_ld = v_ld = dim
-            if heads == 1:
-                q_hd = o_hd = dim
-            if kv == 1:
-                k_hd = v_hd = dim
-            d = _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd)
-            L, s = lib(), seqs.address
-            if workspace is None:
-                have = L.vrs_attention_workspace_size(d, s)
-                if have:
-                    workspace = torch.empty(have, dtype=torch.uint8, device=dev)
-            else:
-                have = workspace.numel() * workspace.element_size()
-            check(L.vrs_attention(self.handle, d, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                  _ptr(workspace), have, self._launch_stream(stream)))
+        if out is None:
+            out = self._empty(stream, sq, dt, dev)
+        o_ld, o_hd, _ = self._strides("attention: out", out, sq, dt)
+        if rows == 1:           # strides along a single row or head are of no account
+            q_ld = o_ld = dim
+        if k_rows == 1:
+            k_ld = v_ld = dim
+        if heads == 1:
+            q_hd = o_hd = dim
+        if kv == 1:
+            k_hd = v_hd = dim
+        d = _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd)
+        L, s = lib(), seqs.address
+        if workspace is None:
+            have = L.vrs_attention_workspace_size(d, s)
+            if have:
+                workspace = self._empty(stream, (have,), torch.uint8, dev)
+        else:
+            have = workspace.numel() * workspace.element_size()
+        check(L.vrs_attention(self.handle, d, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                              _ptr(workspace), have, self._launch_stream(stream)))
         return out
 
     def msda(self, value, shapes, ref, off, attw, out, stream=None):
