@@ -357,6 +357,66 @@ def test_attention_over_a_cache(dtype, q, past):
             check_attention(([q], [past], [3]), dtype, heads, kv, dim, causal, seed=past)
 
 
+@pytest.mark.parametrize("dtype,heads,kv,dim,n,q,past,causal", [
+    ("bf16", 8, 8, 64, 4, 4200, 0, False), ("bf16", 16, 4, 64, 1, 9000, 0, True), ("bf16", 6, 2, 40, 3, 6000, 2500, True),
+    ("bf16", 8, 2, 128, 2, 4500, 0, True), ("bf16", 4, 4, 120, 2, 5000, 0, False), ("f32", 4, 4, 64, 2, 4100, 0, False),
+    ("f32", 4, 1, 128, 1, 4700, 0, True), ("f32", 16, 16, 64, 2, 4100, 0, False), ("f32", 16, 16, 128, 1, 4300, 0, True), ("bf16", 16, 16, 64, 1, 2600, 0, True), ("bf16", 8, 8, 128, 90, 300, 40, True),
+])
+def test_attention_large(dtype, heads, kv, dim, n, q, past, causal):
+    """Workgroups of 256 rows, over 64 sequences, many key tiles: rows picked from all of the output.
+    Causal: the last values of a sequence are not finite, which only its last queries see."""
+    import torch
+    rng = np.random.default_rng(q)
+    q_len = [int(v) for v in rng.integers(max(1, q - 200), q + 1, n)]
+    k_len = [a + past for a in q_len]
+    k_at = [int(v) for v in np.cumsum([0] + k_len[:-1])] if past else None
+    starts = [int(v) for v in np.cumsum([1] + q_len)]
+    rows, n_k = starts[-1] + 2, sum(k_len) + starts[-1] + 2
+    s = vrs.seqs(i32(starts), i32(k_at) if past else None, i32(k_len) if past else None, max_q=max(q_len), max_k=max(k_len))
+    qt, k, v = (randn(rows, heads, dim, dtype=dtype, seed=1, scale=2), randn(n_k, kv, dim, dtype=dtype, seed=2),
+                randn(n_k, kv, dim, dtype=dtype, seed=3))
+    at = k_at if past else starts[:-1]
+    if causal:
+        for a, m in zip(at, k_len):
+            v[a + m - 1, 0, 3], v[a + m - 2, kv - 1, 5] = math.nan, -math.inf
+    out = torch.full_like(qt, 5.0)
+    ctx().attention(qt, k, v, s, causal=causal, out=out)
+    assert torch.all(out[:1] == 5) and torch.all(out[-2:] == 5)
+    for i in sorted({0, n // 2, n - 1}):
+        for j in sorted({0, 1, 31, 32, 127, 128, 255, 256, q_len[i] // 2, q_len[i] - 1} & set(range(q_len[i]))):
+            row, keys = starts[i] + j, k_len[i] - q_len[i] + j + 1 if causal else k_len[i]
+            ref, tol = attention_ref(qt[row:row + 1], k, v, [0, 1], [keys], [at[i]], False, dim ** -0.5, out[row:row + 1], dtype)
+            inside(out[row:row + 1], ref, tol)
+
+
+def test_attention_over_its_queries():
+    """out may be q."""
+    import torch
+    for case in ("cache", ([1], [3000], [0]), ([200], [1500], [0])):
+        starts, rows, k_len, k_at, s = build(case)
+        n_k = max(rows, max(a + n for a, n in zip(k_at, k_len)))
+        q, k, v = randn(rows, 4, 64, seed=1), randn(n_k, 2, 64, seed=2), randn(n_k, 2, 64, seed=3)
+        want = ctx().attention(q, k, v, s, out=q.clone())
+        assert torch.equal(ctx().attention(q, k, v, s, out=q), want)
+
+
+def test_attention_given_workspace():
+    """A workspace of the size asked for, full of NaN; one byte less is refused."""
+    import ctypes as C
+    import torch
+    starts, rows, k_len, k_at, s = build(([1], [5000], [0]))
+    q, k, v = randn(rows, 4, 64, seed=1), randn(5001, 1, 64, seed=2), randn(5001, 1, 64, seed=3)
+    want = ctx().attention(q, k, v, s, out=torch.zeros_like(q))
+    d = vrs.AttentionDesc(rows, 5001, 4, 1, 64, vrs.BF16, 1, 0.0, 256, 64, 64, 64, 64, 64, 256, 64)
+    need = vrs.lib().vrs_attention_workspace_size(C.byref(d), s.address)
+    assert need > 0
+    ws = torch.full((need // 4,), math.nan, device="cuda").view(torch.uint8)
+    assert torch.equal(ctx().attention(q, k, v, s, out=torch.zeros_like(q), workspace=ws), want)
+    with pytest.raises(vrs.VrsError) as e:
+        ctx().attention(q, k, v, s, workspace=ws[:-16])
+    assert e.value.code == -1
+
+
 def test_attention_hints_choose_kernels_only():
     """Unknown, too small and too large hints: right results of every kernel."""
     import torch

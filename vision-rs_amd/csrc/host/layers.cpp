@@ -95,24 +95,25 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
   }
   if (d->rows == 0) return VRS_OK;
 
-  // The fewest threads that hold a row in at most four vectors each: a row
-  // up to 256 vectors (bf16 2048, float32 1024 columns) in one wave, whose
-  // sums need no barrier.
+  // The fewest threads that hold a row in at most four vectors each: a row up to 256 vectors (bf16
+  // 2048, float32 1024 columns) in one wave, whose sums need no barrier; over 1024 vectors in LDS.
   struct Shape { int tpr, nv; };
-  static const Shape kWide[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}, {1024, 8}};
-  static const Shape kOne[] = {{64, 4}, {256, 4}, {256, 16}, {1024, 32}};
+  static const Shape kWide[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {0, 0}};
+  static const Shape kOne[] = {{64, 4}, {256, 4}, {0, 0}};
   const int v = wide ? vec : 1, chunks = (d->cols + v - 1) / v;
   const Shape* sh = wide ? kWide : kOne;
-  while (sh->tpr * sh->nv < chunks) ++sh;
+  while (sh->tpr && sh->tpr * sh->nv < chunks) ++sh;
   char name[64];
-  snprintf(name, sizeof name, "vrs_rms_%s_%s_%dx%d_v%d", dsuffix(d->dtype), f8 ? "e4m3" : "same", sh->tpr, sh->nv, v);
+  const char* out = f8 ? "e4m3" : "same";
+  if (sh->tpr) snprintf(name, sizeof name, "vrs_rms_%s_%s_%dx%d_v%d", dsuffix(d->dtype), out, sh->tpr, sh->nv, v);
+  else snprintf(name, sizeof name, "vrs_rms_%s_%s_wide%dk_v%d", dsuffix(d->dtype), out, d->cols <= 16384 ? 16 : 32, v);
   vrs_rms_args a{};
   a.x = x; a.res = res; a.weight = weight; a.sum = sum; a.y = y; a.scales = scales;
   a.x_ld = d->x_ld; a.res_ld = d->res_ld; a.sum_ld = d->sum_ld; a.y_ld = d->y_ld;
   a.rows = d->rows; a.cols = d->cols; a.eps = d->eps;
   a.group = f8 ? d->group : 0;
   a.inv_step = f8 && d->group == 0 ? 1.f / d->out_step : 1.f;
-  const int wg = std::max(sh->tpr, 256), rpw = wg / sh->tpr;
+  const int wg = sh->tpr ? 256 : 1024, rpw = sh->tpr ? wg / sh->tpr : 1;
   const int64_t steps = ((int64_t)d->rows + rpw - 1) / rpw;
   const int64_t resident = 256ll * (2048 / wg);     // workgroups that fit the card at once
   return launch(ctx, name, dim3((unsigned)std::min(steps, resident)), dim3(wg), 0, &a, stream);
@@ -165,8 +166,9 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   for (int i = 0; i < d->axes; ++i) {
     if (d->axis_pairs[i] < 0) return fail(VRS_EBADSHAPE, "%s: axis_pairs", me);
     end += d->axis_pairs[i];
-    a.axis_end[i] = (int32_t)std::min<int64_t>(end, d->rot);
+    if (i < 3) a.axis_end[i] = i + 1 < d->axes ? (int32_t)std::min<int64_t>(end, d->rot) : d->rot;
   }
+  for (int i = d->axes; i < 3; ++i) a.axis_end[i] = d->rot;
   if (end != d->rot / 2) return fail(VRS_EBADSHAPE, "%s: axes of %lld pairs, rot %d", me, (long long)end, d->rot);
   const size_t es = elt_size(d->dtype);
   if ((rc = check_ptr(freq, 8, me, "freq"))) return rc;
@@ -217,20 +219,15 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   a.pos_ld = d->pos_ld;
   a.rows = d->rows; a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.rot = d->rot;
   a.pairs_layout = d->layout == VRS_ROPE_PAIRS;
-  a.axes = d->axes; a.scale = d->scale;
-  const int64_t pc = d->rot / 2 / vec, tc = (d->head_dim - d->rot) / vec;
-  const int64_t qi = d->heads * pc, qt = q == q_out ? 0 : d->heads * tc, ki = d->kv_heads * pc,
-                kt = k == k_out ? 0 : d->kv_heads * tc, vi = v ? d->kv_heads * (int64_t)(d->head_dim / vec) : 0;
-  const int64_t items = qi + qt + ki + kt + vi;
-  if (items >= (1 << 22)) return fail(VRS_EUNSUPPORTED, "%s: %lld vectors in a row", me, (long long)items);
-  a.qi = (int32_t)qi; a.qt = (int32_t)qt; a.ki = (int32_t)ki; a.kt = (int32_t)kt; a.items = (int32_t)items;
-  a.inv_items = 1.f / (float)items;
-  // four rows to a workgroup (one wave computes a row's angles) once they fill the card twice
-  const int rpw = d->rows >= 2048 ? 4 : 1;
+  a.scale = d->scale;
+  if ((int64_t)std::max(d->heads, d->kv_heads) * d->head_dim >= 1 << 24)    // the kernels' divisions are exact below
+    return fail(VRS_EUNSUPPORTED, "%s: heads of %d elements", me, d->head_dim);
+  // a wave to a row once they fill the card twice, else four
+  const int wpr = d->rows >= 2048 ? 1 : 4, rpw = 4 / wpr;
   const int64_t blocks = ((int64_t)d->rows + rpw - 1) / rpw;
   if (blocks >= (1ll << 32) / 256) return fail(VRS_EBADSHAPE, "%s: %d rows", me, d->rows);
   char name[64];
-  snprintf(name, sizeof name, "vrs_rope_%s_v%d_r%d", dsuffix(d->dtype), vec, rpw);
+  snprintf(name, sizeof name, "vrs_rope_%s_v%d_w%d", dsuffix(d->dtype), vec, wpr);
   return launch(ctx, name, dim3((unsigned)blocks), dim3(256), 0, &a, stream);
 }
 
@@ -361,7 +358,6 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
   a.v_ld = d->v_ld; a.v_hd = d->v_hd; a.o_ld = d->o_ld; a.o_hd = d->o_hd;
   a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.causal = d->causal != 0;
   a.parts = p.parts;
-  a.tiles = (int32_t)p.row_tiles;
   a.c = (float)((d->scale > 0.f ? (double)d->scale : 1.0 / std::sqrt((double)d->head_dim)) * 1.4426950408889634);
   if (need) {
     const int64_t rows = (int64_t)p.parts * d->q_rows * d->heads;

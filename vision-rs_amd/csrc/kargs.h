@@ -368,10 +368,7 @@ typedef struct {
   int64_t qo_ld, qo_hd, ko_ld, ko_hd, vo_ld, vo_hd;
   int64_t pos_ld;
   int32_t rows, heads, kv, dim, rot, pairs_layout;
-  int32_t axes, axis_end[4];   /* pairs before the end of each axis */
-  int32_t items;               /* work items of a row */
-  int32_t qi, ki, qt, kt;      /* items of q and k turns, of the unturned tails */
-  float inv_items;
+  int32_t axis_end[3];         /* pairs before the end of each axis but the last; rot where there is none */
   float scale;                 /* of cosine and sine */
 } vrs_rope_args;
 
@@ -385,7 +382,6 @@ typedef struct {
   int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd;   /* elements between rows, between heads */
   int32_t heads, kv, dim, causal;
   int32_t parts;           /* parts that a sequence's keys are split into */
-  int32_t tiles;           /* ids of query tiles (prompts) */
   float c;                 /* scale * log2(e) */
 } vrs_attention_args;
 

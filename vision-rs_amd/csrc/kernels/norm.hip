@@ -8,7 +8,10 @@
 // Memory bound: x, res read once, sum, y written once.  TPR threads hold one
 // row in registers between its two passes (sum of squares, then scaling), so
 // a row is read once; a workgroup walks rows with the weights it needs in
-// registers.  Wide rows take more threads, not more registers.
+// registers and the next row's loads in flight: 8192 rows of 4096 columns in
+// bfloat16 with the residual take 50 us, 5.4 TB/s (58 us without the loads
+// ahead; a copy moves 5.15 TB/s).  Rows too wide for that (over 1024 vectors)
+// lie in LDS as float32 between the passes, 1024 threads to a row.
 #include "common.h"
 
 namespace {
@@ -91,47 +94,62 @@ __device__ __forceinline__ V row_reduce(V v, V* lds) {
   return v;
 }
 
+// Whether a float32 sum of squares stands for its terms: neither they nor it left the type's range.
+__device__ __forceinline__ bool in_range(float ss) { return ss > 1e-25f && ss < INFINITY; }
+
+// VEC elements of a row to e4m3, on `inv` or on the scale of their group, whose lanes are
+// neighbours in a wave (all of them here, `in` or not).
+template <int VEC>
+__device__ __forceinline__ void put_fp8(const vrs_rms_args& a, int64_t row, int c, bool in, bool per_row, float inv,
+                                        const float (&y)[VEC]) {
+  if (a.group && !per_row) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = fmaxf(m, fabsf(y[e]));
+    const int lanes = a.group / VEC;
+    for (int d = 1; d < lanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    inv = m > 0.f ? kE4m3Max / m : 1.f;
+    if (in && c % a.group == 0) a.scales[row * (a.cols / a.group) + c / a.group] = m > 0.f ? m / kE4m3Max : 1.f;
+  }
+  if (in) {
+    float q[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) q[e] = y[e] * inv;
+    store_fp8<VEC>(static_cast<uint8_t*>(a.y) + row * a.y_ld + c, q);
+  }
+}
+
 template <typename T, int OUT, int TPR, int NV, int VEC>
 __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
-  constexpr int WG = TPR < 256 ? 256 : TPR, RPW = WG / TPR;   // rows per workgroup step
+  constexpr int WG = 256, RPW = WG / TPR;      // rows of a workgroup's step
   __shared__ double lds_d[WG / 64];
   float* lds = reinterpret_cast<float*>(lds_d);
   const int t = threadIdx.x % TPR;
+  const int sub = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);   // a row's threads are whole waves
   const T* x = static_cast<const T*>(a.x);
   const T* res = static_cast<const T*>(a.res);
   T* sum = static_cast<T*>(a.sum);
 
-  // The next row's loads are in flight while this one is reduced and stored (8192 rows of 4096 in
-  // bfloat16 with the residual: 50 us, 5.3 TB/s, against 58 without); not where 1024 threads hold a
-  // row, whose registers are full.
-  constexpr bool kAhead = TPR <= 256;
-  float w[NV][VEC];      // the weights of this thread's columns, held likewise
-  auto weight = [&](int i) {
+  float w[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) w[i][e] = c < a.cols ? a.weight[c + e] : 0.f;
-  };
-  if constexpr (kAhead) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) weight(i);
   }
   float nx[NV][VEC], nr[NV][VEC];
-  auto fetch = [&](int64_t r0) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (row < a.rows && c < a.cols) {
-        load_vec<T, VEC>(x + row * a.x_ld + c, nx[i]);
-        if (res) load_vec<T, VEC>(res + row * a.res_ld + c, nr[i]);
-      }
+  auto fetch = [&](int64_t row, int i, float (&fx)[VEC], float (&fr)[VEC]) {
+    const int c = (i * TPR + t) * VEC;
+    if (row < a.rows && c < a.cols) {
+      load_vec<T, VEC>(x + row * a.x_ld + c, fx);
+      if (res) load_vec<T, VEC>(res + row * a.res_ld + c, fr);
     }
   };
-  if constexpr (kAhead) fetch((int64_t)blockIdx.x * RPW);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) fetch((int64_t)blockIdx.x * RPW + sub, i, nx[i], nr[i]);
   // every thread of a workgroup makes every step (the reductions of wide rows have barriers)
   for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < a.rows; r0 += (int64_t)gridDim.x * RPW) {
-    if constexpr (!kAhead) fetch(r0);
-    const int64_t row = r0 + threadIdx.x / TPR;
+    const int64_t row = r0 + sub;
     const bool ok = row < a.rows;
     float s[NV][VEC];
     float ss = 0.f;
@@ -145,13 +163,13 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) ss += s[i][e] * s[i][e];
     }
-    if constexpr (kAhead) fetch(r0 + (int64_t)gridDim.x * RPW);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) fetch(row + (int64_t)gridDim.x * RPW, i, nx[i], nr[i]);
     ss = row_reduce<float, TPR, false>(ss, lds);
     float r;
-    if (ss > 1e-25f && ss < INFINITY) {
+    if (in_range(ss)) {
       r = 1.f / sqrtf(ss / (float)a.cols + a.eps);
-    } else {
-      // squares below or above float32's range (or a NaN): the same sum in 64 bits
+    } else {     // the same sum in 64 bits
       double sd = 0.0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -162,14 +180,12 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
     }
     float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if constexpr (!kAhead) weight(i);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         s[i][e] = s[i][e] * r * w[i][e];
         if constexpr (OUT == kFp8) amax = fmaxf(amax, fabsf(s[i][e]));
       }
-    }
     if constexpr (OUT == kSame) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -187,22 +203,82 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + t) * VEC;
-        if (a.group && !per_row) {     // lanes of one group are neighbours in a wave
-          float m = 0.f;
+        put_fp8<VEC>(a, row, c, ok && c < a.cols, per_row, inv, s[i]);
+      }
+    }
+  }
+}
+
+// Rows of up to CAP columns through LDS.
+template <typename T, int OUT, int VEC, int CAP>
+__device__ __forceinline__ void rms_wide_body(const vrs_rms_args& a) {
+  constexpr int NT = 1024;
+  __shared__ __attribute__((aligned(16))) float s[CAP];     // a thread reads what it wrote alone
+  __shared__ double lds_d[NT / 64];
+  float* lds = reinterpret_cast<float*>(lds_d);
+  const int c0 = threadIdx.x * VEC, step = NT * VEC;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+    const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_ld : nullptr;
+    T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_ld : nullptr;
+    float ss = 0.f;
+    for (int c = c0; c < a.cols; c += step) {
+      float v[VEC];
+      load_vec<T, VEC>(x + c, v);
+      if (res) {
+        float q[VEC];
+        load_vec<T, VEC>(res + c, q);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) m = fmaxf(m, fabsf(s[i][e]));
-          const int lanes = a.group / VEC;
-          for (int d = 1; d < lanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-          inv = m > 0.f ? kE4m3Max / m : 1.f;
-          if (ok && c < a.cols && c % a.group == 0)
-            a.scales[row * (a.cols / a.group) + c / a.group] = m > 0.f ? m / kE4m3Max : 1.f;
-        }
-        if (ok && c < a.cols) {
-          float q[VEC];
+        for (int e = 0; e < VEC; ++e) v[e] += q[e];
+      }
+      if (sum) store_vec<T, VEC>(sum + c, v);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) q[e] = s[i][e] * inv;
-          store_fp8<VEC>(static_cast<uint8_t*>(a.y) + row * a.y_ld + c, q);
+      for (int e = 0; e < VEC; ++e) {
+        s[c + e] = v[e];
+        ss += v[e] * v[e];
+      }
+    }
+    ss = row_reduce<float, NT, false>(ss, lds);
+    float r;
+    if (in_range(ss)) {
+      r = 1.f / sqrtf(ss / (float)a.cols + a.eps);
+    } else {     // the same sum in 64 bits
+      double sd = 0.0;
+      for (int c = c0; c < a.cols; c += step)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sd += (double)s[c + e] * (double)s[c + e];
+      sd = row_reduce<double, NT, false>(sd, lds_d);
+      r = (float)(1.0 / sqrt(sd / (double)a.cols + (double)a.eps));
+    }
+    auto value = [&](int c, float (&y)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = c < a.cols ? s[c + e] * r * a.weight[c + e] : 0.f;
+    };
+    if constexpr (OUT == kSame) {
+      for (int c = c0; c < a.cols; c += step) {
+        float y[VEC];
+        value(c, y);
+        store_vec<T, VEC>(static_cast<T*>(a.y) + row * a.y_ld + c, y);
+      }
+    } else {
+      float inv = a.inv_step;
+      const bool per_row = a.group == a.cols;
+      if (per_row) {
+        float amax = 0.f;
+        for (int c = c0; c < a.cols; c += step) {
+          float y[VEC];
+          value(c, y);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, fabsf(y[e]));
         }
+        amax = row_reduce<float, NT, true>(amax, lds);
+        inv = amax > 0.f ? kE4m3Max / amax : 1.f;
+        if (threadIdx.x == 0) a.scales[row] = amax > 0.f ? amax / kE4m3Max : 1.f;
+      }
+      for (int b = 0; b < a.cols; b += step) {     // every lane to the end: a group's lanes meet
+        float y[VEC];
+        value(b + c0, y);
+        put_fp8<VEC>(a, row, b + c0, b + c0 < a.cols, per_row, inv, y);
       }
     }
   }
@@ -210,9 +286,16 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
 }  // namespace
 
 #define VRS_RMS(TN, T, ON, OUT, TPR, NV, VEC)                                                          \
-  extern "C" __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void vrs_rms_##TN##_##ON##_##TPR##x##NV##_v##VEC( \
+  extern "C" __global__ __launch_bounds__(256) void vrs_rms_##TN##_##ON##_##TPR##x##NV##_v##VEC( \
       vrs_rms_args a) {                                                                                \
     rms_body<T, OUT, TPR, NV, VEC>(a);                                                                 \
+  }
+#define VRS_RMS_WIDE(TN, T, ON, OUT, VEC)                                                               \
+  extern "C" __global__ __launch_bounds__(1024) void vrs_rms_##TN##_##ON##_wide16k_v##VEC(vrs_rms_args a) { \
+    rms_wide_body<T, OUT, VEC, 16384>(a);                                                               \
+  }                                                                                                     \
+  extern "C" __global__ __launch_bounds__(1024) void vrs_rms_##TN##_##ON##_wide32k_v##VEC(vrs_rms_args a) { \
+    rms_wide_body<T, OUT, VEC, 32768>(a);                                                               \
   }
 #define VRS_RMS_OUT(TN, T, ON, OUT, VEC)  \
   VRS_RMS(TN, T, ON, OUT, 64, 1, VEC)     \
@@ -220,19 +303,15 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
   VRS_RMS(TN, T, ON, OUT, 64, 4, VEC)     \
   VRS_RMS(TN, T, ON, OUT, 256, 2, VEC)    \
   VRS_RMS(TN, T, ON, OUT, 256, 4, VEC)    \
-  VRS_RMS(TN, T, ON, OUT, 1024, 2, VEC)   \
-  VRS_RMS(TN, T, ON, OUT, 1024, 4, VEC)
+  VRS_RMS_WIDE(TN, T, ON, OUT, VEC)
 VRS_RMS_OUT(bf16, bf16_t, same, kSame, 8)
 VRS_RMS_OUT(bf16, bf16_t, e4m3, kFp8, 8)
 VRS_RMS_OUT(f32, float, same, kSame, 4)
 VRS_RMS_OUT(f32, float, e4m3, kFp8, 4)
-VRS_RMS(f32, float, same, kSame, 1024, 8, 4)
-VRS_RMS(f32, float, e4m3, kFp8, 1024, 8, 4)
 // rows that no 16-byte vector divides, one element at a time
 #define VRS_RMS_ONE(TN, T)                \
   VRS_RMS(TN, T, same, kSame, 64, 4, 1)   \
   VRS_RMS(TN, T, same, kSame, 256, 4, 1)  \
-  VRS_RMS(TN, T, same, kSame, 256, 16, 1) \
-  VRS_RMS(TN, T, same, kSame, 1024, 32, 1)
+  VRS_RMS_WIDE(TN, T, same, kSame, 1)
 VRS_RMS_ONE(bf16, bf16_t)
 VRS_RMS_ONE(f32, float)
