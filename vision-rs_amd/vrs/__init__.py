@@ -522,10 +522,11 @@ class Context:
             raise ValueError("rms_norm: scales are [rows, cols / group], contiguous, for e4m3 with a group")
         if rows == 1:
             x_ld = res_ld = sum_ld = y_ld = cols     # a single row's stride is of no account
+        like = stream is None and x.is_contiguous()      # half a microsecond less for each
         if y is None:
-            y = self._empty(stream, shape, y_dt, dev)
+            y = torch.empty_like(x, dtype=y_dt) if like else self._empty(stream, shape, y_dt, dev)
         if sum is None and res is not None:
-            sum = self._empty(stream, shape, dt, dev)
+            sum = torch.empty_like(x) if like else self._empty(stream, shape, dt, dev)
         if scaled and scales is None:
             scales = self._empty(stream, (rows, cols // group), torch.float32, dev)
         d = _RMS(rows, cols, code, FP8 if e4m3 else code, group, eps, out_step, x_ld, res_ld, sum_ld, y_ld)
