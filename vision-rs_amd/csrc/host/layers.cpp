@@ -115,7 +115,8 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
   a.inv_step = f8 && d->group == 0 ? 1.f / d->out_step : 1.f;
   const int wg = sh->tpr ? 256 : 1024, rpw = sh->tpr ? wg / sh->tpr : 1;
   const int64_t steps = ((int64_t)d->rows + rpw - 1) / rpw;
-  const int64_t resident = 256ll * (2048 / wg);     // workgroups that fit the card at once
+  // workgroups that walk the rows: four to a CU (8192 rows of 4096: 42.4 us; three 42.0, eight 45.3)
+  const int64_t resident = sh->tpr ? 1024 : 512;
   return launch(ctx, name, dim3((unsigned)std::min(steps, resident)), dim3(wg), 0, &a, stream);
 }
 

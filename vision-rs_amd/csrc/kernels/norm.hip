@@ -18,24 +18,23 @@ namespace {
 constexpr int kSame = 0, kFp8 = 1;
 constexpr float kE4m3Max = 448.f;
 
+// VEC elements as they lie in memory (16 bytes, or one element), and as floats.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&o)[VEC]) {
-  if constexpr (VEC == 1) {
-    o[0] = Elt<T>::to_f(*p);
-  } else {
-    static_assert(VEC * sizeof(T) == 16, "one 16-byte load");
-    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        o[i] = __uint_as_float(u[i]);
-      } else {
-        o[2 * i] = __uint_as_float(u[i] << 16);
-        o[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      }
-    }
+struct Raw {
+  static_assert(VEC * sizeof(T) == 16, "one 16-byte load");
+  u32x4_t u;
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const u32x4_t*>(p); }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[e]);
+    else return __uint_as_float((e & 1) ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
   }
-}
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ float operator[](int) const { return Elt<T>::to_f(v); }
+};
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
@@ -130,23 +129,27 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
   const T* res = static_cast<const T*>(a.res);
   T* sum = static_cast<T*>(a.sum);
 
+  // Columns past the row's end load its last ones, and rows past the last that one again, so that no
+  // load sits behind a branch; what they hold is dropped.
+  int col[NV];
   float w[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * VEC;
+    col[i] = min((i * TPR + t) * VEC, a.cols - VEC);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) w[i][e] = c < a.cols ? a.weight[c + e] : 0.f;
+    for (int e = 0; e < VEC; ++e) w[i][e] = a.weight[col[i] + e];
   }
-  float nx[NV][VEC], nr[NV][VEC];
-  auto fetch = [&](int64_t row, int i, float (&fx)[VEC], float (&fr)[VEC]) {
-    const int c = (i * TPR + t) * VEC;
-    if (row < a.rows && c < a.cols) {
-      load_vec<T, VEC>(x + row * a.x_ld + c, fx);
-      if (res) load_vec<T, VEC>(res + row * a.res_ld + c, fr);
+  Raw<T, VEC> nx[NV], nr[NV];
+  auto fetch = [&](int64_t r0) {
+    const int64_t row = min(r0 + sub, (int64_t)a.rows - 1);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) nx[i].load(x + row * a.x_ld + col[i]);
+    if (res) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) nr[i].load(res + row * a.res_ld + col[i]);
     }
   };
-#pragma unroll
-  for (int i = 0; i < NV; ++i) fetch((int64_t)blockIdx.x * RPW + sub, i, nx[i], nr[i]);
+  fetch((int64_t)blockIdx.x * RPW);
   // every thread of a workgroup makes every step (the reductions of wide rows have barriers)
   for (int64_t r0 = (int64_t)blockIdx.x * RPW; r0 < a.rows; r0 += (int64_t)gridDim.x * RPW) {
     const int64_t row = r0 + sub;
@@ -163,8 +166,7 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) ss += s[i][e] * s[i][e];
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) fetch(row + (int64_t)gridDim.x * RPW, i, nx[i], nr[i]);
+    if (r0 + (int64_t)gridDim.x * RPW < a.rows) fetch(r0 + (int64_t)gridDim.x * RPW);
     ss = row_reduce<float, TPR, false>(ss, lds);
     float r;
     if (in_range(ss)) {
@@ -224,12 +226,14 @@ __device__ __forceinline__ void rms_wide_body(const vrs_rms_args& a) {
     float ss = 0.f;
     for (int c = c0; c < a.cols; c += step) {
       float v[VEC];
-      load_vec<T, VEC>(x + c, v);
-      if (res) {
-        float q[VEC];
-        load_vec<T, VEC>(res + c, q);
+      Raw<T, VEC> u;
+      u.load(x + c);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] += q[e];
+      for (int e = 0; e < VEC; ++e) v[e] = u[e];
+      if (res) {
+        u.load(res + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] += u[e];
       }
       if (sum) store_vec<T, VEC>(sum + c, v);
 #pragma unroll
