@@ -1,5 +1,6 @@
 /*
- * vrs.h -- C ABI of the MI355X-native (gfx950) YOLO26 inference hot path.
+ * vrs.h -- C ABI of the MI355X-native (gfx950) YOLO26 inference hot path, and
+ * of the operators of transformer layers that run beside it.
  *
  * Drop-in boundary for spinorml/vision-rs.  The reference builds YOLO26 as a
  * symbolic graph from layer closures (src/models/yolo/yolo26/mod.rs:207-219

@@ -6,9 +6,12 @@
 // to float32: exact for any 32-bit position) and read from LDS by all heads.
 //
 // Memory bound: q, k (and v on its way into a cache) read and written once.
-// WPR waves take a row: they compute its angles into LDS, then walk its heads,
-// kBatch vectors (or pairs of them) of a thread at a time, all of a batch's
-// loads before its stores.  Many rows: a wave to a row, no barrier.
+// WPR waves take a row: they load q's first vectors, compute the row's angles
+// into LDS meanwhile, then walk its heads, kBatch vectors (or pairs of them) of
+// a thread at a time, all of a batch's loads before its stores.  Many rows: a
+// wave to a row, no barrier.  7283 rows of 32 + 8 heads of 128 and 8 of values
+// into a cache in bfloat16, 179 MB: 38 us, 4.7 TB/s (42 us with the angles
+// first and a barrier for four rows).
 #include "seqs.h"
 
 namespace {
