@@ -424,8 +424,9 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
  * as many keys as queries.  All three are DEVICE arrays, read by the kernels
  * (so a captured graph follows their values); what they say outside the
  * buffers is cut off, never read or written.
- * max_q, max_k: the most queries and keys of a sequence, 0 if unknown; they
- * choose among kernels, and any value gives right results. */
+ * max_q, max_k: the most queries and keys of a sequence, 0 if unknown (taken
+ * as if all were of one length); they choose among kernels for speed, and any
+ * value gives right results. */
 typedef struct {
   const int32_t* q_start;  /* [n + 1] */
   const int32_t* k_start;  /* [n] or NULL */

@@ -400,6 +400,24 @@ def test_attention_over_its_queries():
         assert torch.equal(ctx().attention(q, k, v, s, out=q), want)
 
 
+def test_nothing_to_do():
+    """No rows, no sequences, no keys."""
+    import torch
+    w = torch.ones(64, device="cuda")
+    y, s_, _ = ctx().rms_norm(randn(0, 64), w, res=randn(0, 64))
+    assert y.shape == s_.shape == (0, 64)
+    freq = vrs.rope_freqs(32).cuda()
+    assert ctx().rope(randn(0, 2, 64), randn(0, 1, 64), freq)[0].shape == (0, 2, 64)
+    q, k = randn(5, 2, 64, seed=1), randn(4, 1, 64, seed=2)
+    for s in (vrs.seqs(i32([0])), vrs.seqs(i32([0, 0, 0])), vrs.seqs(i32([5, 5]), i32([0]), i32([3]))):
+        out = ctx().attention(q, k, k, s, out=torch.full_like(q, 5.0))
+        assert torch.all(out == 5)
+    for max_q in (0, 5, 1000):
+        s = vrs.seqs(i32([1, 4]), i32([0]), i32([0]), max_q=max_q, max_k=0)
+        out = ctx().attention(q, k[:0], k[:0], s, out=torch.full_like(q, 5.0))
+        assert torch.all(out[1:4] == 0) and torch.all(out[0] == 5) and torch.all(out[4] == 5)
+
+
 def test_attention_given_workspace():
     """A workspace of the size asked for, full of NaN; one byte less is refused."""
     import ctypes as C

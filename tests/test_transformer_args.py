@@ -33,7 +33,7 @@ def rms(ctx, x=FAKE, res=None, w=FAKE, s=None, y=2 * FAKE, scales=None, **kw):
     (-1, dict(x=None)), (-1, dict(w=None)), (-1, dict(y=None)),
     (-3, dict(dtype=7)), (-3, dict(y_dtype=vrs.F32)), (-2, dict(rows=-1)), (-2, dict(cols=0)),
     (-3, dict(cols=32769, x_ld=40000, y_ld=40000)), (-1, dict(eps=0.0)), (-1, dict(eps=-1.0)), (-1, dict(eps=math.nan)),
-    (-2, dict(y_ld=63)), (-2, dict(x_ld=-64)), (-2, dict(s=3 * FAKE, sum_ld=8)), (-2, dict(x=FAKE + 1)),
+    (-2, dict(y_ld=63)), (-2, dict(x_ld=-64)), (-2, dict(x_ld=1 << 41)), (-2, dict(s=3 * FAKE, sum_ld=8)), (-2, dict(x=FAKE + 1)),
     (-1, dict(s=2 * FAKE)), (-2, dict(y=FAKE, y_ld=128)), (-1, dict(group=32)),
     # e4m3
     (-1, dict(y_dtype=vrs.FP8)), (-1, dict(y_dtype=vrs.FP8, out_step=0.3)), (-1, dict(y_dtype=vrs.FP8, out_step=-1.0)),
@@ -49,6 +49,7 @@ def test_rms_norm_refuses(ctx, code, kw):
 
 def test_rms_norm_of_no_rows_is_nothing(ctx):
     assert rms(ctx, rows=0)[0] == 0
+    assert rms(ctx, rows=0, x=None, y=None)[0] == 0          # an empty tensor's address
     assert vrs.lib().vrs_rms_norm(None, None, None, None, None, None, None, None, None) == -1
 
 
@@ -76,6 +77,7 @@ MOVED = vrs.Seqs(FAKE, FAKE, FAKE, 1, 0, 0)
     (-2, dict(axes=2, pos=FAKE, axis_pairs=(16, 15, 0, 0))), (-2, dict(axes=2, pos=FAKE, axis_pairs=(33, -1, 0, 0))),
     (-2, dict(pos=FAKE, pos_ld=3)), (-2, dict(pos=FAKE + 1)), (-2, dict(k_out_rows=3)), (-2, dict(q_ld=-1)),
     (-2, dict(qo_ld=32)), (-2, dict(qo_hd=0)), (-2, dict(ko_ld=0)), (-2, dict(qo=FAKE, q_ld=256)),
+    (-2, dict(qo_ld=64)), (-2, dict(qo_hd=32)), (-2, dict(q_hd=1 << 41)),
     (-2, dict(ko=2 * FAKE, seqs=MOVED)), (-1, dict(v=5 * FAKE)), (-1, dict(v=5 * FAKE, vo=5 * FAKE)),
     (-1, dict(kv_heads=0, v=5 * FAKE, vo=6 * FAKE)), (-1, dict(seqs=vrs.Seqs(None, None, None, 1, 0, 0))),
     (-2, dict(seqs=vrs.Seqs(FAKE, None, None, -1, 0, 0))), (-2, dict(head_dim=5000)), (-2, dict(head_dim=1024, rot=514)),
@@ -87,6 +89,7 @@ def test_rope_refuses(ctx, code, kw):
 
 def test_rope_of_no_rows_is_nothing(ctx):
     assert rope(ctx, rows=0)[0] == 0
+    assert rope(ctx, rows=0, q=None, k=None, qo=None, ko=None)[0] == 0
     assert rope(ctx, seqs=vrs.Seqs(FAKE, FAKE, FAKE, 0, 0, 0))[0] == 0
 
 
@@ -145,7 +148,8 @@ BIG = dict(q_rows=1, k_rows=10000, seqs=vrs.Seqs(FAKE, FAKE, FAKE, 1, 1, 10000))
     (-3, dict(head_dim=136)), (-2, dict(heads=3, kv_heads=2)), (-2, dict(heads=0)), (-2, dict(kv_heads=0)),
     (-2, dict(q_rows=-1)), (-2, dict(k_rows=-1)), (-1, dict(scale=-0.5)), (-1, dict(scale=math.nan)),
     (-1, dict(scale=math.inf)), (-2, dict(q_ld=132)), (-2, dict(k_hd=60)), (-2, dict(v_ld=-64)),
-    (-3, dict(k_ld=1 << 22)), (-2, dict(o_ld=32)), (-2, dict(o_hd=0)), (-1, dict(out=2 * FAKE)), (-1, dict(out=3 * FAKE)),
+    (-3, dict(k_ld=1 << 22)), (-2, dict(o_ld=32)), (-2, dict(o_hd=0)), (-2, dict(o_ld=64)),
+    (-2, dict(q_hd=1 << 41)), (-1, dict(out=2 * FAKE)), (-1, dict(out=3 * FAKE)),
     (-1, dict(out=FAKE, q_ld=256)), (-1, dict(seqs=vrs.Seqs(None, None, None, 1, 0, 0))),
     (-2, dict(seqs=vrs.Seqs(FAKE, None, None, -1, 0, 0))), (-1, dict(seqs=vrs.Seqs(FAKE, None, None, 1, -1, 0))),
     (-1, dict(BIG)), (-1, dict(BIG, ws=FAKE, ws_bytes=100)), (-1, dict(BIG, ws=FAKE + 4, ws_bytes=1 << 30)),
@@ -157,6 +161,7 @@ def test_attention_refuses(ctx, code, kw):
 
 def test_attention_of_nothing_is_nothing(ctx):
     assert attention(ctx, q_rows=0)[0] == 0
+    assert attention(ctx, q_rows=0, q=None, out=None)[0] == 0
     assert attention(ctx, seqs=vrs.Seqs(FAKE, None, None, 0, 0, 0))[0] == 0
 
 
@@ -174,6 +179,17 @@ def test_wrappers_check_tensors():
         c.rms_norm(x.half(), torch.ones(64))
     i = torch.zeros(3, dtype=torch.int32)
     assert vrs.seqs(i).n == 2
+    c.device = -1                      # stands for a context on the tensors' device, then for another
+    t = torch.zeros(2, 1, 64)
+    s = vrs.seqs(i)
+    assert c._seqs("x", s) == s.address
+    c.device = 0
+    with pytest.raises(ValueError, match="context's device"):
+        c._seqs("x", s)
+    with pytest.raises(ValueError, match="context's device"):
+        c.attention(t, t, t, s)
+    with pytest.raises(ValueError, match="context's device"):
+        c.rope(t, t, torch.zeros(32, dtype=torch.float64))
     for bad in ((i.long(),), (i[:0],), (i, i), (i, i[:2], i), (torch.zeros(6, dtype=torch.int32)[::2],)):
         with pytest.raises(ValueError):
             vrs.seqs(*bad)

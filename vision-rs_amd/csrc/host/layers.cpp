@@ -27,6 +27,15 @@ int check_ptr(const void* p, size_t es, const char* what, const char* name) {
   return VRS_OK;
 }
 
+// Whether no two (row, head) of an output share an element: heads inside a row's stride, or rows
+// inside a head's.
+bool apart(int64_t ld, int64_t hd, int64_t rows, int64_t heads, int64_t dim) {
+  if (rows <= 1 && heads <= 1) return true;
+  if (rows <= 1) return hd >= dim;
+  if (heads <= 1) return ld >= dim;
+  return (hd >= dim && ld >= (heads - 1) * hd + dim) || (ld >= dim && hd >= (rows - 1) * ld + dim);
+}
+
 int check_seqs(const vrs_seqs* s, const char* what) {
   if (s->n < 0) return fail(VRS_EBADSHAPE, "%s: %d sequences", what, s->n);
   if (!s->q_start) return fail(VRS_EINVAL, "%s: null q_start", what);
@@ -60,6 +69,7 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
   if (d->rows < 0 || d->cols < 1) return fail(VRS_EBADSHAPE, "%s: %d rows of %d columns", me, d->rows, d->cols);
   if (d->cols > 32768) return fail(VRS_EUNSUPPORTED, "%s: %d columns (up to 32768)", me, d->cols);
   if (!(d->eps > 0.f) || std::isinf(d->eps)) return fail(VRS_EINVAL, "%s: eps %g", me, (double)d->eps);
+  if (d->rows == 0) return VRS_OK;      // empty tensors may have null addresses
   const size_t es = elt_size(d->dtype);
   if ((rc = check_ptr(x, es, me, "x")) || (rc = check_ptr(weight, 4, me, "weight")) ||
       (rc = check_ptr(y, f8 ? 1 : es, me, "y")))
@@ -68,7 +78,9 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
   if (sum == y) return fail(VRS_EINVAL, "%s: sum and y are one buffer", me);
   if (f8 && (x == y || res == y)) return fail(VRS_EINVAL, "%s: an e4m3 y over an input", me);
   // outputs must not fold rows onto each other; inputs may (a stride of 0 repeats a row)
-  if (d->x_ld < 0 || (res && d->res_ld < 0) || d->y_ld < d->cols || (sum && d->sum_ld < d->cols))
+  for (int64_t s : {d->x_ld, d->res_ld, d->sum_ld, d->y_ld})
+    if (s < 0 || s >> 40) return fail(VRS_EBADSHAPE, "%s: row stride %lld", me, (long long)s);
+  if (d->y_ld < d->cols || (sum && d->sum_ld < d->cols))
     return fail(VRS_EBADSHAPE, "%s: row strides", me);
   for (const auto& [p, ld, name] : {std::tuple<const void*, int64_t, const char*>{x, d->x_ld, "x"}, {res, d->res_ld, "res"}})
     if (p && ((p == y && ld != d->y_ld) || (p == sum && ld != d->sum_ld)))
@@ -93,7 +105,6 @@ int vrs_rms_norm(vrs_ctx* ctx, const vrs_rms_desc* d, const void* x, const void*
     if (d->group) return fail(VRS_EINVAL, "%s: group %d without VRS_FP8", me, d->group);
     wide = wide && fits(y, d->y_ld);
   }
-  if (d->rows == 0) return VRS_OK;
 
   // The fewest threads that hold a row in at most four vectors each: a row up to 256 vectors (bf16
   // 2048, float32 1024 columns) in one wave, whose sums need no barrier; over 1024 vectors in LDS.
@@ -171,6 +182,8 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   }
   for (int i = d->axes; i < 3; ++i) a.axis_end[i] = d->rot;
   if (end != d->rot / 2) return fail(VRS_EBADSHAPE, "%s: axes of %lld pairs, rot %d", me, (long long)end, d->rot);
+  if (seqs && (rc = check_seqs(seqs, me))) return rc;
+  if (d->rows == 0 || (seqs && seqs->n == 0)) return VRS_OK;      // empty tensors may have null addresses
   const size_t es = elt_size(d->dtype);
   if ((rc = check_ptr(freq, 8, me, "freq"))) return rc;
   if (positions && (rc = check_ptr(positions, 4, me, "positions"))) return rc;
@@ -179,17 +192,14 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   if (d->kv_heads && ((rc = check_ptr(k, es, me, "k")) || (rc = check_ptr(k_out, es, me, "k_out")))) return rc;
   if (v && (!d->kv_heads || (rc = check_ptr(v, es, me, "v")) || (rc = check_ptr(v_out, es, me, "v_out"))))
     return rc ? rc : fail(VRS_EINVAL, "%s: v without kv_heads", me);
-  if (seqs && (rc = check_seqs(seqs, me))) return rc;
   if (d->kv_heads && !seqs && d->k_out_rows < d->rows)
     return fail(VRS_EBADSHAPE, "%s: %d rows into k_out's %d", me, d->rows, d->k_out_rows);
-  const int64_t in_ld[] = {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd};
-  for (int64_t s : in_ld)
-    if (s < 0) return fail(VRS_EBADSHAPE, "%s: negative stride", me);
-  auto out_ok = [&](int64_t ld, int64_t hd, int heads) {
-    return (ld >= d->head_dim || ld == 0) && (hd >= d->head_dim || heads == 1) && (ld > 0 || d->rows <= 1);
-  };
-  if ((d->heads && !out_ok(d->qo_ld, d->qo_hd, d->heads)) || (d->kv_heads && !out_ok(d->ko_ld, d->ko_hd, d->kv_heads)) ||
-      (v && !out_ok(d->vo_ld, d->vo_hd, d->kv_heads)))
+  for (int64_t s : {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd, d->qo_ld, d->qo_hd, d->ko_ld, d->ko_hd,
+                    d->vo_ld, d->vo_hd})
+    if (s < 0 || s >> 40) return fail(VRS_EBADSHAPE, "%s: stride %lld", me, (long long)s);
+  if ((d->heads && !apart(d->qo_ld, d->qo_hd, d->rows, d->heads, d->head_dim)) ||
+      (d->kv_heads && !apart(d->ko_ld, d->ko_hd, d->k_out_rows, d->kv_heads, d->head_dim)) ||
+      (v && !apart(d->vo_ld, d->vo_hd, d->k_out_rows, d->kv_heads, d->head_dim)))
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
   if (d->heads && q == q_out && (d->q_ld != d->qo_ld || d->q_hd != d->qo_hd))
     return fail(VRS_EBADSHAPE, "%s: q_out is q with other strides", me);
@@ -197,7 +207,6 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   if (d->kv_heads && k == k_out && (moves || d->k_ld != d->ko_ld || d->k_hd != d->ko_hd))
     return fail(VRS_EBADSHAPE, "%s: k_out is k, but rows move or strides differ", me);
   if (v && v == v_out) return fail(VRS_EINVAL, "%s: v_out is v", me);
-  if (d->rows == 0 || (seqs && seqs->n == 0)) return VRS_OK;
 
   // the widest vector that divides the pairs, the head and every stride
   int vec = 16 / (int)es;
@@ -248,10 +257,10 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
   if (!(d->scale >= 0.f && d->scale <= 1e30f)) return fail(VRS_EINVAL, "%s: scale %g", me, (double)d->scale);
   const int vec = 16 / (int)elt_size(d->dtype);
   for (int64_t s : {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd, d->o_ld, d->o_hd})
-    if (s < 0 || s % vec) return fail(VRS_EBADSHAPE, "%s: strides must be multiples of 16 bytes", me);
+    if (s < 0 || s >> 40 || s % vec) return fail(VRS_EBADSHAPE, "%s: stride %lld (multiples of 16 bytes)", me, (long long)s);
   for (int64_t s : {d->q_ld, d->k_ld, d->v_ld, d->o_ld})
     if (s >= (1 << 22)) return fail(VRS_EUNSUPPORTED, "%s: row stride %lld", me, (long long)s);
-  if ((d->o_ld < d->head_dim && d->q_rows > 1) || (d->o_hd < d->head_dim && d->heads > 1))
+  if (!apart(d->o_ld, d->o_hd, d->q_rows, d->heads, d->head_dim))
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
   return VRS_OK;
 }
@@ -265,8 +274,10 @@ struct AttentionPlan {
 };
 AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   const int64_t group = d->heads / d->kv_heads;
-  const int64_t mq = std::max<int64_t>(1, s->max_q > 0 ? std::min(s->max_q, d->q_rows) : d->q_rows);
-  const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : d->k_rows;
+  // (unknown: as if all sequences were of one length)
+  const int64_t n = std::max(s->n, 1);
+  const int64_t mq = std::max<int64_t>(1, s->max_q > 0 ? std::min(s->max_q, d->q_rows) : (d->q_rows + n - 1) / n);
+  const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : (d->k_rows + n - 1) / n;
   AttentionPlan p;
   p.qt = 1;
   p.waves = 4;
@@ -339,10 +350,10 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
   if (rc) return rc;
   if (d->q_rows == 0 || seqs->n == 0) return VRS_OK;
   for (const auto& [p, name] : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}}) {
-    if (!p) return fail(VRS_EINVAL, "%s: null %s", me, name);
+    if (!p && (d->k_rows || name[0] == 'q' || name[0] == 'o')) return fail(VRS_EINVAL, "%s: null %s", me, name);
     if (!aligned(p, 16)) return fail(VRS_EBADSHAPE, "%s: %s must be 16-byte aligned", me, name);
   }
-  if (out == k || out == v || (out == q && (d->o_ld != d->q_ld || d->o_hd != d->q_hd)))
+  if ((d->k_rows && (out == k || out == v)) || (out == q && (d->o_ld != d->q_ld || d->o_hd != d->q_hd)))
     return fail(VRS_EINVAL, "%s: out is an input", me);
   const AttentionPlan p = plan_attention(d, seqs);
   const size_t need = attention_bytes(d, p);

@@ -283,11 +283,14 @@ def seqs(q_start, k_start=None, k_len=None, max_q=0, max_k=0):
     for t, size in ((q_start, n + 1), (k_start, n), (k_len, n)):
         if t is not None and (str(t.dtype) != "torch.int32" or t.numel() != size or not t.is_contiguous()):
             raise ValueError("seqs: contiguous int32 tensors q_start [n + 1], k_start [n], k_len [n]")
+        if t is not None and t.get_device() != q_start.get_device():
+            raise ValueError("seqs: tensors on different devices")
     if n < 0:
         raise ValueError("seqs: q_start needs n + 1 elements")
     s = Seqs(_ptr(q_start), _ptr(k_start), _ptr(k_len), n, max_q, max_k)
     s.tensors = (q_start, k_start, k_len)
     s.address = C.addressof(s)
+    s.device = q_start.get_device()
     return s
 
 
@@ -483,6 +486,12 @@ class Context:
                              f"{dtype} on cuda:{self.device} (the context's device), the last dimension contiguous")
         return st
 
+    def _seqs(self, what, seqs):
+        """Address of a vrs_seqs whose arrays lie on this context's device."""
+        if seqs.device != self.device:
+            raise ValueError(f"{what}: seqs on device {seqs.device}, the context's device is {self.device}")
+        return seqs.address
+
     def _launch_stream(self, stream):
         if stream is not None:
             return stream
@@ -541,7 +550,8 @@ class Context:
         k_out, and v as it is into v_out; freq: float64 device tensor [rot_dim / 2] (rope_freqs).
         positions: int32 [rows] or [axes, rows] (or more columns); None: the place in the sequence, or
         the row.  With seqs, k_out and v_out [rows of the cache, kv_heads, dim] receive each sequence's
-        rows at its keys' places.  q_out, k_out None: new tensors.  Returns (q_out, k_out)."""
+        rows at its keys' places.  q_out, k_out None: new tensors (rows of no sequence are unset in them).
+        Returns (q_out, k_out)."""
         import torch
         t0 = q if q is not None else k
         dt, dev = t0.dtype, t0.device
@@ -596,7 +606,7 @@ class Context:
                 if n == 1:
                     ld[i] = dim
         d = _ROPE(rows, k_out_rows, heads, kv, dim, rot, layout, code, axes, *per, *_NONE[axes:], scale, pos_ld, *ld)
-        check(lib().vrs_rope(self.handle, d, None if seqs is None else seqs.address, _ptr(freq), _ptr(positions), _ptr(q),
+        check(lib().vrs_rope(self.handle, d, None if seqs is None else self._seqs("rope", seqs), _ptr(freq), _ptr(positions), _ptr(q),
                              _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out), self._launch_stream(stream)))
         return q_out, k_out
 
@@ -627,12 +637,14 @@ class Context:
         if kv == 1:
             k_hd = v_hd = dim
         d = _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd)
-        L, s = lib(), seqs.address
+        L, s = lib(), self._seqs("attention", seqs)
         if workspace is None:
             have = L.vrs_attention_workspace_size(d, s)
             if have:
                 workspace = self._empty(stream, (have,), torch.uint8, dev)
         else:
+            if workspace.get_device() != self.device or not workspace.is_contiguous():
+                raise ValueError(f"attention: workspace on {workspace.device}; needs a contiguous tensor on cuda:{self.device}")
             have = workspace.numel() * workspace.element_size()
         check(L.vrs_attention(self.handle, d, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                               _ptr(workspace), have, self._launch_stream(stream)))
