@@ -327,21 +327,58 @@ __device__ __forceinline__ void part_of(int keys, int i, int parts, int unit, in
   ke = min(keys, (int)((int64_t)tiles * (i + 1) / parts) * unit);
 }
 
-// The r-th sequence by number of keys, the most first (over 64: the r-th).
-__device__ __forceinline__ int ranked_seq(const vrs_seq_args& s, int r) {
-  if (s.n == 1 || s.n > 64) return r;
-  const int i = threadIdx.x & 63;
-  const int keys = i < s.n ? seq_span(s, i).k_len : -1;
-  int rank = 0;
-  for (int k = 0; k < s.n; ++k) {
-    const int kk = __builtin_amdgcn_readlane(keys, k);
-    rank += kk > keys || (kk == keys && k < i);
-  }
-  return __builtin_ctzll(__ballot(rank == r));
+// Lane i's sequence, without another trip to memory.
+__device__ __forceinline__ SeqSpan span_of_lane(const SeqSpan& s, int i) {
+  SeqSpan p;
+  p.q0 = __builtin_amdgcn_readlane(s.q0, i);
+  p.q_len = __builtin_amdgcn_readlane(s.q_len, i);
+  p.k0 = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(s.k0 >> 32), i) << 32) |
+                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)s.k0, i));
+  p.k_len = __builtin_amdgcn_readlane(s.k_len, i);
+  p.k_lim = __builtin_amdgcn_readlane(s.k_lim, i);
+  return p;
 }
-// Place of a row tile: which sequence, and which of its tiles (of BM rows; a
+// Sum of x (or with ONES their number) over the lanes whose sequence comes
+// before this lane's: those with more keys, or as many and a smaller number
+// (from 2^25 keys on, as many).  Lanes without a sequence: keys -1.
+template <bool ONES>
+__device__ __forceinline__ int sum_before(int n, int keys, int x) {
+  const int lane = threadIdx.x & 63;
+  if (__ballot(lane < n && keys != __builtin_amdgcn_readfirstlane(keys)) == 0) {      // all alike: a prefix sum
+    if constexpr (ONES) return lane;
+    int sum = lane < n ? x : 0;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int o = __shfl_up(sum, m);
+      sum += lane >= m ? o : 0;
+    }
+    return sum - (lane < n ? x : 0);
+  }
+  // one number that orders both, and constant lanes: 64 sequences in about 1 us (3.5 in a plain loop)
+  const int order = keys < 0 ? -1 : min(keys, (1 << 25) - 1) << 6 | (63 - lane);
+  int before = 0;
+#pragma unroll
+  for (int c = 0; c < 64; c += 16) {
+    if (c >= n) break;
+#pragma unroll
+    for (int k = c; k < c + 16; ++k) {
+      const int kx = ONES ? 1 : __builtin_amdgcn_readlane(x, k);
+      before += __builtin_amdgcn_readlane(order, k) > order ? kx : 0;
+    }
+  }
+  return before;
+}
+// The r-th sequence by number of keys, the most first (over 64: the r-th).
+__device__ __forceinline__ SeqSpan ranked_seq(const vrs_seq_args& s, int r) {
+  if (s.n == 1 || s.n > 64) return seq_span(s, r);
+  const int lane = threadIdx.x & 63;
+  const SeqSpan sp = seq_span(s, min(lane, s.n - 1));
+  const int rank = sum_before<true>(s.n, lane < s.n ? sp.k_len : -1, 1);
+  return span_of_lane(sp, __builtin_ctzll(__ballot(lane < s.n && rank == r)));
+}
+// Place of a row tile: its sequence, and which of its tiles (of BM rows; a
 // query has `group` rows, one for each head of a key head).
-struct TilePlace { int seq, tile; };
+struct TilePlace { SeqSpan sp; int tile; };
 // Up to 64 sequences: those with the most keys first, so that the last
 // workgroups to run are short ones; lane i holds sequence i, and its first id is
 // the sum of the tiles of those before it.  More: in order, sequence i's ids
@@ -350,23 +387,18 @@ struct TilePlace { int seq, tile; };
 template <int BM>
 __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group, int id) {
   if (s.n <= 64) {
-    const int i = min((int)(threadIdx.x & 63), s.n - 1);
-    const SeqSpan sp = seq_span(s, i);
-    const int tiles = (int)(((int64_t)sp.q_len * group + BM - 1) / BM), keys = sp.k_len;
-    int before = 0;
-    for (int k = 0; k < s.n; ++k) {
-      const int kk = __builtin_amdgcn_readlane(keys, k), kt = __builtin_amdgcn_readlane(tiles, k);
-      if (kk > keys || (kk == keys && k < i)) before += kt;
-    }
-    const uint64_t hit = __ballot(id >= before && id < before + tiles && (int)(threadIdx.x & 63) < s.n);
-    if (!hit) return {0, -1};
-    const int at = __builtin_ctzll(hit);
-    return {at, id - __builtin_amdgcn_readlane(before, at)};
+    const int lane = threadIdx.x & 63;
+    const SeqSpan sp = seq_span(s, min(lane, s.n - 1));
+    const int tiles = (int)(((int64_t)sp.q_len * group + BM - 1) / BM);
+    const int before = sum_before<false>(s.n, lane < s.n ? sp.k_len : -1, tiles);
+    const uint64_t hit = __ballot(id >= before && id < before + tiles && lane < s.n);
+    const int at = hit ? __builtin_ctzll(hit) : 0;
+    return {span_of_lane(sp, at), hit ? id - __builtin_amdgcn_readlane(before, at) : -1};
   }
   auto first = [&](int i) { return (int)((int64_t)min(max(s.q_start[i], 0), s.q_rows) * group / BM) + i; };
-  if (id < first(0)) return {0, -1};
+  if (id < first(0)) return {SeqSpan{}, -1};
   const int sq = find_seq(s.n, id, first);
-  return {sq, id - first(sq)};
+  return {seq_span(s, sq), id - first(sq)};
 }
 
 // ---------------------------------------------------------------------------
@@ -415,7 +447,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   const int group = a.heads / a.kv;
   const TilePlace at = place_tile<BM>(a.s, group, rest / a.parts);
   if (at.tile < 0) return;
-  const SeqSpan sp = seq_span(a.s, at.seq);
+  const SeqSpan sp = at.sp;
   const int64_t rows = (int64_t)sp.q_len * group;
   const int tiles = (int)((rows + BM - 1) / BM);
   if (at.tile >= tiles) return;
@@ -439,6 +471,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   int kb, ke;
   part_of(visible(sp, (int)((min(r0 + BM, rows) - 1) / group), a.causal), part, a.parts, KT, kb, ke);
   const int all = visible(sp, (int)(r0 / group), a.causal);   // keys that every row of the workgroup sees
+  const int mine = __builtin_amdgcn_readlane(w.lim[QT - 1], 31);   // keys that some row of the wave sees
 
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
@@ -514,18 +547,21 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const bool last = n == NS - 1;
-        w.follow(t, a.c);
+        const bool live = !TAIL || kc + n * 32 < mine;
+        if (live) w.follow(t, a.c);
         if (last) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the next tile
         if (last || (TAIL && kc + KT > all)) __syncthreads();
         if (last && kc + 2 * KT < ke) load(buf == 0 ? 2 : buf - 1, kc + 2 * KT);
         f32x16_t s1[QT];
-        const bool ahead = !TAIL || !last || more;
+        const bool ahead = !TAIL || ((!last || more) && kc + (n + 1) * 32 < mine);
         __builtin_amdgcn_s_setprio(1);
         if (ahead) w.scores(last ? smem + nbuf * 2 * TILE : sK, last ? 0 : (n + 1) * 32, s1);
-        typename Wave<T, D, QT>::P p[QT];
+        if (live) {
+          typename Wave<T, D, QT>::P p[QT];
 #pragma unroll
-        for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], a.c);
-        w.pv(sK + TILE, n * 32, p);
+          for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], a.c);
+          w.pv(sK + TILE, n * 32, p);
+        }
         __builtin_amdgcn_s_setprio(0);
         if (ahead) {
 #pragma unroll
@@ -579,8 +615,8 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   // no two workgroups share keys: in the order of launch, round the XCDs, the
   // sequences with the most keys first
   const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv;
-  const int part = rest % a.parts, sq = ranked_seq(a.s, rest / a.parts);
-  const SeqSpan sp = seq_span(a.s, sq);
+  const int part = rest % a.parts;
+  const SeqSpan sp = ranked_seq(a.s, rest / a.parts);
   const int G_ = a.heads / a.kv;
   const int64_t rows = (int64_t)sp.q_len * G_;
   T* sV = reinterpret_cast<T*>(mem) + wave * 32 * D;
