@@ -427,7 +427,7 @@ __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group
 // LDS bank conflicts; 8 waves and 64-key tiles against 4 waves and 32: 516 us to
 // 548.  At head sizes up to 64 the same exponentials serve half the products
 // and the VALU is the busier (64 % against 36 %): 24 images of 196 .. 1600
-// patches, 12 heads: 125 us, 715 TFLOP/s; four 4-wave workgroups on a CU with
+// patches, 12 heads: 122 .. 128 us, 715 TFLOP/s; four 4-wave workgroups on a CU with
 // 32-key tiles against three with 64: 124 us to 130; two query tiles to a wave
 // for the large (4096 x 32 heads: 148 us to 159).  float32 is bound by its
 // matrix instructions (64 cycles each).

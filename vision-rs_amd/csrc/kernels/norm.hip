@@ -9,8 +9,9 @@
 // row in registers between its two passes (sum of squares, then scaling), so
 // a row is read once; a workgroup walks rows with the weights it needs in
 // registers and the next row's loads in flight, which no branch holds up.
-// 8192 rows of 4096 columns in bfloat16 with the residual, 268 MB: 43 us,
-// 6.2 TB/s (58 us without the loads ahead; a copy of 1 GiB moves 5.15 TB/s).
+// 8192 rows of 4096 columns in bfloat16 with the residual, 268 MB: 43 us in
+// bursts and 50 sustained, 6.2 and 5.3 TB/s (58 us without the loads ahead; a
+// copy of 1 GiB moves 5.15 TB/s).
 // Rows too wide for that (over 1024 vectors) lie in LDS as float32 between
 // the passes, 1024 threads to a row.
 #include "common.h"
