@@ -476,8 +476,8 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
   // A thread's chunks of a tile, straight to LDS: one instruction of a wave fills 1 KiB in lane
-  // order, so the swizzle is in what each lane loads.  Elements past the head read nothing (they
-  // stay 0 in LDS); keys past the sequence's last leave what was there, masked and, for V, cleaned.
+  // order, so the swizzle is in what each lane loads.  Elements past the head and keys past the
+  // sequence's last are out of the buffer's range and fill in 0; such keys are masked besides.
   uint32_t ko[IT], vo[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
@@ -513,10 +513,6 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   };
   if (kb < ke) {
     if (tid < 3) odd_tile[tid] = -1;
-    if (a.dim < D) {
-      for (int i = tid; i < 3 * 2 * TILE / PER; i += NT) reinterpret_cast<u32x4_t*>(smem)[i] = (u32x4_t){0, 0, 0, 0};
-      __syncthreads();
-    }
     load(0, kb);
     if (kb + KT < ke) {
       load(1, kb + KT);
