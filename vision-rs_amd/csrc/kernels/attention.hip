@@ -47,15 +47,11 @@ __device__ __forceinline__ float sum32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A buffer resource in scalar registers, and a 16-byte load of each lane straight to LDS: lane i's
-// at `to` + 16 i.  Nothing waits for it by itself: the vmcnt waits below do.
+// A buffer resource in scalar registers, for load_lds.
 __device__ __forceinline__ i32x4_hw lds_rsrc(const void* base, int bytes) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);
   return (i32x4_hw){__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff),
                     __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
-}
-__device__ __forceinline__ void load_lds(const i32x4_hw& r, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r) : "memory", "m0");
 }
 
 // Layout of a K or V tile in LDS: rows of D elements, 16-byte chunks XORed

@@ -92,6 +92,15 @@ __device__ __forceinline__ uint32_t upper_half_mask() {
   return m;
 }
 
+// A 16-byte load of each lane straight to LDS: lane i's at `to` + 16 i.  Nothing waits for it by itself, the
+// compiler does not count it: its users' vmcnt waits do.  No wait states are inserted inside inline assembly
+// either: a scalar write of M0 has to be one before the load, and one of r by a vector instruction (the
+// readfirstlanes that make it uniform) five, of which the move of M0 is one.
+__device__ __forceinline__ void load_lds(const i32x4_hw& r, uint32_t off, uint32_t to) {
+  asm volatile("s_nop 2\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r)
+               : "memory", "m0");
+}
+
 // ---- element traits --------------------------------------------------------
 // A "group" is 8 consecutive elements along K: the unit one lane feeds into
 // the 16x16x32 MFMA step (bf16: one 16-byte register quad; f32: two quads).

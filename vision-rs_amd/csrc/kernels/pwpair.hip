@@ -241,8 +241,7 @@ __device__ __forceinline__ void pwpair_w_body(const vrs_pwpair_args& a) {
   const int base_lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)xbase);
   const int base_hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(xbase >> 32) & 0xffff);
   const int xbytes = __builtin_amdgcn_readfirstlane(a.x_bytes);
-  typedef int i4_t __attribute__((ext_vector_type(4)));
-  const i4_t rd = {base_lo, base_hi, xbytes, 0x00020000};
+  const i32x4_hw rd = {base_lo, base_hi, xbytes, 0x00020000};
   auto stage = [&](int t, int b) {
     const int m0 = t * NP;
 #pragma unroll
@@ -252,8 +251,7 @@ __device__ __forceinline__ void pwpair_w_body(const vrs_pwpair_args& a) {
       const uint32_t off = m0 + p < a.M ? (uint32_t)(((m0 + p) * a.x_pitch + c * 8) * 2) : kOOB;
       const uint32_t la = __builtin_amdgcn_readfirstlane(
           (uint32_t)(uintptr_t)(lds_void_t*)(xs + b * XB + (wave * NQ + q) * 64 * 8));
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(la), "v"(off), "s"(rd)
-                   : "memory", "m0");
+      load_lds(rd, off, la);
     }
   };
   int t = blockIdx.x;
