@@ -396,7 +396,8 @@ int vrs_msda(vrs_ctx* ctx, const vrs_msda_desc* d, const float* value, const flo
  * y_dtype == VRS_FP8: y is e4m3, rne(clamp(y / scale)), with
  *   group == 0:     scale = out_step (a power of two), as vrs_conv2d reads
  *                   with x_e4m3 and in_scale = out_step; scales unused
- *   group == cols:  one scale per row, max|y| / 448 (1 for a zero row)
+ *   group == cols:  one scale per row, max|y| / 448 (1 where that is 0: a zero
+ *                   row, or one below 3.2e-43, all of whose e4m3 values are 0)
  *   32, 64 or 128:  one per that many columns (cols a multiple of it)
  * stored in scales[rows][cols / group].  NaN elements do not count in a
  * maximum and stay NaN.  cols <= 32768.  e4m3 needs 16-byte aligned rows

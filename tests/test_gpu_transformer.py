@@ -138,6 +138,34 @@ def test_rms_norm_values_at_the_ends_of_the_range():
     assert q.isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols,group", [(512, 32), (512, 64), (4096, 128), (256, 256), (4096, 4096), (16384, 128), (16384, 16384)])
+def test_rms_norm_e4m3_of_tiny_maxima(dtype, cols, group):
+    """Scales that are no normal number, or none at all: quotients by them, and zeros stay zeros."""
+    import torch
+    x = randn(6, cols, dtype=dtype, seed=8)
+    x[:, ::5] = 0
+    tiny = [1.0, 3e-36, 2e-37, 1e-38, 1e-40, 3e-42, 2e-44]
+    groups = cols // group
+    for first in range(0, 7, 1 if groups == 1 else 4):      # one group: its weights are each size in turn
+        w = randn(cols, dtype="f32", seed=9).sign()
+        for g in range(groups):
+            w[g * group:(g + 1) * group] *= tiny[(first + g) % 7]
+        y, _, scales = ctx().rms_norm(x, w, 1e-6, e4m3=True, group=group)
+        _, ry = rms_ref(x, None, w, 1e-6)
+        e = rms_tol(cols)
+        # y and the scale are off by half a unit of 2^-149 besides, twice for the maximum's own
+        amax = ry.abs().view(6, groups, group).amax(2)
+        rscale = amax / 448
+        rscale = torch.where(rscale < 2.0 ** -150, torch.ones_like(rscale), rscale)
+        inside(scales, rscale, rscale * (e + 4 * F) + 2.0 ** -149)
+        scale = scales.double().repeat_interleave(group, 1)
+        q = (ry / scale).clamp(-448, 448)
+        got = y.view(torch.float8_e4m3fn)
+        inside(got, q, (q.abs() * U["e4m3"]).clamp(min=2.0 ** -10) + q.abs() * (e + 4 * F) * 1.1 + 2.0 ** -149 / scale * (1 + U["e4m3"]))
+        assert torch.all(got.float()[:, ::5] == 0)
+
+
 # ---- rotary positions ----------------------------------------------------------------
 
 

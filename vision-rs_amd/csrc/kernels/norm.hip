@@ -19,6 +19,7 @@
 namespace {
 constexpr int kSame = 0, kFp8 = 1;
 constexpr float kE4m3Max = 448.f;
+constexpr float kMinNormal = 1.17549435e-38f;     // 2^-126
 
 // VEC elements as they lie in memory (16 bytes, or one element), and as floats.
 template <typename T, int VEC>
@@ -98,10 +99,22 @@ __device__ __forceinline__ V row_reduce(V v, V* lds) {
 // Whether a float32 sum of squares stands for its terms: neither they nor it left the type's range.
 __device__ __forceinline__ bool in_range(float ss) { return ss > 1e-25f && ss < INFINITY; }
 
-// VEC elements of a row to e4m3, on `inv` or on the scale of their group, whose lanes are
+// How a maximum m of |y| scales to e4m3: by m / 448, by 1 where that is 0 (no values, or none that a
+// scale could stand for).  Quotients by the scale are products with 448 / m as long as the scale is a
+// normal number and so that inverse finite; by smaller scales (inv 0) they are divided.
+struct Scale {
+  float scale, inv;
+  static __device__ __forceinline__ Scale step(float inv) { return {1.f, inv}; }
+  static __device__ __forceinline__ Scale of(float m) {
+    const float s = m / kE4m3Max;
+    return {s > 0.f ? s : 1.f, m >= kE4m3Max * kMinNormal ? kE4m3Max / m : 0.f};
+  }
+};
+
+// VEC elements of a row to e4m3, on `sc` or on the scale of their group, whose lanes are
 // neighbours in a wave (all of them here, `in` or not).
 template <int VEC>
-__device__ __forceinline__ void put_fp8(const vrs_rms_args& a, int64_t row, int c, bool in, bool per_row, float inv,
+__device__ __forceinline__ void put_fp8(const vrs_rms_args& a, int64_t row, int c, bool in, bool per_row, Scale sc,
                                         const float (&y)[VEC]) {
   if (a.group && !per_row) {
     float m = 0.f;
@@ -109,13 +122,16 @@ __device__ __forceinline__ void put_fp8(const vrs_rms_args& a, int64_t row, int 
     for (int e = 0; e < VEC; ++e) m = fmaxf(m, fabsf(y[e]));
     const int lanes = a.group / VEC;
     for (int d = 1; d < lanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    inv = m > 0.f ? kE4m3Max / m : 1.f;
-    if (in && c % a.group == 0) a.scales[row * (a.cols / a.group) + c / a.group] = m > 0.f ? m / kE4m3Max : 1.f;
+    sc = Scale::of(m);
+    if (in && c % a.group == 0) a.scales[row * (a.cols / a.group) + c / a.group] = sc.scale;
   }
   if (in) {
     float q[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) q[e] = y[e] * inv;
+    for (int e = 0; e < VEC; ++e) q[e] = y[e] * sc.inv;
+    if (sc.inv == 0.f)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) q[e] = y[e] / sc.scale;
     store_fp8<VEC>(static_cast<uint8_t*>(a.y) + row * a.y_ld + c, q);
   }
 }
@@ -197,17 +213,16 @@ __device__ __forceinline__ void rms_body(const vrs_rms_args& a) {
         if (ok && c < a.cols) store_vec<T, VEC>(static_cast<T*>(a.y) + row * a.y_ld + c, s[i]);
       }
     } else {
-      float inv = a.inv_step;
+      Scale sc = Scale::step(a.inv_step);
       const bool per_row = a.group == a.cols;
       if (per_row) {
-        amax = row_reduce<float, TPR, true>(amax, lds);
-        inv = amax > 0.f ? kE4m3Max / amax : 1.f;
-        if (ok && t == 0) a.scales[row] = amax > 0.f ? amax / kE4m3Max : 1.f;
+        sc = Scale::of(row_reduce<float, TPR, true>(amax, lds));
+        if (ok && t == 0) a.scales[row] = sc.scale;
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + t) * VEC;
-        put_fp8<VEC>(a, row, c, ok && c < a.cols, per_row, inv, s[i]);
+        put_fp8<VEC>(a, row, c, ok && c < a.cols, per_row, sc, s[i]);
       }
     }
   }
@@ -267,7 +282,7 @@ __device__ __forceinline__ void rms_wide_body(const vrs_rms_args& a) {
         store_vec<T, VEC>(static_cast<T*>(a.y) + row * a.y_ld + c, y);
       }
     } else {
-      float inv = a.inv_step;
+      Scale sc = Scale::step(a.inv_step);
       const bool per_row = a.group == a.cols;
       if (per_row) {
         float amax = 0.f;
@@ -277,14 +292,13 @@ __device__ __forceinline__ void rms_wide_body(const vrs_rms_args& a) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, fabsf(y[e]));
         }
-        amax = row_reduce<float, NT, true>(amax, lds);
-        inv = amax > 0.f ? kE4m3Max / amax : 1.f;
-        if (threadIdx.x == 0) a.scales[row] = amax > 0.f ? amax / kE4m3Max : 1.f;
+        sc = Scale::of(row_reduce<float, NT, true>(amax, lds));
+        if (threadIdx.x == 0) a.scales[row] = sc.scale;
       }
       for (int b = 0; b < a.cols; b += step) {     // every lane to the end: a group's lanes meet
         float y[VEC];
         value(b + c0, y);
-        put_fp8<VEC>(a, row, b + c0, b + c0 < a.cols, per_row, inv, y);
+        put_fp8<VEC>(a, row, b + c0, b + c0 < a.cols, per_row, sc, y);
       }
     }
   }
