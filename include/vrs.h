@@ -443,7 +443,9 @@ typedef struct {
  *                      they are, under `low` turns f / factor, linear in the
  *                      turns between
  *   VRS_ROPE_BY_INDEX  the same with a ramp linear in the pair's index, from
- *                      floor(index of `high` turns) to ceil(index of `low`)
+ *                      floor(index of `high` turns), 0 at least, to ceil(index
+ *                      of `low`), 2 pairs - 1 at most and past the last pair
+ *                      where that makes more turns than `low`
  * Host arithmetic in 64 bits; out has `pairs` doubles (put them on the
  * device for vrs_rope; several axes: one call for each, one after another). */
 #define VRS_ROPE_PLAIN 0

@@ -115,6 +115,22 @@ def test_rope_frequencies():
     assert torch.all(share[lo:hi + 1].diff() < 0)
 
 
+@pytest.mark.parametrize("pairs,base,orig,lo,hi", [
+    (64, 10000.0, 65536, 40, 65), (64, 10000.0, 131072, 45, 70), (32, 10000.0, 65536, 20, 33), (8, 100.0, 32768, 8, 15),
+    (8, 100.0, 131072, 11, 15), (64, 10000.0, 100, 0, 20)])
+def test_rope_frequencies_whose_ramp_passes_the_last_pair(pairs, base, orig, lo, hi):
+    """By index: the ramp ends at the index of `low` turns, which may lie past the last pair (up to 2 pairs - 1) and
+    whose first may lie before the first pair."""
+    import torch
+    at = [pairs * math.log(orig / (t * 2 * math.pi)) / math.log(base) for t in (32.0, 1.0)]
+    assert lo == max(math.floor(at[0]), 0) and hi == min(math.ceil(at[1]), 2 * pairs - 1)
+    f = vrs.rope_freqs(pairs, base, vrs.ROPE_BY_INDEX, 8.0, 1.0, 32.0, orig)
+    for i in range(pairs):
+        plain = base ** (-i / pairs) / (2 * math.pi)
+        keep = 1 - min(max((i - lo) / (hi - lo), 0.0), 1.0)
+        assert math.isclose(f[i].item(), plain * keep + plain / 8 * (1 - keep), rel_tol=1e-12), i
+
+
 @pytest.mark.parametrize("args", [
     (0, 1e4, 0, 1, 1, 2, 100), (257, 1e4, 0, 1, 1, 2, 100), (8, 1.0, 0, 1, 1, 2, 100), (8, math.nan, 0, 1, 1, 2, 100),
     (8, 1e4, 4, 1, 1, 2, 100), (8, 1e4, 1, 0, 1, 2, 100), (8, 1e4, 2, 2, 2, 2, 100), (8, 1e4, 3, 2, 0, 2, 100),

@@ -151,7 +151,7 @@ int vrs_rope_freqs(int32_t pairs, double base, int32_t scaling, double factor, d
     if (scaling == VRS_ROPE_BY_TURNS) keep = std::clamp((f * orig_len - low) / (high - low), 0.0, 1.0);
     if (scaling == VRS_ROPE_BY_INDEX) {
       const double from = std::max(std::floor(index_of(high)), 0.0);
-      const double to = std::max(std::min(std::ceil(index_of(low)), pairs - 1.0), from + 1e-3);
+      const double to = std::max(std::min(std::ceil(index_of(low)), 2.0 * pairs - 1.0), from + 1e-3);
       keep = 1.0 - std::clamp((i - from) / (to - from), 0.0, 1.0);
     }
     out[i] = f * keep + f / (scaling == VRS_ROPE_PLAIN ? 1.0 : factor) * (1.0 - keep);
