@@ -499,7 +499,8 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
  * not see, and whatever lies behind a sequence's keys, do not touch its result
  * even where they hold NaN.  head_dim: a multiple of 8 up to 128; q, k, v, out
  * and their strides 16-byte aligned, row strides under 4 M elements.  Scores,
- * softmax and sums are float32; bfloat16 rounds the probabilities once.
+ * softmax and sums are float32 (scores of any size that twice log2(e) times
+ * scale leaves in its range); bfloat16 rounds the probabilities once.
  * Results do not depend on the run (fixed order of every sum), but the kernel
  * chosen from max_q, max_k, q_rows and k_rows decides that order.
  * workspace: 16-byte aligned, of at least vrs_attention_workspace_size bytes

@@ -484,6 +484,46 @@ def test_attention_scale_and_large_scores():
         check_attention(([70], None, None), dtype, scale=1e-30)
 
 
+LARGE = [(1, 60, 4, 2, 64), (1, 5000, 8, 1, 128), (3, 900, 4, 2, 64), (130, 0, 4, 2, 64), (100, 6000, 8, 1, 128), (2100, 0, 32, 32, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("base,step", [(2.0 ** 20, 1.0), (2.0 ** 20, 0.25), (-2.0 ** 20, 1.0), (-2.0 ** 31, 2.0 ** 12), (2.0 ** 40, 2.0 ** 30), (-2.0 ** 40, 2.0 ** 30),
+                                       (-2.0 ** 100, 2.0 ** 90), (2.0 ** 100, 2.0 ** 90), (-2.0 ** 29, 2.0 ** 6), (0.0, 2.0 ** 60), (0.0, 2.0 ** 28), (0.0, 2.0 ** 110)])
+@pytest.mark.parametrize("q_len,past,heads,kv,dim", LARGE)
+def test_attention_scores_far_from_zero(dtype, base, step, q_len, past, heads, kv, dim):
+    """Scores that float32 holds exactly, all far below or above zero or growing from one to the other:
+    base + step * level, the level a key's own."""
+    import torch
+    n = q_len + past
+    causal = q_len < 1000
+    g = torch.Generator(device="cuda").manual_seed(q_len)
+    level = torch.randint(0, 5 if step > 0.5 else 60, (n,), generator=g, device="cuda")
+    if base == 0:
+        level = torch.arange(n, device="cuda") * 5 // n - 2       # rising
+    q = torch.zeros(q_len, heads, dim, dtype=tdt(dtype), device="cuda")
+    k = torch.zeros(n, kv, dim, dtype=tdt(dtype), device="cuda")
+    half = 2.0 ** (math.log2(abs(base)) // 2) if base else 0.0
+    q[..., 0], q[..., dim - 1] = half, step ** 0.5 if step > 1 else 1.0
+    k[..., 0], k[..., dim - 1] = (base / half if base else 0.0), level[:, None] * (step / q[0, 0, dim - 1].item())
+    v = randn(n, kv, dim, dtype=dtype, seed=3)
+    s = base + step * level.double()
+    assert torch.equal((q[0, 0].double() @ k[:, 0].double().t()), s) and torch.equal(s.float().double(), s)
+    seqs = vrs.seqs(i32([0, q_len]), i32([0]), i32([n]), max_q=q_len, max_k=n)
+    got = ctx().attention(q, k, v, seqs, causal=causal, scale=1.0)
+    seen = torch.ones(q_len, n, dtype=torch.bool, device="cuda")
+    if causal:
+        seen = seen.tril(past)
+    s = s[None].masked_fill(~seen, -math.inf)
+    w = torch.softmax(s, 1)
+    vd = v.double().repeat_interleave(heads // kv, 1)
+    ref = (w @ vd.view(n, -1)).view(q_len, heads, dim)
+    size = (w @ vd.abs().view(n, -1)).view(q_len, heads, dim)
+    # as in attention_ref, the scores exact: exponents under 2^5 of half a unit, and a function off by one
+    u = 0.0 if dtype == "f32" else U["bf16"]
+    inside(got, ref, (size + ref.abs()) * (u + 64 * F) * 1.02 + size * (2 * n + 70) * F + ref.abs() * U[dtype] * 1.01)
+
+
 def test_attention_strided():
     """Queries, keys and values of one product; heads outermost; a repeated head."""
     import torch

@@ -374,7 +374,7 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
   if (need) {
     const int64_t rows = (int64_t)p.parts * d->q_rows * d->heads;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * d->head_dim);
+    a.part_rl = reinterpret_cast<float2*>(a.part_o + rows * d->head_dim);
   }
   const int64_t blocks = p.parts * (p.few ? (int64_t)seqs->n : p.row_tiles) * d->kv_heads;
   const int64_t joins = ((int64_t)d->q_rows * d->heads * (d->head_dim / 4) + 255) / 256;

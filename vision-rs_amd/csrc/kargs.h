@@ -377,7 +377,7 @@ typedef struct {
   const void *q, *k, *v;
   void* out;
   float* part_o;           /* parts > 1: [parts][q_rows][heads][dim] */
-  float2* part_ml;         /* parts > 1: [parts][q_rows][heads] running maximum (log2 units) and sum */
+  float2* part_rl;         /* parts > 1: [parts][q_rows][heads] reference of the weights and their sum */
   vrs_seq_args s;
   int64_t q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd;   /* elements between rows, between heads */
   int32_t heads, kv, dim, causal;

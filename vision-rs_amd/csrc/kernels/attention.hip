@@ -7,7 +7,7 @@
 //
 // Both kernels work in wave tiles of 32 queries x 32 keys:
 //   S^T(keys x queries) = K Q^T     on 32x32 MFMA, K rows as A, Q^T as B
-//   p = exp2(s c - m c)             c = scale log2 e; one FMA and one v_exp
+//   p = 2^(s c - R)                 c = scale log2 e, R near m c (Log2)
 //   O^T(d x queries) += V^T P^T     the accumulator of S^T is already P^T's
 //                                   operand layout, V^T in the same key order
 // A lane holds 16 keys of one query, so the row maximum and sum need one
@@ -46,6 +46,36 @@ __device__ __forceinline__ float sum32(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// A query's weights are p = 2^(s c - R), one FMA and one v_exp, against a reference R that follows its
+// running maximum m: R = m c rounded to float32, and every later factor is taken from that R, so its
+// rounding weighs all keys alike.  Far from zero it could leave the range of 2^x: from |m c| = 2^30 on a
+// power of two w >= c stands for c, whose products are exact.  Distinct scores are 2^6 log2 units apart
+// there, so that the lower one weighs nothing on either.
+constexpr float kFar = 1073741824.f;
+constexpr float kNone = -3.40282347e38f;     // R before the first key: 2^(kNone - R) is 0, and so is p of a score -inf
+struct Log2 {
+  float c, w;
+  __device__ __forceinline__ explicit Log2(float c_)
+      : c(c_), w(__uint_as_float((__float_as_uint(c_) + 0x7fffffu) & 0x7f800000u)) {}
+  static __device__ __forceinline__ bool far(float R) { return !(fabsf(R) < kFar); }
+  __device__ __forceinline__ float unit(float R) const { return far(R) ? w : c; }
+  __device__ __forceinline__ float exponent(float s, float R) const { return __builtin_fmaf(s, unit(R), -R); }
+  __device__ __forceinline__ float reference(float m) const {
+    const float R = m * c;
+    return far(R) ? m * w : R;
+  }
+  // what weights on `from` are multiplied by on `to`
+  __device__ __forceinline__ float factor(float from, float to) const {
+#pragma clang fp contract(off)       // the references are rounded already
+    float e = from - to;
+    if (far(from) != far(to)) {      // the far one's m c, whole
+      const float per_w = __uint_as_float(0x7f000000u - __float_as_uint(w));     // 1 / w
+      e = far(from) ? __builtin_fmaf(from * per_w, c, -to) : -__builtin_fmaf(to * per_w, c, -from);
+    }
+    return __builtin_amdgcn_exp2f(e);
+  }
+};
 
 // A buffer resource in scalar registers, for load_lds.
 __device__ __forceinline__ i32x4_hw lds_rsrc(const void* base, int bytes) {
@@ -91,7 +121,7 @@ struct Wave {
   static constexpr int PER = 16 / (int)sizeof(T);   // elements of a chunk
   G qf[QT][D / 16];
   f32x16_t o[QT][D / 32];
-  float m[QT], l[QT];   // running maximum (raw scores) and this lane's share of the sum
+  float R[QT], l[QT];   // reference (see Log2) and this lane's share of the sum
   int lim[QT];          // keys that the lane's query sees
   int l32, hh;
 
@@ -100,7 +130,7 @@ struct Wave {
     hh = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-      m[q] = -INFINITY;
+      R[q] = kNone;
       l[q] = 0.f;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
@@ -130,18 +160,17 @@ struct Wave {
     for (int r = 1; r < 16; ++r) t = fmaxf(t, s[r]);
     return max32(t);
   }
-  // the running maxima follow the tile maxima t where one is exceeded by more than 2^kTau
-  __device__ __forceinline__ void follow(const float (&t)[QT], float c) {
-    bool far = false;
+  // the references follow the tile maxima t where one is exceeded by more than 2^kTau
+  __device__ __forceinline__ void follow(const float (&t)[QT], const Log2& u) {
+    bool over = false;
 #pragma unroll
-    for (int q = 0; q < QT; ++q) far |= (t[q] - m[q]) * c > kTau;
-    if (__any(far)) {
-      // (a first maximum: t - -inf; lanes without any key yet keep -inf and factor 1)
+    for (int q = 0; q < QT; ++q) over |= u.exponent(t[q], R[q]) > kTau;
+    if (__any(over)) {
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-        const float mn = fmaxf(m[q], t[q]);
-        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[q] - mn) * c);
-        m[q] = mn;
+        const float to = u.exponent(t[q], R[q]) > 0.f ? u.reference(t[q]) : R[q];
+        const float alpha = u.factor(R[q], to);
+        R[q] = to;
         l[q] *= alpha;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) o[q][d] *= alpha;
@@ -150,21 +179,20 @@ struct Wave {
   }
   // scores -> probabilities: packed pairs (bfloat16, l summing the rounded ones) or float32
   struct P { uint32_t u[sizeof(T) == 2 ? 8 : 16]; };
-  __device__ __forceinline__ P probs(int q, const f32x16_t& s, float c) {
-    const float mc = m[q] == -INFINITY ? 0.f : m[q] * c;
+  __device__ __forceinline__ P probs(int q, const f32x16_t& s, const Log2& u) {
     P p;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p.u[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, -mc)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, -mc)));
+        p.u[i] = pack_bf16x2(__builtin_amdgcn_exp2f(u.exponent(s[2 * i], R[q])),
+                             __builtin_amdgcn_exp2f(u.exponent(s[2 * i + 1], R[q])));
         l[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v_t, p.u[i]),
                                                __builtin_bit_cast(bf16x2v_t, 0x3f803f80u), l[q], false);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mc));
+        const float e = __builtin_amdgcn_exp2f(u.exponent(s[r], R[q]));
         p.u[r] = __float_as_uint(e);
         l[q] += e;
       }
@@ -296,10 +324,10 @@ struct Wave {
     }
   }
 
-  // the unfinished query to a workspace: O (float32), running maximum in log2 units, sum
-  __device__ __forceinline__ void store_part(int q, float* po, float2* pml, int dim, float c, bool ok) const {
+  // the unfinished query to a workspace: O (float32), reference, sum
+  __device__ __forceinline__ void store_part(int q, float* po, float2* prl, int dim, bool ok) const {
     const float lt = sum32(l[q]);
-    if (ok && hh == 0) *pml = make_float2(m[q] == -INFINITY ? -INFINITY : m[q] * c, lt);
+    if (ok && hh == 0) *prl = make_float2(R[q], lt);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -449,6 +477,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   if (at.tile >= tiles) return;
   const int64_t r0 = (int64_t)(tiles - 1 - at.tile) * BM;     // late rows (causal: the most keys) first
 
+  const Log2 u(a.c);
   Wave<T, D, QT> w;
   w.init();
   int64_t qrow[QT];
@@ -540,7 +569,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       for (int n = 0; n < NS; ++n) {
         const bool last = n == NS - 1;
         const bool live = !TAIL || kc + n * 32 < mine;
-        if (live) w.follow(t, a.c);
+        if (live) w.follow(t, u);
         if (last) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the next tile
         if (last || (TAIL && kc + KT > all)) __syncthreads();
         if (last && kc + 2 * KT < ke) load(buf == 0 ? 2 : buf - 1, kc + 2 * KT);
@@ -551,7 +580,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
         if (live) {
           typename Wave<T, D, QT>::P p[QT];
 #pragma unroll
-          for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], a.c);
+          for (int q = 0; q < QT; ++q) p[q] = w.probs(q, s[q], u);
           w.pv(sK + TILE, n * 32, p);
         }
         __builtin_amdgcn_s_setprio(0);
@@ -579,7 +608,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
       w.store(q, static_cast<T*>(a.out) + qrow[q] * a.o_ld + head[q] * a.o_hd, a.dim, ok[q]);
     } else {
       const int64_t i = ((int64_t)part * a.s.q_rows + qrow[q]) * a.heads + head[q];
-      w.store_part(q, a.part_o + i * a.dim, a.part_ml + i, a.dim, a.c, ok[q]);
+      w.store_part(q, a.part_o + i * a.dim, a.part_rl + i, a.dim, ok[q]);
     }
   }
 }
@@ -602,7 +631,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   constexpr int OL = D + 4;                        // O row in LDS (float32)
   constexpr int V_BYTES = NW * 32 * D * (int)sizeof(T), O_BYTES = NW * 32 * OL * 4;
   __shared__ __attribute__((aligned(16))) char mem[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
-  __shared__ float sm[NW][32], sl[NW][32];
+  __shared__ float sR[NW][32], sl[NW][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // no two workgroups share keys: in the order of launch, round the XCDs, the
   // sequences with the most keys first
@@ -614,6 +643,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   T* sV = reinterpret_cast<T*>(mem) + wave * 32 * D;
   float* sO = reinterpret_cast<float*>(mem);
 
+  const Log2 u(a.c);
   // row tiles of the sequence, one workgroup each (and more than were counted on, in turn)
   for (int64_t r0 = blockIdx.y * 32; r0 < rows; r0 += gridDim.y * 32) {
     Wave<T, D, 1> w;
@@ -678,17 +708,17 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
       if (kc < ke) load(kc);
       if (masked) w.mask(0, s[0], at);
       const float t[1] = {w.top(s[0])};
-      w.follow(t, a.c);
-      const typename Wave<T, D, 1>::P p[1] = {w.probs(0, s[0], a.c)};
+      w.follow(t, u);
+      const typename Wave<T, D, 1>::P p[1] = {w.probs(0, s[0], u)};
       w.pv(sV, 0, p);
       if (__any(bad)) w.add_specials(vp + (int64_t)at * a.v_ld, a.v_ld, sp.k_lim - at, a.dim, at);
       __builtin_amdgcn_wave_barrier();
     }
-    // join the waves: the largest maximum, sums and O scaled to it
+    // join the waves: the largest reference, sums and O scaled to it
     const float lt = sum32(w.l[0]);
     __syncthreads();                       // every wave is done with its V tile
     if (w.hh == 0) {
-      sm[wave][w.l32] = w.m[0];
+      sR[wave][w.l32] = w.R[0];
       sl[wave][w.l32] = lt;
     }
 #pragma unroll
@@ -703,18 +733,18 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
     if (r0 + rr < rows) {
       const int jj = (int)((r0 + rr) / G_), ho = hk * G_ + (int)(r0 + rr - (int64_t)jj * G_);
       const int64_t orow = sp.q0 + jj;
-      float mx = sm[0][rr];
+      float mx = sR[0][rr];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sm[i][rr]);
+      for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sR[i][rr]);
       float f[NW], lsum = 0.f;
 #pragma unroll
       for (int i = 0; i < NW; ++i) {       // a wave without keys has l = 0, O = 0
-        f[i] = sm[i][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[i][rr] - mx) * a.c);
+        f[i] = u.factor(sR[i][rr], mx);
         lsum += f[i] * sl[i][rr];
       }
       const float inv = a.parts > 1 ? 1.f : lsum == 0.f ? 0.f : 1.f / lsum;
       const int64_t at = ((int64_t)part * a.s.q_rows + orow) * a.heads + ho;
-      if (a.parts > 1 && e0 == 0) a.part_ml[at] = make_float2(mx == -INFINITY ? mx : mx * a.c, lsum);
+      if (a.parts > 1 && e0 == 0) a.part_rl[at] = make_float2(mx, lsum);
       T* out = static_cast<T*>(a.out) + orow * a.o_ld + ho * a.o_hd;
       for (int e = e0; e < a.dim; e += 8 * NW) {
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
@@ -754,17 +784,18 @@ __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
   const SeqSpan sp = seq_span(a.s, sq);
   if (row < sp.q0 || row >= sp.q0 + sp.q_len) return;
   const int64_t step = (int64_t)a.s.q_rows * a.heads;
-  float mx = -INFINITY;
+  const Log2 u(a.c);
+  float mx = kNone;
 #pragma unroll 4
-  for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.part_ml[p * step + id].x);
+  for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.part_rl[p * step + id].x);
   float l = 0.f;
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int p = 0; p < a.parts; ++p) {
-    const float2 ml = a.part_ml[p * step + id];
+    const float2 rl = a.part_rl[p * step + id];
     const f32x4_t o = *reinterpret_cast<const f32x4_t*>(a.part_o + (p * step + id) * a.dim + e);
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);   // no key seen: l, O are 0
-    l += f * ml.y;
+    const float f = u.factor(rl.x, mx);          // (no key seen: l, O are 0)
+    l += f * rl.y;
     v += f * o;
   }
   v *= l == 0.f ? 0.f : 1.f / l;
