@@ -524,6 +524,29 @@ def test_attention_scores_far_from_zero(dtype, base, step, q_len, past, heads, k
     inside(got, ref, (size + ref.abs()) * (u + 64 * F) * 1.02 + size * (2 * n + 70) * F + ref.abs() * U[dtype] * 1.01)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q_len,past,heads,kv,dim", LARGE[:5])
+def test_attention_scores_all_minus_infinity(dtype, q_len, past, heads, kv, dim):
+    """A query all of whose keys score -inf has no weights: NaN, not the 0 of one that sees no key; such keys
+    weigh nothing beside others."""
+    import torch
+    for lost in (5, past + 5, q_len + past):              # keys from the first on that score -inf
+        lost = min(lost, q_len + past)
+        n_k = past + max(q_len - 3, 1)                    # a prompt's first queries see none
+        lost = min(lost, n_k)
+        starts, k_at, k_len = [0, q_len], [2], [n_k]
+        q, k, v = randn(q_len, heads, dim, dtype=dtype, seed=1), randn(n_k + 4, kv, dim, dtype=dtype, seed=2), \
+            randn(n_k + 4, kv, dim, dtype=dtype, seed=3)
+        q[..., 1] = 1.0
+        out = torch.zeros_like(q)
+        seqs = vrs.seqs(i32(starts), i32(k_at), i32(k_len), max_q=q_len, max_k=n_k)
+        ref, tol = attention_ref(q, k, v, starts, [n_k - lost], [2 + lost], True, dim ** -0.5, out, dtype)
+        sees = n_k - q_len + torch.arange(q_len, device="cuda") + 1      # keys of each query
+        ref[(sees > 0) & (sees <= lost)] = math.nan
+        k[2:2 + lost, :, 1] = -math.inf
+        inside(ctx().attention(q, k, v, seqs, out=out), ref, tol)
+
+
 def test_attention_strided():
     """Queries, keys and values of one product; heads outermost; a repeated head."""
     import torch

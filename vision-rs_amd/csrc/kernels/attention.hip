@@ -77,6 +77,10 @@ struct Log2 {
   }
 };
 
+// 1 / l; where no key weighs anything, 0 for a query that sees none and NaN for one all of whose keys
+// score -inf.
+__device__ __forceinline__ float share(float l, int keys) { return l == 0.f ? (keys > 0 ? NAN : 0.f) : 1.f / l; }
+
 // A buffer resource in scalar registers, for load_lds.
 __device__ __forceinline__ i32x4_hw lds_rsrc(const void* base, int bytes) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);
@@ -294,10 +298,10 @@ struct Wave {
       }
   }
 
-  // O / l of the lane's query to `out` (element type), `dim` elements; no key seen: zeros
+  // O / l of the lane's query to `out` (element type), `dim` elements
   __device__ __forceinline__ void store(int q, T* out, int dim, bool ok) const {
     const float lt = sum32(l[q]);
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float inv = share(lt, lim[q]);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
       if constexpr (sizeof(T) == 4) {
@@ -742,7 +746,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
         f[i] = u.factor(sR[i][rr], mx);
         lsum += f[i] * sl[i][rr];
       }
-      const float inv = a.parts > 1 ? 1.f : lsum == 0.f ? 0.f : 1.f / lsum;
+      const float inv = a.parts > 1 ? 1.f : share(lsum, visible(sp, jj, a.causal));
       const int64_t at = ((int64_t)part * a.s.q_rows + orow) * a.heads + ho;
       if (a.parts > 1 && e0 == 0) a.part_rl[at] = make_float2(mx, lsum);
       T* out = static_cast<T*>(a.out) + orow * a.o_ld + ho * a.o_hd;
@@ -798,7 +802,7 @@ __device__ __forceinline__ void join_body(const vrs_attention_args& a) {
     l += f * rl.y;
     v += f * o;
   }
-  v *= l == 0.f ? 0.f : 1.f / l;
+  v *= share(l, visible(sp, (int)(row - sp.q0), a.causal));
   T* out = static_cast<T*>(a.out) + row * a.o_ld + h * a.o_hd + e;
   if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4_t*>(out) = v;
   else *reinterpret_cast<u32x2_t*>(out) = (u32x2_t){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
