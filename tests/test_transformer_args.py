@@ -219,3 +219,11 @@ def test_packed_descriptors_have_the_structures_layout():
     assert vrs._ROPE(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 0.5, *range(14, 27)) == bytes(rope_d)
     att_d = vrs.AttentionDesc(1, 2, 3, 4, 5, 6, 7, 0.5, *range(8, 16))
     assert vrs._ATTENTION(1, 2, 3, 4, 5, 6, 7, 0.5, *range(8, 16)) == bytes(att_d)
+
+
+def test_workspace_of_more_sequences_than_an_int_counts_groups():
+    """Sequences times key heads past 2^31: split as any other that fill the card, in four parts."""
+    d = vrs.AttentionDesc(q_rows=1, k_rows=1 << 20, heads=4, kv_heads=4, head_dim=64, dtype=vrs.BF16, causal=1, scale=0.0,
+                          q_ld=256, q_hd=64, k_ld=256, k_hd=64, v_ld=256, v_hd=64, o_ld=256, o_hd=64)
+    size = lambda n: vrs.lib().vrs_attention_workspace_size(C.byref(d), C.byref(vrs.Seqs(FAKE, FAKE, FAKE, n, 1, 1 << 20)))   # noqa: E731
+    assert size(1 << 20) == size(1 << 30) == 4 * 4 * (64 + 2) * 4

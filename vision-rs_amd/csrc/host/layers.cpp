@@ -288,7 +288,7 @@ AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
     // a part, four parts at most beyond that, so that long and short sequences even out.  Measured in
     // bfloat16 at head_dim 128: 64 tokens over 500 .. 8000 keys, 512 workgroups: 1 part 278 us, 2 246,
     // 4 236, 8 254; one token, 8 key heads, 4000 keys: 192 keys a part 14.5 us, 256 16.5, 384 16.8.
-    const int64_t wgs = std::max<int64_t>(1, s->n * d->kv_heads * p.row_tiles);
+    const int64_t wgs = std::max<int64_t>(1, n * d->kv_heads * p.row_tiles);
     p.parts = (int)std::clamp<int64_t>(std::min(std::max<int64_t>(4, 512 / wgs), mk / 192), 1, 64);
     // short ones: eight waves and no second launch (head_dim 128, 300 keys: 9.6 us against 10.2, 700:
     // 13.7 against 12.6; head_dim 64, 700: 8.5 against 9.5)
