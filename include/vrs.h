@@ -468,7 +468,10 @@ int vrs_rope_freqs(int32_t pairs, double base, int32_t scaling, double factor, d
  * is): row by row without seqs; with seqs, at the rows of the sequence's keys
  * that vrs_attention with the same seqs reads, i.e. appended to the cache
  * (rows whose place lies outside k_out are not written; sequences must not
- * share rows of it).  q_out may be q and k_out may be k, with the same
+ * share elements of it).  A cache [sequence][kv_heads][room][head_dim] is one of
+ * k_out_rows = (sequences * kv_heads - (kv_heads - 1)) * room with ko_ld =
+ * head_dim, ko_hd = room * head_dim and k_start[i] = i * kv_heads * room, for
+ * vrs_attention too.  q_out may be q and k_out may be k, with the same
  * strides; k_out must not be k where rows move.  heads or kv_heads may be 0.
  * rot even, <= 512, <= head_dim <= 4096. */
 #define VRS_ROPE_HALF 0

@@ -277,6 +277,29 @@ def test_rope_into_a_cache(dtype, dim, rot, case):
     assert torch.equal(vo.double(), rv)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rope_into_a_cache_with_heads_outside_rows(dtype):
+    """A cache [sequence, head, room, dim], filled and read through strides: the bits of one with rows of heads."""
+    import torch
+    n, kv, room, dim, q_len, past = 3, 2, 40, 64, [3, 1, 8], [0, 39, 20]
+    starts = [0, 3, 4, 12]
+    k_len = [a + b for a, b in zip(q_len, past)]
+    qkv = randn(12, 4 + 2 * kv, dim, dtype=dtype, seed=1)
+    q, k, v = qkv[:, :4], qkv[:, 4:4 + kv], qkv[:, 4 + kv:]
+    freq = vrs.rope_freqs(dim // 2).cuda()
+    kc, vc = randn(n, kv, room, dim, dtype=dtype, seed=2), randn(n, kv, room, dim, dtype=dtype, seed=3)
+    rows = [t.transpose(1, 2).reshape(n * room, kv, dim).clone() for t in (kc, vc)]
+    view = [t.as_strided(((n * kv - (kv - 1)) * room, kv, dim), (dim, room * dim, 1)) for t in (kc, vc)]
+    outs = []
+    for (ko, vo), per in ((rows, room), (view, kv * room)):
+        s = vrs.seqs(i32(starts), i32([i * per for i in range(n)]), i32(k_len), max_q=8, max_k=room)
+        qo, _ = ctx().rope(q, k, freq, seqs=s, k_out=ko, v=v, v_out=vo)
+        outs += [qo, ctx().attention(qo, ko, vo, s)]
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    for a, b in zip((kc, vc), rows):
+        assert torch.equal(a, b.view(n, room, kv, dim).transpose(1, 2))
+
+
 def test_rope_writes_no_row_outside_the_cache():
     """Starts, lengths and rows that do not fit the buffers are cut off."""
     import torch

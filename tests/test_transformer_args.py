@@ -87,6 +87,13 @@ def test_rope_refuses(ctx, code, kw):
     assert rc == code and "vrs_rope" in msg, (rc, msg)
 
 
+@pytest.mark.parametrize("kw", [dict(ko_ld=32), dict(ko_hd=32), dict(v=5 * FAKE, vo=6 * FAKE, vo_ld=63), dict(v=5 * FAKE, vo=6 * FAKE, vo_hd=0)])
+def test_rope_refuses_caches_that_fold(ctx, kw):
+    """Rows of one head, or heads of one row, on each other, wherever k_start puts them."""
+    rc, msg = rope(ctx, seqs=MOVED, **dict(dict(kv_heads=2, k_ld=128, ko_ld=64, ko_hd=256, vo_ld=64, vo_hd=256, k_out_rows=20), **kw))
+    assert rc == -2 and "fold" in msg, (rc, msg)
+
+
 def test_rope_of_no_rows_is_nothing(ctx):
     assert rope(ctx, rows=0)[0] == 0
     assert rope(ctx, rows=0, q=None, k=None, qo=None, ko=None)[0] == 0

@@ -197,9 +197,15 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
   for (int64_t s : {d->q_ld, d->q_hd, d->k_ld, d->k_hd, d->v_ld, d->v_hd, d->qo_ld, d->qo_hd, d->ko_ld, d->ko_hd,
                     d->vo_ld, d->vo_hd})
     if (s < 0 || s >> 40) return fail(VRS_EBADSHAPE, "%s: stride %lld", me, (long long)s);
+  // Rows that go where k_start says may leave gaps between sequences in which other heads lie (a cache with
+  // the heads outside each sequence's rows): there the strides alone show no fold, but of one row or one head.
+  auto folds = [&](int64_t ld, int64_t hd) {
+    if (seqs && seqs->k_start)
+      return (d->k_out_rows > 1 && ld < d->head_dim) || (d->kv_heads > 1 && hd < d->head_dim);
+    return !apart(ld, hd, d->k_out_rows, d->kv_heads, d->head_dim);
+  };
   if ((d->heads && !apart(d->qo_ld, d->qo_hd, d->rows, d->heads, d->head_dim)) ||
-      (d->kv_heads && !apart(d->ko_ld, d->ko_hd, d->k_out_rows, d->kv_heads, d->head_dim)) ||
-      (v && !apart(d->vo_ld, d->vo_hd, d->k_out_rows, d->kv_heads, d->head_dim)))
+      (d->kv_heads && folds(d->ko_ld, d->ko_hd)) || (v && folds(d->vo_ld, d->vo_hd)))
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
   if (d->heads && q == q_out && (d->q_ld != d->qo_ld || d->q_hd != d->qo_hd))
     return fail(VRS_EBADSHAPE, "%s: q_out is q with other strides", me);
