@@ -613,6 +613,21 @@ def test_attention_not_finite_in_masked_places(dtype, case):
     check_attention(case, dtype, 4, 2, 64, True, edit=lowest)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [8, 24, 40, 56, 72, 80, 96, 120])
+def test_attention_narrow_heads_after_full_ones(dtype, dim):
+    """What earlier kernels left in LDS does not reach heads narrower than their tile."""
+    import torch
+    for case, big in ((([200, 33], None, None), ([9000, 9000], None, None)), (([1, 2], [700, 40], [0, 800]), ([1] * 300, [64] * 300, list(range(300))))):
+        starts, rows, k_len, k_at, s = build(big)
+        n_k = max(rows, max(a + n for a, n in zip(k_at, k_len)))
+        nan = torch.full((n_k, 4, 128), math.nan, dtype=tdt(dtype), device="cuda")
+        for _ in range(2):         # prompts: a workgroup to each CU at least, and in it 96 KB, the most that these use
+            assert ctx().attention(torch.ones_like(nan[:rows]), nan, nan, s, causal=False)[starts[0]:starts[-1]].isnan().all()
+        for causal in (True, False):
+            check_attention(case, dtype, 4, 2, dim, causal)
+
+
 def test_attention_nan_keys():
     """A NaN key: NaN for the queries that see it, nothing for the others."""
     import torch
