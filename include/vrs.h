@@ -499,10 +499,10 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
  * or before the query's own place (see vrs_seqs: the queries are the last of
  * their sequence, so a prompt, a later piece of one over a cache, and a single
  * new token are the same call).  A query that sees no key gets 0, one whose
- * keys all score -infinity NaN; keys it does
- * not see, and whatever lies behind a sequence's keys, do not touch its result
- * even where they hold NaN.  head_dim: a multiple of 8 up to 128; q, k, v, out
- * and their strides 16-byte aligned, row strides under 4 M elements.  Scores,
+ * keys all score -infinity NaN; keys it does not see, and whatever lies behind
+ * a sequence's keys, do not touch its result even where they hold NaN.
+ * head_dim: a multiple of 8 up to 128; q, k, v, out and their strides 16-byte
+ * aligned, row strides under 4 M elements, k_rows up to 2^31 - 1024.  Scores,
  * softmax and sums are float32 (scores of any size that twice log2(e) times
  * scale leaves in its range); bfloat16 rounds the probabilities once.
  * Results do not depend on the run (fixed order of every sum), but the kernel

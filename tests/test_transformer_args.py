@@ -182,6 +182,18 @@ def test_attention_refuses(ctx, code, kw):
     assert rc == code and "vrs_attention" in msg, (rc, msg)
 
 
+def test_attention_refuses_keys_past_its_indexes(ctx):
+    """Key numbers are int32 and run up to 2^9 past a sequence's last key."""
+    rc, msg = attention(ctx, k_rows=(1 << 31) - 512, kv_heads=2)
+    assert rc == -3 and "rows" in msg, (rc, msg)
+    d = vrs.AttentionDesc(q_rows=1, k_rows=(1 << 31) - 1, heads=4, kv_heads=1, head_dim=64, dtype=vrs.BF16, causal=1, scale=0.0,
+                          q_ld=256, q_hd=64, k_ld=64, k_hd=64, v_ld=64, v_hd=64, o_ld=256, o_hd=64)
+    size = lambda: vrs.lib().vrs_attention_workspace_size(C.byref(d), C.byref(vrs.Seqs(FAKE, FAKE, FAKE, 1, 1, 0)))   # noqa: E731
+    assert size() == 0
+    d.k_rows = (1 << 31) - 1024
+    assert size() > 0
+
+
 def test_attention_of_nothing_is_nothing(ctx):
     assert attention(ctx, q_rows=0)[0] == 0
     assert attention(ctx, q_rows=0, q=None, out=None)[0] == 0

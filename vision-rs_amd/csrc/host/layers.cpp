@@ -258,6 +258,8 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
   if (rc || (rc = check_seqs(seqs, me))) return rc;
   if (d->q_rows < 0 || d->k_rows < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads)
     return fail(VRS_EBADSHAPE, "%s: %d and %d rows, %d heads on %d", me, d->q_rows, d->k_rows, d->heads, d->kv_heads);
+  // the kernels' key numbers run on to the end of the tiles ahead, 512 at most past the last key
+  if (d->k_rows > 0x7fffffff - 1023) return fail(VRS_EUNSUPPORTED, "%s: %d key rows", me, d->k_rows);
   if (d->head_dim < 8 || d->head_dim % 8 || d->head_dim > 128)
     return fail(VRS_EUNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 128)", me, d->head_dim);
   if (!(d->scale >= 0.f && d->scale <= 1e30f)) return fail(VRS_EINVAL, "%s: scale %g", me, (double)d->scale);
