@@ -293,11 +293,15 @@ AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   if (p.few) {
     p.row_tiles = (mq * group + 31) / 32;
     // Workgroups of four waves, two on a CU at once: two of each wherever there are enough keys for 192
-    // a part, four parts at most beyond that, so that long and short sequences even out.  Measured in
-    // bfloat16 at head_dim 128: 64 tokens over 500 .. 8000 keys, 512 workgroups: 1 part 278 us, 2 246,
-    // 4 236, 8 254; one token, 8 key heads, 4000 keys: 192 keys a part 14.5 us, 256 16.5, 384 16.8.
+    // a part.  bfloat16, bound by memory, takes four parts beyond that, so that long and short sequences
+    // even out; float32, bound by the matrix instructions that most of a row tile spends on no row, does
+    // not gain.  Measured, head_dim 128, 8 key heads: bfloat16, 64 tokens over 500 .. 8000 keys, 512
+    // workgroups: 1 part 278 us, 2 246, 4 236, 8 254; one token, 4000 keys: 192 keys a part 14.5 us, 256
+    // 16.5, 384 16.8.  float32, the same 64 tokens: 1 part 475 us, 2 516, 4 574; 64 over 500 .. 2000: 1 183,
+    // 2 209, 4 246; 16 over 500 .. 8000: 2 208, 4 158, 8 166; one, 4000 keys: 128 keys a part 36 us, 192 30.
     const int64_t wgs = std::max<int64_t>(1, n * d->kv_heads * p.row_tiles);
-    p.parts = (int)std::clamp<int64_t>(std::min(std::max<int64_t>(4, 512 / wgs), mk / 192), 1, 64);
+    const int64_t least = d->dtype == VRS_BF16 ? 4 : 1;
+    p.parts = (int)std::clamp<int64_t>(std::min(std::max(least, 512 / wgs), mk / 192), 1, 64);
     // short ones: eight waves and no second launch (head_dim 128, 300 keys: 9.6 us against 10.2, 700:
     // 13.7 against 12.6; head_dim 64, 700: 8.5 against 9.5)
     if (d->dtype == VRS_BF16 && wgs <= 256 && mk * (d->head_dim <= 64 ? 64 : 128) <= 1 << 16) p.waves = 8, p.parts = 1;
