@@ -399,8 +399,9 @@ int vrs_msda(vrs_ctx* ctx, const vrs_msda_desc* d, const float* value, const flo
  *   group == cols:  one scale per row, max|y| / 448 (1 where that is 0: a zero
  *                   row, or one below 3.2e-43, all of whose e4m3 values are 0)
  *   32, 64 or 128:  one per that many columns (cols a multiple of it)
- * stored in scales[rows][cols / group].  NaN elements do not count in a
- * maximum and stay NaN.  cols <= 32768.  e4m3 needs 16-byte aligned rows
+ * stored in scales[rows][cols / group], for a program's own products: those of
+ * this library take one step for a tensor (group 0).  NaN elements do not count
+ * in a maximum and stay NaN.  cols <= 32768.  e4m3 needs 16-byte aligned rows
  * (x, res, sum and y) and cols % 16 == 0; others take any alignment of their
  * elements and are fastest at 16 bytes.  weight: float32 [cols]. */
 typedef struct {

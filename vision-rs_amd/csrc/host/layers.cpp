@@ -290,10 +290,11 @@ AttentionPlan plan_attention(const vrs_attention_desc* d, const vrs_seqs* s) {
   p.qt = 1;
   p.waves = 4;
   // Rows of a key head that fit one row tile, or two of them where that still leaves workgroups few, or in
-  // float32; the prompts' kernel reads the keys once for 128 rows.  Measured, head_dim 128, 8 key heads, 2000
-  // keys, 64 rows, bfloat16: one sequence 17.5 us against the prompts' 18.2, 8 sequences 30.5 against 26.2, 64
-  // 281 against 97; float32, 64 sequences: 496 against 532.  32 rows: bfloat16, one 17.0 against 17.7, 64 141
-  // against 95; 64 of 300 keys 21.4 against 19.3, but head_dim 64 13.5 against 14.2; float32, 64: 333 against 528.
+  // float32; the prompts' kernel takes 128 rows and more.  Measured against it, 8 key heads of 128, bfloat16:
+  // one token of 64 sequences over 500 .. 8000 keys 250 us against 305, over 8000 each 425 against 509, over
+  // 2000 each 121 against 94; of one over 2000 17.1 against 17.7.  64 rows (16 queries of 4 heads) over 2000
+  // keys: one sequence 17.5 against 18.2, 8 30.5 against 26.2, 64 281 against 97.  float32: the 64 tokens 537
+  // against 2418, 64 rows of 64 sequences 496 against 532.
   p.few = mq * group <= 32 || (mq * group <= 64 && (n * d->kv_heads <= 64 || d->dtype == VRS_F32));
   if (p.few) {
     p.row_tiles = (mq * group + 31) / 32;

@@ -435,12 +435,13 @@ __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group
 // little and the keys serve the whole group), a wave 32 * QT of them; K and V
 // tiles of KT keys are shared through LDS.
 //
-// Per 32 keys x 32 queries at D = 128 the matrix cores are busy for 512 cycles
-// of a SIMD, its exponentials and the rest of the softmax take about 300 and
-// the operand reads from LDS 512 / QT (K and V fragments serve QT query
-// tiles).  So the loop is a software pipeline: the next 32 keys' scores are
-// multiplied while these 32 keys' exponentials are taken, and P V while the
-// next maximum is.
+// The loop is written as a software pipeline: the next 32 keys' scores are
+// multiplied between these 32 keys' maximum and their exponentials, so that
+// neither kind of instruction waits for the other's results.  Measured per 32
+// keys x 32 queries and SIMD: 512 cycles of matrix instructions and 459 of
+// vector ones in 1020 at D = 128, 256 and 475 in 713 at D = 64: close to their
+// sums, so the waves of a SIMD hardly overlap one kind with the other, and
+// neither unit is full (50 and 45 % at 128, 36 and 67 % at 64).
 //
 // LDS holds three tiles, filled by loads that go straight there: one barrier
 // before tile i's last 32 keys (whose step reads tile i + 1's first scores)
@@ -449,16 +450,17 @@ __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group
 // take the general form of the step; the others three at a time, so that LDS
 // addresses are constants.
 //
-// 8192 causal queries, 32 heads on 8 of 128: 500 .. 525 us (the clock differs
-// between cards), 1050 .. 1100 TFLOP/s; an 8192^3 product reaches 1110.  The
-// matrix cores are busy 53 % of the cycles, the VALU 45 %, at 1.84 GHz, without
-// LDS bank conflicts; 8 waves and 64-key tiles against 4 waves and 32: 516 us to
-// 548.  At head sizes up to 64 the same exponentials serve half the products
-// and the VALU is the busier (64 % against 36 %): 24 images of 196 .. 1600
-// patches, 12 heads: 122 .. 128 us, 715 TFLOP/s; four 4-wave workgroups on a CU with
+// 8192 causal queries, 32 heads on 8 of 128: 503 .. 525 us queued (cards and
+// their clock under this load differ), 1045 .. 1095 TFLOP/s; an 8192^3 product
+// reaches 1110 .. 1160.  Traced one by one: 568 us at 1.86 GHz, 1.05 M cycles,
+// rising to 670 as the clock falls to 1.52.  No LDS bank conflicts.  8 waves and
+// 64-key tiles against 4 waves and 32: 516 us to 548.  At head sizes up to 64 the
+// same exponentials serve half the products: 24 images of 196 .. 1600 patches,
+// 12 heads: 120 .. 128 us, 700 TFLOP/s; four 4-wave workgroups on a CU with
 // 32-key tiles against three with 64: 124 us to 130; two query tiles to a wave
-// for the large (4096 x 32 heads: 148 us to 159).  float32 is bound by its
-// matrix instructions (64 cycles each).
+// for the large (4096 x 32 heads: 148 us to 159).  Heads of 72 .. 120 run padded
+// to 128 (64 sequences of 512, 16 heads: 64 113 us, 72 177, 80 180, 96 191, 128
+// 207).  float32 is bound by its matrix instructions (64 cycles each).
 template <typename T, int D, int KT, int QT, int NW>
 __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
   constexpr int NT = 64 * NW, BM = 32 * NW * QT, NS = KT / 32;
