@@ -60,7 +60,6 @@ struct Log2 {
       : c(c_), w(__uint_as_float((__float_as_uint(c_) + 0x7fffffu) & 0x7f800000u)) {}
   static __device__ __forceinline__ bool far(float R) { return !(fabsf(R) < kFar); }
   __device__ __forceinline__ float unit(float R) const { return far(R) ? w : c; }
-  __device__ __forceinline__ float exponent(float s, float R) const { return __builtin_fmaf(s, unit(R), -R); }
   __device__ __forceinline__ float reference(float m) const {
     const float R = m * c;
     return far(R) ? m * w : R;
@@ -126,15 +125,17 @@ struct Wave {
   G qf[QT][D / 16];
   f32x16_t o[QT][D / 32];
   float R[QT], l[QT];   // reference (see Log2) and this lane's share of the sum
+  float unit[QT];       // c or w, as R has it (8192 causal queries: 503 us, 507 where each tile asks R)
   int lim[QT];          // keys that the lane's query sees
   int l32, hh;
 
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void init(const Log2& u) {
     l32 = threadIdx.x & 31;
     hh = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
       R[q] = kNone;
+      unit[q] = u.w;
       l[q] = 0.f;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t)
@@ -168,13 +169,14 @@ struct Wave {
   __device__ __forceinline__ void follow(const float (&t)[QT], const Log2& u) {
     bool over = false;
 #pragma unroll
-    for (int q = 0; q < QT; ++q) over |= u.exponent(t[q], R[q]) > kTau;
+    for (int q = 0; q < QT; ++q) over |= __builtin_fmaf(t[q], unit[q], -R[q]) > kTau;
     if (__any(over)) {
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-        const float to = u.exponent(t[q], R[q]) > 0.f ? u.reference(t[q]) : R[q];
+        const float to = __builtin_fmaf(t[q], unit[q], -R[q]) > 0.f ? u.reference(t[q]) : R[q];
         const float alpha = u.factor(R[q], to);
         R[q] = to;
+        unit[q] = u.unit(to);
         l[q] *= alpha;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) o[q][d] *= alpha;
@@ -188,15 +190,15 @@ struct Wave {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p.u[i] = pack_bf16x2(__builtin_amdgcn_exp2f(u.exponent(s[2 * i], R[q])),
-                             __builtin_amdgcn_exp2f(u.exponent(s[2 * i + 1], R[q])));
+        p.u[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], unit[q], -R[q])),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], unit[q], -R[q])));
         l[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v_t, p.u[i]),
                                                __builtin_bit_cast(bf16x2v_t, 0x3f803f80u), l[q], false);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(u.exponent(s[r], R[q]));
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit[q], -R[q]));
         p.u[r] = __float_as_uint(e);
         l[q] += e;
       }
@@ -450,8 +452,8 @@ __device__ __forceinline__ TilePlace place_tile(const vrs_seq_args& s, int group
 // take the general form of the step; the others three at a time, so that LDS
 // addresses are constants.
 //
-// 8192 causal queries, 32 heads on 8 of 128: 503 .. 525 us queued (cards and
-// their clock under this load differ), 1045 .. 1095 TFLOP/s; an 8192^3 product
+// 8192 causal queries, 32 heads on 8 of 128: 500 .. 540 us queued (cards and
+// their clock under this load differ), 1020 .. 1100 TFLOP/s; an 8192^3 product
 // reaches 1110 .. 1160.  Traced one by one: 568 us at 1.86 GHz, 1.05 M cycles,
 // rising to 670 as the clock falls to 1.52.  No LDS bank conflicts.  8 waves and
 // 64-key tiles against 4 waves and 32: 516 us to 548.  At head sizes up to 64 the
@@ -485,7 +487,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a) {
 
   const Log2 u(a.c);
   Wave<T, D, QT> w;
-  w.init();
+  w.init(u);
   int64_t qrow[QT];
   int head[QT];
   bool ok[QT];
@@ -653,7 +655,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a) {
   // row tiles of the sequence, one workgroup each (and more than were counted on, in turn)
   for (int64_t r0 = blockIdx.y * 32; r0 < rows; r0 += gridDim.y * 32) {
     Wave<T, D, 1> w;
-    w.init();
+    w.init(u);
     const int64_t pr = min(r0 + w.l32, rows - 1);
     const bool ok = r0 + w.l32 < rows;
     const int j = (int)(pr / G_), h = hk * G_ + (int)(pr - (int64_t)j * G_);
