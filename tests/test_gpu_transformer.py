@@ -486,6 +486,15 @@ def test_attention_given_workspace():
     assert e.value.code == -1
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 2, 128)])
+def test_attention_pieces_and_tokens_in_one_call(dtype, heads, kv, dim):
+    """A prompt, pieces and single tokens over long and short caches: workgroups most of whose waves have no row."""
+    case = ([1, 300, 1, 70, 1, 5, 1], [2500, 0, 900, 1500, 0, 40, 130], [0, 2600, 3000, 4000, 5700, 5800, 5900])
+    for causal in (True, False):
+        check_attention(case, dtype, heads, kv, dim, causal)
+
+
 def test_attention_hints_choose_kernels_only():
     """Unknown, too small and too large hints: right results of every kernel."""
     import torch
