@@ -524,6 +524,133 @@ size_t vrs_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs*
 int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seqs, const void* q, const void* k,
                   const void* v, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- generation from a cache -------------------------------------------------
+ * What a program that continues prompts needs beside vrs_attention: requests
+ * whose sequences share a prefix, the step of a beam search, and caches cut to
+ * the keys that matter.  No counterpart in the reference. */
+
+/* Groups of sequences that share a prefix: the sequences first[g] ..
+ * first[g + 1] - 1 of a vrs_seqs (first does not fall; a group may be empty;
+ * sequences before the first and behind the last group have no prefix) begin
+ * with the k_len[g] keys in the rows from k_start[g], and their own keys, those
+ * of the vrs_seqs, follow.  All three are DEVICE arrays, read by the kernels;
+ * what they say outside the buffers is cut off.
+ * max_rows: the most queries of all sequences of a group together, max_k: the
+ * most keys of a prefix, 0 if unknown; they choose among kernels for speed, and
+ * any value gives right results. */
+typedef struct {
+  const int32_t* first;    /* [n + 1] */
+  const int32_t* k_start;  /* [n] */
+  const int32_t* k_len;    /* [n] */
+  int32_t n;
+  int32_t max_rows, max_k;
+} vrs_prefixes;
+
+/* vrs_attention where the keys of a sequence are its group's prefix and then its
+ * own.  Every query sees the whole prefix; causal is about the own keys.  The
+ * descriptor, the buffers (k and v hold prefixes and own keys), their
+ * alignment, the rounding and the workspace are vrs_attention's, and so is the
+ * result: a query that sees no key gets 0.  A prefix is read once for up to 128
+ * rows (queries times heads of a key head) of its group instead of once for each
+ * sequence. */
+size_t vrs_prefix_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs* seqs,
+                                           const vrs_prefixes* prefixes);
+int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seqs, const vrs_prefixes* prefixes,
+                         const void* q, const void* k, const void* v, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Beam search's selection: for each request (batch entry) the k best of the
+ * candidates (beam i, token t),
+ *   c = scores[i] + (logits[i][t] - lse_i),  lse_i = log sum_t exp(logits[i][t])
+ * in falling order, equal ones by the lowest i * vocab + t; candidates of one beam
+ * are in the order of their logits.  lse comes from float32 exponentials summed in
+ * 64 bits and c is compared in 64 bits, out_scores rounds it once.  done (may be
+ * NULL): a beam whose byte is not 0 is at its end and goes on with the token `eos`
+ * alone, c = scores[i].  A candidate whose c is not a number counts as -infinity:
+ * tokens with a logit of -infinity, all others of a beam at its end, and every
+ * token of a beam whose score is not finite or whose logits hold a NaN or
+ * +infinity, or nothing else than -infinity.
+ * logits: rows (beams of all requests, one after another) of contiguous elements,
+ * ld elements apart, of any alignment of their elements.  k <= 128 and
+ * <= beams * vocab, beams <= 64, beams * vocab < 2^31.
+ * workspace: 16-byte aligned, vrs_beam_select_workspace_size bytes; a call uses it
+ * until its kernels end. */
+typedef struct {
+  int32_t batch, beams, vocab, k;
+  int32_t dtype;           /* VRS_BF16 or VRS_F32: logits */
+  int32_t eos;             /* 0 .. vocab - 1, with done */
+  int64_t ld;              /* elements between rows of logits */
+} vrs_beam_desc;
+size_t vrs_beam_select_workspace_size(const vrs_beam_desc* d);
+int vrs_beam_select(vrs_ctx* ctx, const vrs_beam_desc* d, const void* logits, const float* scores, const uint8_t* done,
+                    float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Reordering of the beams' states after a selection, in place: the slot of beam i
+ * receives what the slot of beam parents[i] of the same request held, in every
+ * layer.  A slot has `rows` rows of row_bytes contiguous bytes; of a slot's rows
+ * the first len[slot] move (len NULL: all; by the slot they come from), the others
+ * of a receiving slot stay as they were.  A parent outside 0 .. beams - 1 leaves its
+ * beam's slot alone.  Slots are numbered request * beams + beam.  Caches (rows of
+ * keys), lengths (one row of 4 bytes) and tokens are such states alike.  Offsets are
+ * in bytes; no two rows may overlap; fastest where all are multiples of 16.
+ * beams <= 64. */
+typedef struct {
+  int32_t batch, beams, layers, rows;
+  int64_t row_bytes, row_ld, slot_ld, layer_ld;
+} vrs_reorder_desc;
+int vrs_beam_reorder(vrs_ctx* ctx, const vrs_reorder_desc* d, const int32_t* parents, const int32_t* len, void* state,
+                     void* stream);
+
+/* Attention that keys receive:
+ *   acc[j, g] = decay * acc[j, g] + sum over the queries i of the sequence and the
+ *               heads h of key head g of softmax_j(scale * q[i, h] . k[j, g])
+ * for every key j of every sequence, over the keys that a query sees as in
+ * vrs_attention (a query whose keys all score -infinity gives NaN to those it
+ * sees).  acc: float32, of key row r and key head g at acc[r * acc_ld + g * acc_hd];
+ * sequences must not share key rows.  decay 0 does not read acc.
+ * Scores, weights and sums are float32 and each sum has a fixed order.  head_dim,
+ * alignment, strides and workspace as in vrs_attention. */
+typedef struct {
+  int32_t q_rows, k_rows;
+  int32_t heads, kv_heads, head_dim, dtype;   /* VRS_BF16 or VRS_F32 */
+  int32_t causal;
+  float scale;                 /* > 0; 0: head_dim^-0.5 */
+  float decay;                 /* 0 .. 1 */
+  int64_t q_ld, q_hd, k_ld, k_hd, acc_ld, acc_hd;   /* elements between rows, between heads */
+} vrs_weights_desc;
+size_t vrs_attention_weights_workspace_size(const vrs_weights_desc* d, const vrs_seqs* seqs);
+int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seqs* seqs, const void* q, const void* k,
+                          float* acc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction from a cache: of sequence i's k_len[i] keys, for each key head by itself,
+ * the `first` first and the `recent` last stay, and of the others those with the
+ * largest acc (equal ones: the earliest; NaN counts as the largest) until `budget`
+ * keys are left; up to `budget` keys all stay.  They keep their order: kept key j of
+ * the sequence moves to row out_start[i] + j (out_start NULL: k_start) of k_out,
+ * v_out and acc_out, which may be k, v and acc themselves, with the same strides and
+ * without out_start, but must not overlap them otherwise.  Rows behind the kept ones
+ * stay as they were.
+ * kept [n][kv_heads][budget] receives the places of the kept keys (-1 behind them),
+ * len_out [n] (may be k_len; NULL: not stored) min(k_len, budget).  k_start, k_len,
+ * out_start are DEVICE arrays; what they say outside the buffers is cut off.
+ * Sequences must not share rows.  k and v: any alignment of their elements, fastest
+ * at 16 bytes.  acc as in vrs_attention_weights.  max_k: the most keys of a sequence,
+ * 0 if unknown (for speed alone).  Keys keep the rotary positions that they have:
+ * give vrs_rope positions of its own afterwards. */
+typedef struct {
+  int32_t n;                   /* sequences */
+  int32_t k_rows, out_rows;
+  int32_t kv_heads, head_dim, dtype;
+  int32_t budget, first, recent, max_k;
+  /* elements between rows, between heads */
+  int64_t k_ld, k_hd, v_ld, v_hd, acc_ld, acc_hd;
+  int64_t ko_ld, ko_hd, vo_ld, vo_hd, acco_ld, acco_hd;
+} vrs_evict_desc;
+int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_start, const int32_t* k_len,
+                    const int32_t* out_start, const void* k, const void* v, const float* acc, void* k_out, void* v_out,
+                    float* acc_out, int32_t* len_out, int32_t* kept, void* stream);
+
 /* ---- models (layer closures + graph runtime) ------------------------------ */
 #define VRS_BLOCK_CONV 1        /* conv / conv_bn / dwconv / conv_plain (blocks/conv.rs) */
 #define VRS_BLOCK_C3K2 2        /* c3k2 (blocks/c3k2.rs:94-127) */

@@ -7,53 +7,9 @@
 #include <cstring>
 #include <tuple>
 
-#include "vrs_internal.h"
+#include "layers.h"
 
 using namespace vrs;
-
-namespace {
-
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-int check_type(int dtype, const char* what) {
-  if (dtype == VRS_BF16 || dtype == VRS_F32) return VRS_OK;
-  return fail(VRS_EUNSUPPORTED, "%s: dtype %d (VRS_BF16 or VRS_F32)", what, dtype);
-}
-
-// Element types need their own alignment whatever the kernel.
-int check_ptr(const void* p, size_t es, const char* what, const char* name) {
-  if (!p) return fail(VRS_EINVAL, "%s: null %s", what, name);
-  if (!aligned(p, es)) return fail(VRS_EBADSHAPE, "%s: %s is not aligned to its elements", what, name);
-  return VRS_OK;
-}
-
-// Whether no two (row, head) of an output share an element: heads inside a row's stride, or rows
-// inside a head's.
-bool apart(int64_t ld, int64_t hd, int64_t rows, int64_t heads, int64_t dim) {
-  if (rows <= 1 && heads <= 1) return true;
-  if (rows <= 1) return hd >= dim;
-  if (heads <= 1) return ld >= dim;
-  return (hd >= dim && ld >= (heads - 1) * hd + dim) || (ld >= dim && hd >= (rows - 1) * ld + dim);
-}
-
-int check_seqs(const vrs_seqs* s, const char* what) {
-  if (s->n < 0) return fail(VRS_EBADSHAPE, "%s: %d sequences", what, s->n);
-  if (!s->q_start) return fail(VRS_EINVAL, "%s: null q_start", what);
-  if (s->max_q < 0 || s->max_k < 0) return fail(VRS_EINVAL, "%s: negative max_q or max_k", what);
-  return VRS_OK;
-}
-
-int launch(vrs_ctx* ctx, const char* name, dim3 grid, dim3 block, uint32_t lds, void* args, void* stream) {
-  hipFunction_t f;
-  if (int rc = get_fn(ctx, name, &f)) return rc;
-  void* params[] = {args};
-  hipError_t e = hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, block.x, block.y, block.z, lds,
-                                       static_cast<hipStream_t>(stream), params, nullptr);
-  if (e != hipSuccess) return fail(VRS_EHIP, "launch %s: %s", name, hipGetErrorString(e));
-  return VRS_OK;
-}
-
-}  // namespace
 
 extern "C" {
 
@@ -249,10 +205,9 @@ int vrs_rope(vrs_ctx* ctx, const vrs_rope_desc* d, const vrs_seqs* seqs, const d
 
 }  // extern "C"
 
-namespace {
+namespace vrs {
 
-int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
-  const char* me = "vrs_attention";
+int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs, const char* me) {
   if (!d || !seqs) return fail(VRS_EINVAL, "%s: null argument", me);
   int rc = check_type(d->dtype, me);
   if (rc || (rc = check_seqs(seqs, me))) return rc;
@@ -272,6 +227,21 @@ int check_attention(const vrs_attention_desc* d, const vrs_seqs* seqs) {
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
   return VRS_OK;
 }
+
+int check_attention_buffers(const vrs_attention_desc* d, const void* q, const void* k, const void* v, const void* out,
+                            const char* me) {
+  for (const auto& [p, name] : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}}) {
+    if (!p && (d->k_rows || name[0] == 'q' || name[0] == 'o')) return fail(VRS_EINVAL, "%s: null %s", me, name);
+    if (!aligned(p, 16)) return fail(VRS_EBADSHAPE, "%s: %s must be 16-byte aligned", me, name);
+  }
+  if ((d->k_rows && (out == k || out == v)) || (out == q && (d->o_ld != d->q_ld || d->o_hd != d->q_hd)))
+    return fail(VRS_EINVAL, "%s: out is an input", me);
+  return VRS_OK;
+}
+
+}  // namespace vrs
+
+namespace {
 
 // Which kernel, and into how many parts the keys are split.
 struct AttentionPlan {
@@ -356,7 +326,7 @@ size_t attention_bytes(const vrs_attention_desc* d, const AttentionPlan& p) {
 extern "C" {
 
 size_t vrs_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs* seqs) {
-  if (check_attention(d, seqs) || d->q_rows == 0 || seqs->n == 0) return 0;
+  if (check_attention(d, seqs, "vrs_attention") || d->q_rows == 0 || seqs->n == 0) return 0;
   return attention_bytes(d, plan_attention(d, seqs));
 }
 
@@ -364,15 +334,10 @@ int vrs_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seq
                   const void* v, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   const char* me = "vrs_attention";
   if (!ctx) return fail(VRS_EINVAL, "%s: null ctx", me);
-  int rc = check_attention(d, seqs);
+  int rc = check_attention(d, seqs, me);
   if (rc) return rc;
   if (d->q_rows == 0 || seqs->n == 0) return VRS_OK;
-  for (const auto& [p, name] : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {out, "out"}}) {
-    if (!p && (d->k_rows || name[0] == 'q' || name[0] == 'o')) return fail(VRS_EINVAL, "%s: null %s", me, name);
-    if (!aligned(p, 16)) return fail(VRS_EBADSHAPE, "%s: %s must be 16-byte aligned", me, name);
-  }
-  if ((d->k_rows && (out == k || out == v)) || (out == q && (d->o_ld != d->q_ld || d->o_hd != d->q_hd)))
-    return fail(VRS_EINVAL, "%s: out is an input", me);
+  if ((rc = check_attention_buffers(d, q, k, v, out, me))) return rc;
   const AttentionPlan p = plan_attention(d, seqs);
   const size_t need = attention_bytes(d, p);
   if (need) {

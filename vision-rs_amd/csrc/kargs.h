@@ -385,4 +385,67 @@ typedef struct {
   float c;                 /* scale * log2(e) */
 } vrs_attention_args;
 
+/* Attention over prefixes that groups of sequences share, then over each sequence's own keys (prefix.hip).
+ * a: the own keys; a.parts of the workspace, those of the prefixes first. */
+typedef struct {
+  vrs_attention_args a;
+  const int32_t* first;    /* [groups + 1] sequences of each group */
+  const int32_t* p_start;  /* [groups] */
+  const int32_t* p_len;    /* [groups] */
+  int32_t groups;
+  int32_t pre_parts, own_parts;
+  int32_t pre_blocks;      /* workgroups of the launch that take prefixes (in x; the others own keys) */
+  int32_t pre_rows, own_rows;   /* few rows: row tiles of either kind (in y) */
+} vrs_prefix_args;
+
+/* Attention that keys receive (weights.hip). */
+typedef struct {
+  const void *q, *k;
+  float* acc;
+  float* scores;           /* few rows: [q_rows][heads][s_ld] */
+  float2* rl;              /* [parts][q_rows][heads] reference of the weights and their sum */
+  vrs_seq_args s;
+  int64_t q_ld, q_hd, k_ld, k_hd, acc_ld, acc_hd;
+  int64_t s_ld;
+  int32_t heads, kv, dim, causal, parts;
+  float c, decay;
+} vrs_weights_args;
+
+/* Beam search's selection (beam.hip). */
+typedef struct {
+  const void* logits;
+  const float* scores;     /* [batch][beams] */
+  const uint8_t* done;     /* [batch][beams] or NULL */
+  uint2* list;             /* [batch * beams][chunks][k] the best of a chunk: logit, token; a token < 0 ends it */
+  double2* part;           /* [batch * beams][chunks] maximum and sum of exp */
+  float* out_scores;
+  int32_t *out_parents, *out_tokens;
+  int64_t ld;
+  int32_t batch, beams, vocab, k, eos, chunks, chunk;
+} vrs_beam_args;
+
+/* Reordering of beams' states (beam.hip); offsets in bytes. */
+typedef struct {
+  char* state;
+  const int32_t* parents;  /* [batch][beams] */
+  const int32_t* len;      /* [batch][beams] or NULL: all rows */
+  int64_t row_ld, slot_ld, layer_ld;
+  int32_t batch, beams, rows;
+  int32_t cols;            /* vectors of a row */
+} vrs_reorder_args;
+
+/* Eviction from a cache (evict.hip). */
+typedef struct {
+  const void *k, *v;
+  const float* acc;
+  void *ko, *vo;
+  float* acco;
+  const int32_t *k_start, *k_len, *o_start;
+  int32_t *len_out, *kept; /* kept: [n][kv][budget] */
+  int64_t k_ld, k_hd, v_ld, v_hd, ko_ld, ko_hd, vo_ld, vo_hd, acc_ld, acc_hd, acco_ld, acco_hd;
+  int32_t n, k_rows, o_rows, kv, dim, budget, first, recent;
+  int32_t slices;          /* parts of a row's vectors that workgroups share out */
+  int32_t cols;            /* vectors of a row */
+} vrs_evict_args;
+
 #endif

@@ -110,6 +110,34 @@ class AttentionDesc(C.Structure):
                 *[(n, C.c_int64) for n in ("q_ld", "q_hd", "k_ld", "k_hd", "v_ld", "v_hd", "o_ld", "o_hd")]]
 
 
+class Prefixes(C.Structure):
+    _fields_ = [("first", C.c_void_p), ("k_start", C.c_void_p), ("k_len", C.c_void_p), ("n", C.c_int32),
+                ("max_rows", C.c_int32), ("max_k", C.c_int32)]
+
+
+class BeamDesc(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("k", C.c_int32),
+                ("dtype", C.c_int32), ("eos", C.c_int32), ("ld", C.c_int64)]
+
+
+class ReorderDesc(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("beams", C.c_int32), ("layers", C.c_int32), ("rows", C.c_int32),
+                *[(n, C.c_int64) for n in ("row_bytes", "row_ld", "slot_ld", "layer_ld")]]
+
+
+class WeightsDesc(C.Structure):
+    _fields_ = [("q_rows", C.c_int32), ("k_rows", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+                ("decay", C.c_float), *[(n, C.c_int64) for n in ("q_ld", "q_hd", "k_ld", "k_hd", "acc_ld", "acc_hd")]]
+
+
+class EvictDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "k_rows", "out_rows", "kv_heads", "head_dim", "dtype", "budget", "first",
+                                         "recent", "max_k")] + \
+               [(n, C.c_int64) for n in ("k_ld", "k_hd", "v_ld", "v_hd", "acc_ld", "acc_hd",
+                                         "ko_ld", "ko_hd", "vo_ld", "vo_hd", "acco_ld", "acco_hd")]
+
+
 class BlockDesc(C.Structure):
     _fields_ = [("kind", C.c_int32), ("c_in", C.c_int32), ("c_out", C.c_int32), ("k", C.c_int32), ("s", C.c_int32),
                 ("g", C.c_int32), ("conv_kind", C.c_int32), ("n", C.c_int32), ("c3k", C.c_int32),
@@ -134,6 +162,10 @@ PLAN_FP8 = 0x10000
 _RMS = struct.Struct("5i2f4q").pack
 _ROPE = struct.Struct("9i4if13q").pack
 _ATTENTION = struct.Struct("7if8q").pack
+_BEAM = struct.Struct("6iq").pack
+_REORDER = struct.Struct("4i4q").pack
+_WEIGHTS = struct.Struct("7i2f4x6q").pack
+_EVICT = struct.Struct("10i12q").pack
 _NONE = (0, 0, 0, 0)
 
 # Every exported symbol of include/vrs.h with its ctypes signature.
@@ -173,6 +205,14 @@ SIGNATURES = {
     "vrs_rope": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vrs_attention_workspace_size": (_sz, [_vp, _vp]),
     "vrs_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vrs_prefix_attention_workspace_size": (_sz, [_vp, _vp, _vp]),
+    "vrs_prefix_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vrs_beam_select_workspace_size": (_sz, [_vp]),
+    "vrs_beam_select": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vrs_beam_reorder": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "vrs_attention_weights_workspace_size": (_sz, [_vp, _vp]),
+    "vrs_attention_weights": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "vrs_cache_evict": (C.c_int, [_vp] * 14),
     "vrs_model_create": (C.c_int, [_vp, _P(BlockDesc), _i32, _i32, _i32, _i32, _f32, _P(_vp)]),
     "vrs_model_set_autotune": (C.c_int, [_vp, _i32]),
     "vrs_model_num_params": (C.c_int, [_vp]),
@@ -291,6 +331,24 @@ def seqs(q_start, k_start=None, k_len=None, max_q=0, max_k=0):
     s.tensors = (q_start, k_start, k_len)
     s.address = C.addressof(s)
     s.device = q_start.get_device()
+    return s
+
+
+def prefixes(first, k_start, k_len, max_rows=0, max_k=0):
+    """vrs_prefixes: groups of sequences that share a prefix, from int32 device tensors first [n + 1] (sequences of
+    each group) and k_start, k_len [n] (the prefix's keys).  Holds the tensors, as vrs.seqs."""
+    n = first.numel() - 1
+    if n < 0:
+        raise ValueError("prefixes: first needs n + 1 elements")
+    for t, size in ((first, n + 1), (k_start, n), (k_len, n)):
+        if str(t.dtype) != "torch.int32" or t.numel() != size or not t.is_contiguous():
+            raise ValueError("prefixes: contiguous int32 tensors first [n + 1], k_start [n], k_len [n]")
+        if t.get_device() != first.get_device():
+            raise ValueError("prefixes: tensors on different devices")
+    s = Prefixes(_ptr(first), _ptr(k_start), _ptr(k_len), n, max_rows, max_k)
+    s.tensors = (first, k_start, k_len)
+    s.address = C.addressof(s)
+    s.device = first.get_device()
     return s
 
 
@@ -486,6 +544,12 @@ class Context:
                              f"{dtype} on cuda:{self.device} (the context's device), the last dimension contiguous")
         return st
 
+    def _packed(self, what, t, shape, dtype):
+        """A contiguous tensor of this shape and type on this context's device."""
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}; needs {tuple(shape)} "
+                             f"{dtype} on cuda:{self.device} (the context's device), contiguous")
+
     def _seqs(self, what, seqs):
         """Address of a vrs_seqs whose arrays lie on this context's device."""
         if seqs.device != self.device:
@@ -610,24 +674,20 @@ class Context:
                              _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out), self._launch_stream(stream)))
         return q_out, k_out
 
-    def attention(self, q, k, v, seqs, causal=True, scale=0.0, out=None, workspace=None, stream=None):
-        """vrs_attention: q [rows, heads, dim], k and v [key rows, kv_heads, dim] (a cache as one run of
-        rows), seqs from vrs.seqs; scale 0: dim^-0.5.  workspace: a uint8 device tensor of at least
-        vrs_attention_workspace_size bytes, else allocated.  Returns out (rows of no sequence: as they
-        were, or unset where out is new)."""
-        import torch
+    def _attention_desc(self, what, q, k, v, causal, scale, out, stream):
+        """Descriptor of attention, and its output, new if none is given."""
         dt, dev, sq, sk = q.dtype, q.device, q.shape, k.shape
         code = dtype_code(dt)
         if len(sq) != 3 or len(sk) != 3:
-            raise ValueError(f"attention: q {tuple(sq)}, k {tuple(sk)}; needs [rows, heads, dim]")
+            raise ValueError(f"{what}: q {tuple(sq)}, k {tuple(sk)}; needs [rows, heads, dim]")
         rows, heads, dim = sq
         k_rows, kv, _ = sk
-        q_ld, q_hd, _ = self._strides("attention: q", q, sq, dt)
-        k_ld, k_hd, _ = self._strides("attention: k", k, (k_rows, kv, dim), dt)
-        v_ld, v_hd, _ = self._strides("attention: v", v, sk, dt)
+        q_ld, q_hd, _ = self._strides(what + ": q", q, sq, dt)
+        k_ld, k_hd, _ = self._strides(what + ": k", k, (k_rows, kv, dim), dt)
+        v_ld, v_hd, _ = self._strides(what + ": v", v, sk, dt)
         if out is None:
             out = self._empty(stream, sq, dt, dev)
-        o_ld, o_hd, _ = self._strides("attention: out", out, sq, dt)
+        o_ld, o_hd, _ = self._strides(what + ": out", out, sq, dt)
         if rows == 1:           # strides along a single row or head are of no account
             q_ld = o_ld = dim
         if k_rows == 1:
@@ -636,7 +696,16 @@ class Context:
             q_hd = o_hd = dim
         if kv == 1:
             k_hd = v_hd = dim
-        d = _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd)
+        return _ATTENTION(rows, k_rows, heads, kv, dim, code, causal, scale, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, o_ld, o_hd), out
+
+    def attention(self, q, k, v, seqs, causal=True, scale=0.0, out=None, workspace=None, stream=None):
+        """vrs_attention: q [rows, heads, dim], k and v [key rows, kv_heads, dim] (a cache as one run of
+        rows), seqs from vrs.seqs; scale 0: dim^-0.5.  workspace: a uint8 device tensor of at least
+        vrs_attention_workspace_size bytes, else allocated.  Returns out (rows of no sequence: as they
+        were, or unset where out is new)."""
+        import torch
+        dev = q.device
+        d, out = self._attention_desc("attention", q, k, v, causal, scale, out, stream)
         L, s = lib(), self._seqs("attention", seqs)
         if workspace is None:
             have = L.vrs_attention_workspace_size(d, s)
@@ -649,6 +718,154 @@ class Context:
         check(L.vrs_attention(self.handle, d, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                               _ptr(workspace), have, self._launch_stream(stream)))
         return out
+
+    def _workspace(self, what, workspace, need, stream, dev):
+        """The workspace of a call that needs `need` bytes, allocated if none is given, and its size."""
+        import torch
+        if workspace is None:
+            return (self._empty(stream, (need,), torch.uint8, dev), need) if need else (None, 0)
+        if workspace.get_device() != self.device or not workspace.is_contiguous():
+            raise ValueError(f"{what}: workspace on {workspace.device}; needs a contiguous tensor on cuda:{self.device}")
+        return workspace, workspace.numel() * workspace.element_size()
+
+    def prefix_attention(self, q, k, v, seqs, prefixes, causal=True, scale=0.0, out=None, workspace=None, stream=None):
+        """vrs_prefix_attention: attention whose sequences begin with the keys of their group's prefix
+        (vrs.prefixes), rows of the same k and v; else as attention."""
+        dev = q.device
+        d, out = self._attention_desc("prefix_attention", q, k, v, causal, scale, out, stream)
+        L, s = lib(), self._seqs("prefix_attention", seqs)
+        p = self._seqs("prefix_attention", prefixes)
+        need = L.vrs_prefix_attention_workspace_size(d, s, p) if workspace is None else 0
+        workspace, have = self._workspace("prefix_attention", workspace, need, stream, dev)
+        check(L.vrs_prefix_attention(self.handle, d, s, p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                     _ptr(workspace), have, self._launch_stream(stream)))
+        return out
+
+    def beam_select(self, logits, scores, k, done=None, eos=-1, outs=None, workspace=None, stream=None):
+        """vrs_beam_select: the k best continuations of each request, from logits [batch, beams, vocab] and the beams'
+        scores [batch, beams] (float32); done [batch, beams] (uint8 or bool): beams that go on with the token eos
+        alone.  Returns (scores, parents, tokens) [batch, k]; outs: those of an earlier call, written again."""
+        import torch
+        dt, dev, shape = logits.dtype, logits.device, logits.shape
+        code = dtype_code(dt)
+        if len(shape) != 3:
+            raise ValueError(f"beam_select: logits of {tuple(shape)}, needs [batch, beams, vocab]")
+        batch, beams, vocab = shape
+        st = self._strides("beam_select: logits", logits, shape, dt)
+        ld = st[1] if beams > 1 else st[0] if batch > 1 else vocab
+        if beams > 1 and batch > 1 and st[0] != beams * ld:
+            raise ValueError(f"beam_select: logits with strides {st}; rows of all requests lie one stride apart")
+        self._packed("beam_select: scores", scores, (batch, beams), torch.float32)
+        if done is not None:
+            self._packed("beam_select: done", done, (batch, beams), torch.bool if done.dtype is torch.bool else torch.uint8)
+        if outs is None:
+            outs = tuple(self._empty(stream, (batch, k), t, dev) for t in (torch.float32, torch.int32, torch.int32))
+        else:
+            for t, want in zip(outs, (torch.float32, torch.int32, torch.int32)):
+                self._packed("beam_select: outs", t, (batch, k), want)
+        d = _BEAM(batch, beams, vocab, k, code, eos, ld)
+        L = lib()
+        need = L.vrs_beam_select_workspace_size(d) if workspace is None else 0
+        workspace, have = self._workspace("beam_select", workspace, need, stream, dev)
+        check(L.vrs_beam_select(self.handle, d, _ptr(logits), _ptr(scores), _ptr(done), _ptr(outs[0]), _ptr(outs[1]),
+                                _ptr(outs[2]), _ptr(workspace), have, self._launch_stream(stream)))
+        return outs
+
+    def beam_reorder(self, state, parents, lens=None, stream=None):
+        """vrs_beam_reorder, in place: state [layers, batch * beams, rows, ...] of any type (the dimensions behind the
+        rows contiguous), parents [batch, beams] int32, lens [batch * beams] int32: the rows of each slot that move
+        (None: all).  Returns state."""
+        import torch
+        if state.ndim < 3 or parents.ndim != 2:
+            raise ValueError("beam_reorder: state [layers, batch * beams, rows, ...], parents [batch, beams]")
+        shape, st, es = state.shape, state.stride(), state.element_size()
+        batch, beams = parents.shape
+        self._packed("beam_reorder: parents", parents, (batch, beams), torch.int32)
+        if shape[1] != batch * beams or state.get_device() != self.device:
+            raise ValueError(f"beam_reorder: state of {tuple(shape)} on {state.device} for {batch} x {beams} beams on "
+                             f"cuda:{self.device} (the context's device)")
+        if lens is not None:
+            self._packed("beam_reorder: lens", lens, (batch * beams,) if lens.ndim == 1 else (batch, beams), torch.int32)
+        row = es
+        for n, s in zip(reversed(shape[3:]), reversed(st[3:])):
+            if n > 1 and s * es != row:
+                raise ValueError(f"beam_reorder: rows of {tuple(shape[3:])} with strides {st[3:]}; needs contiguous ones")
+            row *= n
+        d = _REORDER(batch, beams, shape[0], shape[2], row, st[2] * es, st[1] * es, st[0] * es)
+        check(lib().vrs_beam_reorder(self.handle, d, _ptr(parents), _ptr(lens), _ptr(state), self._launch_stream(stream)))
+        return state
+
+    def attention_weights(self, q, k, seqs, acc, decay=1.0, causal=True, scale=0.0, workspace=None, stream=None):
+        """vrs_attention_weights, into acc [kv_heads, key rows] (float32, any strides): decay * acc and the attention
+        that each key of the sequences receives from q [rows, heads, dim] over k [key rows, kv_heads, dim].
+        Returns acc."""
+        import torch
+        dt, dev, sq, sk = q.dtype, q.device, q.shape, k.shape
+        code = dtype_code(dt)
+        if len(sq) != 3 or len(sk) != 3:
+            raise ValueError(f"attention_weights: q {tuple(sq)}, k {tuple(sk)}; needs [rows, heads, dim]")
+        rows, heads, dim = sq
+        k_rows, kv, _ = sk
+        q_ld, q_hd, _ = self._strides("attention_weights: q", q, sq, dt)
+        k_ld, k_hd, _ = self._strides("attention_weights: k", k, (k_rows, kv, dim), dt)
+        if acc.shape != (kv, k_rows) or acc.dtype is not torch.float32 or acc.get_device() != self.device:
+            raise ValueError(f"attention_weights: acc {tuple(acc.shape)} {acc.dtype} on {acc.device}; needs {(kv, k_rows)} "
+                             f"float32 on cuda:{self.device} (the context's device)")
+        acc_hd, acc_ld = acc.stride()
+        if rows <= 1:           # strides along a single row or head are of no account
+            q_ld = dim
+        if k_rows == 1:
+            k_ld, acc_ld = dim, 1
+        if heads == 1:
+            q_hd = dim
+        if kv == 1:
+            k_hd, acc_hd = dim, 1
+        d = _WEIGHTS(rows, k_rows, heads, kv, dim, code, causal, scale, decay, q_ld, q_hd, k_ld, k_hd, acc_ld, acc_hd)
+        L, s = lib(), self._seqs("attention_weights", seqs)
+        need = L.vrs_attention_weights_workspace_size(d, s) if workspace is None else 0
+        workspace, have = self._workspace("attention_weights", workspace, need, stream, dev)
+        check(L.vrs_attention_weights(self.handle, d, s, _ptr(q), _ptr(k), _ptr(acc), _ptr(workspace), have,
+                                      self._launch_stream(stream)))
+        return acc
+
+    def cache_evict(self, k, v, acc, k_start, k_len, budget, first=0, recent=0, max_k=0, k_out=None, v_out=None,
+                    acc_out=None, out_start=None, len_out=None, kept=None, stream=None):
+        """vrs_cache_evict of k and v [key rows, kv_heads, dim] by acc [kv_heads, key rows]: of the k_len[i] keys from
+        row k_start[i] at most `budget` stay.  k_out, v_out, acc_out: where they go (None: in place); len_out [n],
+        kept [n, kv_heads, budget] int32: outputs to write, else new.  Returns (kept, len_out)."""
+        import torch
+        dt, dev, sk = k.dtype, k.device, k.shape
+        code = dtype_code(dt)
+        if len(sk) != 3:
+            raise ValueError(f"cache_evict: k {tuple(sk)}; needs [rows, heads, dim]")
+        k_rows, kv, dim = sk
+        n = k_start.numel()
+        for name, t in (("k_start", k_start), ("k_len", k_len), ("out_start", out_start), ("len_out", len_out)):
+            if t is not None:
+                self._packed("cache_evict: " + name, t, (n,), torch.int32)
+        k_out, v_out, acc_out = k if k_out is None else k_out, v if v_out is None else v_out, acc if acc_out is None else acc_out
+        out_rows = k_out.shape[0]
+        ld = []
+        for name, t, rows in (("k", k, k_rows), ("v", v, k_rows), ("k_out", k_out, out_rows), ("v_out", v_out, out_rows)):
+            s = self._strides("cache_evict: " + name, t, (rows, kv, dim), dt)
+            ld.append((dim if rows == 1 else s[0], dim if kv == 1 else s[1]))
+        for name, t, rows in (("acc", acc, k_rows), ("acc_out", acc_out, out_rows)):
+            if t.shape != (kv, rows) or t.dtype is not torch.float32 or t.get_device() != self.device:
+                raise ValueError(f"cache_evict: {name} {tuple(t.shape)} {t.dtype} on {t.device}; needs {(kv, rows)} float32 "
+                                 f"on cuda:{self.device} (the context's device)")
+            ld.append((1 if rows == 1 else t.stride(1), 1 if kv == 1 else t.stride(0)))
+        if len_out is None:
+            len_out = self._empty(stream, (n,), torch.int32, dev)
+        if kept is None:
+            kept = self._empty(stream, (n, kv, budget), torch.int32, dev)
+        else:
+            self._packed("cache_evict: kept", kept, (n, kv, budget), torch.int32)
+        d = _EVICT(n, k_rows, out_rows, kv, dim, code, budget, first, recent, max_k, *ld[0], *ld[1], *ld[4], *ld[2],
+                   *ld[3], *ld[5])
+        check(lib().vrs_cache_evict(self.handle, d, _ptr(k_start), _ptr(k_len), _ptr(out_start), _ptr(k), _ptr(v), _ptr(acc),
+                                    _ptr(k_out), _ptr(v_out), _ptr(acc_out), _ptr(len_out), _ptr(kept),
+                                    self._launch_stream(stream)))
+        return kept, len_out
 
     def msda(self, value, shapes, ref, off, attw, out, stream=None):
         n, s, heads, dh = value.shape
