@@ -371,6 +371,22 @@ def test_beam_select_of_what_is_no_number(dtype):
     check_select(logits_of(2, 4, 6000, dtype, seed=5), first, 8)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_beam_select_of_masks_at_the_end_of_the_range(dtype):
+    """Tokens masked by the type's lowest number are candidates like others, rows of nothing else too."""
+    import torch
+    low = torch.finfo(tdt(dtype)).min
+    x, s = logits_of(2, 3, 5000, dtype, seed=3), scores_of(2, 3)
+    x[0, 0, 4:] = low
+    x[0, 1] = low
+    x[0, 2, ::2] = low
+    x[1] = -low
+    check_select(x, s, 12)
+    x[:] = low
+    x[0, 1, 77] = 0
+    check_select(x, s, 12)
+
+
 def test_beam_select_equal_beams():
     """The same logits and score in every beam: equal candidates by the lowest beam."""
     x = logits_of(2, 1, 3000, "f32", seed=9).expand(2, 6, 3000).contiguous()

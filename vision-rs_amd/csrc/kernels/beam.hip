@@ -27,11 +27,11 @@ __device__ __forceinline__ uint64_t order64(double x) {
   return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
 
-// A number that r lanes of the wave reach at least, within 2^-15 of the r-th largest one's order (0: no number).
+// A number that r lanes of the wave reach at least: the r-th largest order, its lower 16 bits cleared (0: none).
 __device__ __forceinline__ uint32_t reached(uint32_t o, int r) {
   uint32_t t = 0;
 #pragma unroll
-  for (int b = 31; b >= 12; --b) {
+  for (int b = 31; b >= 16; --b) {
     const uint32_t trial = t | 1u << b;
     if (__builtin_popcountll(__ballot(o >= trial)) >= r) t = trial;
   }
@@ -55,11 +55,15 @@ __device__ __forceinline__ void best_of(uint64_t& o, uint32_t& at, uint64_t (&so
 }
 
 // ---------------------------------------------------------------------------
-// A chunk of one row: VT vectors of 16 bytes to a thread.
+// A chunk of one row: VT vectors of 16 bytes to a thread.  The sum is of 2^((x - m) L), L = log2 e rounded to
+// float32, and lse = m + log2(sum) / L with the same L, so that its rounding (1.3e-8) counts times the entropy only.
+// (One FMA of x L - m L would serve, but not at the ends of the range, where masks lie.)  A NaN or +infinity makes
+// the sum NaN.
+constexpr float kL = 1.44269502f;
 template <typename T, int VT>
 __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   constexpr int V = 16 / (int)sizeof(T), N = VT * V;
-  __shared__ uint2 cand[kCand];
+  __shared__ __attribute__((aligned(16))) uint2 cand[kCand];
   __shared__ int count;
   __shared__ float swm[kWaves];
   __shared__ double sws[kWaves];
@@ -71,69 +75,82 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   if (a.done && a.done[row]) return;           // such a beam goes on with the end token alone
   const int c0 = ch * a.chunk, n = min(a.chunk, a.vocab - c0);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.ld + c0;
-  float v[N];
-  bool nan = false;
+  u32x4_t raw[VT];
+  if (n == N * kT) {
 #pragma unroll
-  for (int j = 0; j < VT; ++j) {
-    const int e0 = (j * kT + tid) * V;
-    if (e0 + V <= n) {
-      T r[V];
-      __builtin_memcpy(r, x + e0, 16);         // rows start anywhere
+    for (int j = 0; j < VT; ++j) __builtin_memcpy(&raw[j], x + (j * kT + tid) * V, 16);      // rows start anywhere
+  } else {
+    constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;                    // -infinity
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[j * V + e] = Elt<T>::to_f(r[e]);
-    } else {
+    for (int j = 0; j < VT; ++j) {
+      const int e0 = (j * kT + tid) * V;
+      raw[j] = (u32x4_t){none, none, none, none};
+      if (e0 + V <= n) {
+        __builtin_memcpy(&raw[j], x + e0, 16);
+      } else if (e0 < n) {                     // the row ends in this vector
+        T last[V];
+        __builtin_memcpy(last, &raw[j], 16);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[j * V + e] = e0 + e < n ? Elt<T>::to_f(x[e0 + e]) : -INFINITY;
+        for (int e = 0; e < V; ++e)
+          if (e0 + e < n) last[e] = x[e0 + e];
+        __builtin_memcpy(&raw[j], last, 16);
+      }
     }
   }
-  float m = -INFINITY;
+  reinterpret_cast<u32x4_t*>(cand)[tid] = (u32x4_t){0, 0, 0, 0};    // the ranks below read whole eights
+  reinterpret_cast<u32x4_t*>(cand)[kT + tid] = (u32x4_t){0, 0, 0, 0};
+  float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    nan |= v[i] != v[i];
-    m = fmaxf(m, v[i]);                        // (a NaN is passed over)
+    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i / 4][i % 4]);
+    else v[i] = __uint_as_float(i % 2 ? raw[i / 8][i % 8 / 2] & 0xffff0000u : raw[i / 8][i % 8 / 2] << 16);
   }
-  const float mine = m;
+  auto token = [&](int i) { return (uint32_t)(c0 + ((i / V) * kT + tid) * V + i % V); };
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);                   // (a NaN is passed over)
+  if (!(m > -INFINITY)) m = -INFINITY;                              // (nothing else but NaN)
+  // what every wave has at least ceil(k / waves) numbers of, or one of them k (short chunks fill one wave only)
+  const uint32_t top = m == -INFINITY ? 0 : order32(m);
+  const uint32_t each = reached(top, (a.k + kWaves - 1) / kWaves);
+  const uint32_t alone = n < N * kT && a.k <= 64 ? reached(top, a.k) : 0;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  if (lane == 0) swm[wave] = m;
-  // what every wave has at least ceil(k / waves) numbers of, or one of them k (short chunks fill one wave only)
-  const uint32_t top = mine == -INFINITY ? 0 : order32(mine);
-  const uint32_t each = reached(top, (a.k + kWaves - 1) / kWaves), alone = a.k <= 64 ? reached(top, a.k) : 0;
-  if (lane == 0) sth[wave] = each, salone[wave] = alone;
+  if (lane == 0) swm[wave] = m, sth[wave] = each, salone[wave] = alone;
   if (tid == 0) count = 0;
   __syncthreads();
-  m = swm[0];
-  uint32_t T0 = sth[0];
+  m = fmaxf(fmaxf(swm[0], swm[1]), fmaxf(swm[2], swm[3]));
+  uint32_t T0 = min(min(sth[0], sth[1]), min(sth[2], sth[3]));
+  T0 = max(T0, max(max(salone[0], salone[1]), max(salone[2], salone[3])));
+  const float Tf = T0 ? __uint_as_float(T0 ^ ((int32_t)T0 < 0 ? 0x80000000u : 0xffffffffu)) : -3.40282347e38f;
+  // candidates (none is -infinity or NaN): a wave's places by one addition, then what each ballot holds
+  int mine = 0;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, swm[w]), T0 = min(T0, sth[w]);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) T0 = max(T0, salone[w]);
-  // the sum: 2^((x - m) log2 e), the exponent's factor in two parts, so that its rounding is that of one product
-  float sum = 0.f;
+  for (int i = 0; i < N; ++i) mine += __builtin_popcountll(__ballot(v[i] >= Tf));
+  int base = 0;
+  if (lane == 0 && mine) base = atomicAdd(&count, mine);
   const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = v[i] - ref;
-    sum += __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.44269502f, d * 1.92596300e-8f));
-  }
-  double total = nan ? (double)NAN : (double)sum;
+  for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * kL);
+  double total = sum;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) total += __shfl_xor(total, k);
   if (lane == 0) sws[wave] = total;
-  // candidates
+  base = __builtin_amdgcn_readfirstlane(base);
+  if (mine) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const bool in = v[i] > -INFINITY && order32(v[i]) >= T0;      // (false for NaN)
-    const uint64_t mask = __ballot(in);
-    if (mask == 0) continue;
-    int base = 0;
-    if (lane == 0) base = atomicAdd(&count, __builtin_popcountll(mask));
-    base = __builtin_amdgcn_readfirstlane(base) + __builtin_popcountll(mask & ((1ull << lane) - 1));
-    if (in && base < kCand) cand[base] = make_uint2(order32(v[i]), (uint32_t)(c0 + ((i / V) * kT + tid) * V + i % V));
+    for (int i = 0; i < N; ++i) {
+      const uint64_t mask = __ballot(v[i] >= Tf);
+      if (mask == 0) continue;
+      const int p = base + __builtin_popcountll(mask & ((1ull << lane) - 1));
+      if (v[i] >= Tf && p < kCand) cand[p] = make_uint2(order32(v[i]), token(i));
+      base += __builtin_popcountll(mask);
+    }
   }
   __syncthreads();
   const int64_t at = (int64_t)row * a.chunks + ch;
-  if (tid == 0) a.part[at] = make_double2(m, sws[0] + sws[1] + sws[2] + sws[3]);
+  if (tid == 0) a.part[at] = make_double2((double)m * kL, sws[0] + sws[1] + sws[2] + sws[3]);
   uint2* list = a.list + at * a.k;
   const int have = count;
   auto logit = [](uint32_t o) { return o ^ (((int32_t)o >> 31) ? 0x80000000u : 0xffffffffu); };
@@ -141,7 +158,14 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
     for (int i = tid; i < have; i += kT) {
       const uint2 me = cand[i];
       int rank = 0;
-      for (int j = 0; j < have; ++j) rank += cand[j].x > me.x || (cand[j].x == me.x && cand[j].y < me.y);
+      for (int j = 0; j < have; j += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u32x4_t c = reinterpret_cast<const u32x4_t*>(cand + j)[e];
+          rank += c[0] > me.x || (c[0] == me.x && c[1] < me.y);
+          rank += c[2] > me.x || (c[2] == me.x && c[3] < me.y);
+        }
+      }
       if (rank < a.k) list[rank] = make_uint2(logit(me.x), me.y);
     }
     if (tid < a.k && tid >= have) list[tid] = make_uint2(0, 0xffffffffu);
@@ -151,10 +175,10 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
     for (int k = 0; k < a.k; ++k) {
       uint64_t o = 0;
       uint32_t p = 0xffffffffu;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t q = (uint32_t)(c0 + ((i / V) * kT + tid) * V + i % V);
-        const uint64_t c = v[i] > -INFINITY ? order32(v[i]) : 0;
+      for (int e = tid; e < n; e += kT) {      // (from memory again: rare, so small code rather than fast)
+        const float f = Elt<T>::to_f(x[e]);
+        const uint32_t q = (uint32_t)(c0 + e);
+        const uint64_t c = f > -INFINITY ? order32(f) : 0;
         const bool after = c < lo || (c == lo && q > lat);
         if (c && after && (c > o || (c == o && q < p))) o = c, p = q;
       }
@@ -171,87 +195,112 @@ template <typename T>
 __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
   __shared__ double lse[64], score[64];
   __shared__ uint8_t kind[64];                 // 0: nothing but -infinity, 1: its lists, 2: the end token alone
-  __shared__ uint64_t co[kCand];
-  __shared__ uint32_t cat[kCand];
-  __shared__ uint32_t smax[kT];
-  __shared__ int count, found;
+  __shared__ __attribute__((aligned(16))) uint64_t co[kCand];
+  __shared__ __attribute__((aligned(16))) uint32_t cat[kCand];
+  __shared__ __attribute__((aligned(16))) uint32_t smax[kT];
+  __shared__ int count;
   __shared__ uint32_t sth;
   __shared__ uint64_t so[kWaves];
   __shared__ uint32_t sat[kWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
-  // lse of a beam: a wave over its chunks
-  for (int i = wave; i < a.beams; i += kWaves) {
+  // Lists are in order, so the first `per` entries of a list are its largest: a thread takes every per-th from
+  // one of them, and the k-th largest of the threads' first ones is reached by k entries at least.
+  const int lists = a.beams * a.chunks;
+  int per = 1, lg = 0;
+  while (per * 2 * lists <= kT) per *= 2, ++lg;
+  const int l0 = tid >> lg, j0 = tid & (per - 1);
+  const uint2* base = a.list + (int64_t)b * lists * a.k;
+  // (loaded early; a beam at its end has no lists, and what lies there is not used)
+  constexpr int kEarly = 4;
+  uint2 early[kEarly];
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i) {
+    const int j = j0 + i * per;
+    early[i] = l0 < lists && j < a.k ? base[(int64_t)l0 * a.k + j] : make_uint2(0, 0xffffffffu);
+  }
+  // lse of a beam: 2^w lanes over its chunks
+  int w = 0;
+  while ((1 << w) < a.chunks && w < 6) ++w;
+  for (int i0 = 0; i0 < a.beams; i0 += kT >> w) {
+    const int i = i0 + (tid >> w), c0 = tid & ((1 << w) - 1);
+    const bool in = i < a.beams;
     const int64_t row = (int64_t)b * a.beams + i;
-    const float s = a.scores[row];
-    const bool fine = s - s == 0.f, done = a.done && a.done[row];
-    float m = -INFINITY;
-    double l = 0;
-    bool odd = false;
-    if (!done) {
-      for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, (float)a.part[row * a.chunks + c].x);
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-      for (int c = lane; c < a.chunks; c += 64) {
-        const double2 p = a.part[row * a.chunks + c];
-        if (p.y != p.y) odd = true;
-        else if (p.y > 0.0) l += p.y * exp(p.x - (double)m);
-      }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) l += __shfl_xor(l, k);
-      odd = __any(odd);
+    const float s = in ? a.scores[row] : 0.f;
+    double m = -INFINITY, l = 0;
+    double2 p = make_double2(-INFINITY, 0);
+    if (in && c0 < a.chunks) p = a.part[row * a.chunks + c0];
+    const bool done = in && a.done && a.done[row], mine = in && !done;
+    for (int c = c0; mine && c < a.chunks; c += 64) m = fmax(m, c == c0 ? p.x : a.part[row * a.chunks + c].x);
+    for (int k = 1; k < 1 << w; k <<= 1) m = fmax(m, __shfl_xor(m, k));
+    for (int c = c0; mine && c < a.chunks; c += 64) {
+      if (c != c0) p = a.part[row * a.chunks + c];
+      l += p.y == 0.0 ? 0.0 : p.y * exp2(p.x - m);       // (a NaN stays one)
     }
-    if (lane == 0) {
+    for (int k = 1; k < 1 << w; k <<= 1) l += __shfl_xor(l, k);
+    if (in && c0 == 0) {
       score[i] = s;
-      lse[i] = (double)m + log(l);
-      kind[i] = !fine ? 0 : done ? 2 : (odd || m == -INFINITY || m == INFINITY) ? 0 : 1;
+      lse[i] = (m + log2(l)) / (double)kL;
+      kind[i] = !(s - s == 0.f) ? 0 : done ? 2 : !(l > 0.0 && l < INFINITY && m > -INFINITY && m < INFINITY) ? 0 : 1;
     }
   }
-  if (tid == 0) count = 0, found = 0;
+  if (tid == 0) count = 0, sth = 0;
   __syncthreads();
-  // entry j of list l (a beam's chunk): its order (0: none) and flat place
-  const int lists = a.beams * a.chunks;
-  const uint2* base = a.list + (int64_t)b * lists * a.k;
-  auto entry = [&](int l, int j, uint64_t& o, uint32_t& at) {
-    const int i = l / a.chunks;
+  // an entry's order (0: none) and flat place
+  auto valued = [&](int l, int j, uint2 e, uint64_t& o, uint32_t& at) {
+    const int i = l / a.chunks, k = kind[i];
     o = 0;
-    if (kind[i] == 1) {
-      const uint2 e = base[(int64_t)l * a.k + j];
-      if (e.y != 0xffffffffu) {
-        o = order64(score[i] + ((double)__uint_as_float(e.x) - lse[i]));
-        at = (uint32_t)(i * a.vocab) + e.y;
-      }
-    } else if (kind[i] == 2 && j == 0 && l == i * a.chunks) {
+    if (k == 1 && e.y != 0xffffffffu) {
+      o = order64(score[i] + ((double)__uint_as_float(e.x) - lse[i]));
+      at = (uint32_t)(i * a.vocab) + e.y;
+    } else if (k == 2 && j == 0 && l == i * a.chunks) {
       o = order64(score[i]);
       at = (uint32_t)(i * a.vocab + a.eos);
     }
   };
-  // Lists are in order, so the first `per` entries of a list are its largest: a thread takes every per-th from
-  // one of them, and the k-th largest of the threads' first ones is reached by k entries at least.
-  int per = 1;
-  while (per * 2 * lists <= kT) per *= 2;
+  auto entry = [&](int l, int j, uint64_t& o, uint32_t& at) {
+    valued(l, j, base[(int64_t)l * a.k + j], o, at);
+  };
   uint32_t top = 0;
-  for (int l = tid / per; l < lists; l += kT / per) {
+  for (int l = l0; l < lists; l += kT >> lg) {
     uint64_t o = 0;
     uint32_t at = 0;
-    if (tid % per < a.k) entry(l, tid % per, o, at);
+    if (l == l0) valued(l, j0, early[0], o, at);
+    else if (j0 < a.k) entry(l, j0, o, at);
     top = max(top, (uint32_t)(o >> 32));
   }
   smax[tid] = top;
-  if (tid == 0) sth = 0;
   __syncthreads();
-  int rank = 0;
-  for (int j = 0; j < kT; ++j) rank += smax[j] > top || (smax[j] == top && j < tid);
-  if (rank == a.k - 1) sth = top;
+  int above = 0, reach = 0;
+#pragma unroll 8
+  for (int j = 0; j < kT / 4; ++j) {
+    const u32x4_t c = reinterpret_cast<const u32x4_t*>(smax)[j];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) above += c[e] > top, reach += c[e] >= top;
+  }
+  if (above < a.k && reach >= a.k) sth = top;
   __syncthreads();
   const uint32_t T0 = max(sth, 1u);
-  for (int l = tid / per; l < lists; l += kT / per) {
-    for (int j = tid % per; j < a.k; j += per) {
+  auto take = [&](uint64_t o, uint32_t at) {
+    if ((uint32_t)(o >> 32) < T0) return false;
+    const int p = atomicAdd(&count, 1);
+    if (p < kCand) co[p] = o, cat[p] = at;
+    return true;
+  };
+  bool more = l0 < lists;
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i) {
+    uint64_t o = 0;
+    uint32_t at = 0;
+    if (more) valued(l0, j0 + i * per, early[i], o, at);
+    more = more && take(o, at);
+  }
+  for (int l = l0; l < lists; l += kT >> lg) {
+    if (l == l0 && !more) continue;
+    for (int j = j0 + (l == l0 ? kEarly * per : 0); j < a.k; j += per) {
       uint64_t o;
       uint32_t at = 0;
       entry(l, j, o, at);
-      if ((uint32_t)(o >> 32) < T0) break;
-      const int p = atomicAdd(&count, 1);
-      if (p < kCand) co[p] = o, cat[p] = at;
+      if (!take(o, at)) break;
     }
   }
   __syncthreads();
@@ -268,6 +317,7 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
       const uint64_t o = co[i];
       const uint32_t at = cat[i];
       int r = 0;
+#pragma unroll 8
       for (int j = 0; j < have; ++j) r += co[j] > o || (co[j] == o && cat[j] < at);
       if (r < a.k) put(r, o, at);
     }
@@ -277,8 +327,8 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
     for (int k = 0; k < a.k; ++k) {
       uint64_t o = 0;
       uint32_t p = 0xffffffffu;
-      for (int l = tid / per; l < lists; l += kT / per)
-        for (int j = tid % per; j < a.k; j += per) {
+      for (int l = l0; l < lists; l += kT >> lg)
+        for (int j = j0; j < a.k; j += per) {
           uint64_t c;
           uint32_t q = 0;
           entry(l, j, c, q);
