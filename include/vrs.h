@@ -610,7 +610,8 @@ int vrs_beam_reorder(vrs_ctx* ctx, const vrs_reorder_desc* d, const int32_t* par
  * sees).  acc: float32, of key row r and key head g at acc[r * acc_ld + g * acc_hd];
  * sequences must not share key rows.  decay 0 does not read acc.
  * Scores, weights and sums are float32 and each sum has a fixed order.  head_dim,
- * alignment, strides and workspace as in vrs_attention. */
+ * alignment, strides and workspace as in vrs_attention, but that the heads of a key
+ * head and 65 rows of q lie within 2^29 elements. */
 typedef struct {
   int32_t q_rows, k_rows;
   int32_t heads, kv_heads, head_dim, dtype;   /* VRS_BF16 or VRS_F32 */

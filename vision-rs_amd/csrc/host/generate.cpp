@@ -273,6 +273,9 @@ int check_weights(const vrs_weights_desc* d, const vrs_seqs* seqs, const char* m
   if (!(d->decay >= 0.f && d->decay <= 1.f)) return fail(VRS_EINVAL, "%s: decay %g", me, (double)d->decay);
   for (int64_t s : {d->acc_ld, d->acc_hd})
     if (s < 0 || s >> 40) return fail(VRS_EBADSHAPE, "%s: stride %lld", me, (long long)s);
+  // (the kernels' offsets from a row tile's first query)
+  if ((d->heads / d->kv_heads) * d->q_hd + 65 * d->q_ld >= (1ll << 31) / 4)
+    return fail(VRS_EUNSUPPORTED, "%s: query strides %lld and %lld", me, (long long)d->q_ld, (long long)d->q_hd);
   if ((d->k_rows > 1 && d->acc_ld < 1) || (d->kv_heads > 1 && d->acc_hd < 1))
     return fail(VRS_EBADSHAPE, "%s: acc strides fold rows or heads onto each other", me);
   return VRS_OK;
@@ -280,8 +283,9 @@ int check_weights(const vrs_weights_desc* d, const vrs_seqs* seqs, const char* m
 
 struct WeightsPlan {
   bool few;
-  int parts;
-  int64_t row_tiles, s_ld, key_tiles;
+  int parts, key_parts;
+  int64_t row_tiles;       // few: 32-row tiles of the longest sequence; else ids of 128-row tiles
+  int64_t s_ld, key_tiles; // keys counted on, in whole tiles; tiles of them
 };
 WeightsPlan plan_weights(const vrs_weights_desc* d, const vrs_seqs* s) {
   const int64_t group = d->heads / d->kv_heads, n = s->n;
@@ -289,16 +293,27 @@ WeightsPlan plan_weights(const vrs_weights_desc* d, const vrs_seqs* s) {
   const int64_t mk = std::max<int64_t>(1, s->max_k > 0 ? std::min(s->max_k, d->k_rows) : up(d->k_rows, n));
   WeightsPlan p;
   p.few = mq * group <= 32;
-  p.row_tiles = up(mq * group, 32);
-  const int64_t wgs = n * d->kv_heads * p.row_tiles;
-  p.parts = (int)std::clamp<int64_t>(std::min(up(512, wgs), mk / 192), 1, 64);
-  p.s_ld = p.few ? up(mk, 4) * 4 : 0;
-  p.key_tiles = up(mk, p.few ? 256 : 128);
+  p.key_parts = 1;
+  if (p.few) {
+    p.row_tiles = up(mq * group, 32);
+    const int64_t wgs = n * d->kv_heads * p.row_tiles;
+    p.parts = (int)std::clamp<int64_t>(std::min(std::max<int64_t>(4, up(512, wgs)), mk / 192), 1, 64);
+    p.key_tiles = up(mk, 1024);
+    p.s_ld = p.key_tiles * 1024;
+  } else {
+    p.row_tiles = d->q_rows * group / 128 + n;
+    const int64_t wgs = std::min(p.row_tiles, n * up(mq * group, 128)) * d->kv_heads;
+    p.parts = (int)std::clamp<int64_t>(std::min(1024 / wgs, mk / 256), 1, 32);
+    p.key_tiles = up(mk, 128);
+    p.s_ld = p.key_tiles * 128;
+    p.key_parts = (int)std::clamp<int64_t>(std::min(2048 / (n * d->kv_heads * p.key_tiles), mq * group / 256), 1, 16);
+  }
   return p;
 }
 size_t weights_rl_bytes(const vrs_weights_desc* d, const WeightsPlan& p) { return (size_t)up((int64_t)p.parts * d->q_rows * d->heads, 2) * 16; }
-size_t weights_bytes(const vrs_weights_desc* d, const WeightsPlan& p) {
-  return weights_rl_bytes(d, p) + (size_t)d->q_rows * d->heads * p.s_ld * 4;
+size_t weights_bytes(const vrs_weights_desc* d, int32_t n, const WeightsPlan& p) {
+  const size_t rows = p.few ? (size_t)d->q_rows * d->heads : p.key_parts > 1 ? (size_t)p.key_parts * n * d->kv_heads : 0;
+  return weights_rl_bytes(d, p) + rows * p.s_ld * 4;
 }
 
 }  // namespace
@@ -307,7 +322,7 @@ extern "C" {
 
 size_t vrs_attention_weights_workspace_size(const vrs_weights_desc* d, const vrs_seqs* seqs) {
   if (check_weights(d, seqs, "vrs_attention_weights") || d->k_rows == 0 || seqs->n == 0) return 0;
-  return weights_bytes(d, plan_weights(d, seqs));
+  return weights_bytes(d, seqs->n, plan_weights(d, seqs));
 }
 
 int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seqs* seqs, const void* q, const void* k,
@@ -320,7 +335,7 @@ int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seq
   if ((d->q_rows && (rc = check_ptr(q, 16, me, "q"))) || (rc = check_ptr(k, 16, me, "k")) || (rc = check_ptr(acc, 4, me, "acc"))) return rc;
   if ((const void*)acc == q || (const void*)acc == k) return fail(VRS_EINVAL, "%s: acc is an input", me);
   const WeightsPlan p = plan_weights(d, seqs);
-  if ((rc = check_workspace(workspace, workspace_bytes, weights_bytes(d, p), me))) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, weights_bytes(d, seqs->n, p), me))) return rc;
   vrs_weights_args a{};
   a.q = q; a.k = k; a.acc = acc;
   a.rl = static_cast<float2*>(workspace);
@@ -330,20 +345,27 @@ int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seq
   a.q_ld = d->q_ld; a.q_hd = d->q_hd; a.k_ld = d->k_ld; a.k_hd = d->k_hd; a.acc_ld = d->acc_ld; a.acc_hd = d->acc_hd;
   a.s_ld = p.s_ld;
   a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.causal = d->causal != 0; a.parts = p.parts;
+  a.key_parts = p.key_parts;
   a.c = (float)((d->scale > 0.f ? (double)d->scale : 1.0 / std::sqrt((double)d->head_dim)) * 1.4426950408889634);
   a.decay = d->decay;
-  const int64_t pairs = (int64_t)seqs->n * d->kv_heads, first = pairs * p.parts;
-  if (first >= (1ll << 32) / 256) return fail(VRS_EBADSHAPE, "%s: grid too large", me);
+  const int64_t pairs = (int64_t)seqs->n * d->kv_heads;
+  const int64_t first = (p.few ? pairs : p.row_tiles * d->kv_heads) * p.parts;
+  if (p.row_tiles >= (1ll << 30) || first >= (1ll << 32) / 256 || pairs * p.key_parts >= (1ll << 32) / 256)
+    return fail(VRS_EBADSHAPE, "%s: grid too large", me);
   const int D = d->head_dim <= 64 ? 64 : 128;
   char name[64];
   if (d->q_rows) {
     snprintf(name, sizeof name, "vrs_weights_%s_%s_d%d", p.few ? "scores" : "stats", dsuffix(d->dtype), D);
-    rc = launch(ctx, name, dim3((unsigned)first, (unsigned)std::min<int64_t>(p.row_tiles, 65535)), dim3(256), 0, &a, stream);
+    const unsigned y = p.few ? (unsigned)std::min<int64_t>(p.row_tiles, 65535) : 1;
+    rc = launch(ctx, name, dim3((unsigned)first, y), dim3(256), 0, &a, stream);
     if (rc) return rc;
   }
   if (p.few) snprintf(name, sizeof name, "vrs_weights_sum_%s", dsuffix(d->dtype));
   else snprintf(name, sizeof name, "vrs_weights_keys_%s_d%d", dsuffix(d->dtype), D);
-  return launch(ctx, name, dim3((unsigned)pairs, (unsigned)std::min<int64_t>(p.key_tiles, 65535)), dim3(256), 0, &a, stream);
+  const unsigned tiles = (unsigned)std::min<int64_t>(p.key_tiles, 65535);
+  rc = launch(ctx, name, dim3((unsigned)(pairs * p.key_parts), tiles), dim3(256), 0, &a, stream);
+  if (rc || p.key_parts == 1) return rc;
+  return launch(ctx, "vrs_weights_join", dim3((unsigned)pairs, (unsigned)up(p.s_ld, 256)), dim3(256), 0, &a, stream);
 }
 
 // ---- eviction ----------------------------------------------------------------------

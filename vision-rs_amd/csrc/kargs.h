@@ -402,12 +402,14 @@ typedef struct {
 typedef struct {
   const void *q, *k;
   float* acc;
-  float* scores;           /* few rows: [q_rows][heads][s_ld] */
+  float* scores;           /* few rows: [q_rows][heads][s_ld]; many: sums [key_parts][n * kv][s_ld] */
   float2* rl;              /* [parts][q_rows][heads] reference of the weights and their sum */
   vrs_seq_args s;
   int64_t q_ld, q_hd, k_ld, k_hd, acc_ld, acc_hd;
-  int64_t s_ld;
-  int32_t heads, kv, dim, causal, parts;
+  int64_t s_ld;            /* keys of a sequence that were counted on, in whole tiles */
+  int32_t heads, kv, dim, causal;
+  int32_t parts;           /* of a row's keys (statistics) */
+  int32_t key_parts;       /* many: of the rows of a key */
   float c, decay;
 } vrs_weights_args;
 

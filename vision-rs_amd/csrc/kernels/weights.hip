@@ -11,15 +11,19 @@
 
 namespace {
 
-// Stage 1: a workgroup of 4 waves takes 32 rows of one key head against a part of
-// the keys, its waves every fourth 32 of them.
-template <typename T, int D, bool KEEP>
-__device__ __forceinline__ void stats_body(const vrs_weights_args& a) {
-  using E = Elt<T>;
-  using G = typename E::group;
-  constexpr int NW = 4;
+// Stage 1, few rows: a workgroup of 4 waves takes 32 rows of one key head against a
+// part of the keys, its waves every fourth 32 of them.  Memory bound: K is loaded by
+// whole rows (a lane's operand straight from memory touches a row in eight
+// instructions, and the lines are gone from L1 in between: 165 us instead of 128
+// for the scores of 64 tokens over 500 .. 8000 keys, 32 heads on 8 of 128) and turned in a wave's own
+// LDS tile, the next tile's loads in flight meanwhile.
+template <typename T, int D>
+__device__ __forceinline__ void scores_body(const vrs_weights_args& a) {
+  constexpr int NW = 4, CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T), IT = 32 * CH / 64;
+  __shared__ __attribute__((aligned(16))) T tiles[NW][32 * D];
   __shared__ float sR[NW][32], sl[NW][32];
-  const int wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  T* const sK = tiles[wave];
   const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv, part = rest % a.parts;
   const SeqSpan sp = ranked_seq(Sequences{a.s}, rest / a.parts);
   const int G_ = a.heads / a.kv;
@@ -39,39 +43,42 @@ __device__ __forceinline__ void stats_body(const vrs_weights_args& a) {
     int kb, ke;
     part_of(lim_max, part, a.parts, 32, kb, ke);
     const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
-    G kr[D / 16];
-    uint32_t ko[D / 16];                   // offsets in a tile; elements past the head read 0
+    u32x4_t held[IT];
+    uint32_t ko[IT];                       // offsets in a tile; elements past the head read 0
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const int d = i * 16 + w.hh * 8;
-      ko[i] = d < a.dim ? (uint32_t)(w.l32 * (int)a.k_ld + d) * (uint32_t)sizeof(T) : kOOB;
+    for (int i = 0; i < IT; ++i) {
+      const int it = lane + i * 64, r = it / CH, ch = it % CH;
+      ko[i] = ch * PER < a.dim ? (uint32_t)(r * (int)a.k_ld + ch * PER) * (uint32_t)sizeof(T) : kOOB;
     }
     auto load = [&](int kc) {              // keys past the sequence's last are masked, whatever they read
       const int n = min(32, sp.k_lim - kc);
       const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) kr[i] = E::bload(rk, ko[i], 0);
+      for (int i = 0; i < IT; ++i) held[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, ko[i], 0, 0);
     };
     float* keep = a.scores + (row * a.heads + h) * a.s_ld;
     int kc = kb + wave * 32;
     if (kc < ke) load(kc);
     while (kc < ke) {
-      f32x16_t s;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) s = mfma32_k16(kr[i], w.qf[0][i], s);
+      for (int i = 0; i < IT; ++i) {
+        const int it = lane + i * 64, r = it / CH, ch = it % CH;
+        *reinterpret_cast<u32x4_t*>(sK + r * D + (ch ^ Lds<T, D>::kswz(r)) * PER) = held[i];
+      }
+      __builtin_amdgcn_wave_barrier();     // the wave's own tile: order alone is needed
       const int at = kc;
       kc += NW * 32;
       if (kc < ke) load(kc);
+      f32x16_t sc[1];
+      w.scores(sK, 0, sc);
+      __builtin_amdgcn_wave_barrier();
+      f32x16_t& s = sc[0];
       if (at + 32 > lim_min) w.mask(0, s, at);
-      if constexpr (KEEP) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int64_t key = at + g * 8 + w.hh * 4;
-          const f32x4_t v = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
-          if (ok && key < a.s_ld) *reinterpret_cast<f32x4_t*>(keep + key) = v;
-        }
+      for (int g = 0; g < 4; ++g) {
+        const int64_t key = at + g * 8 + w.hh * 4;
+        const f32x4_t v = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+        if (ok && key < a.s_ld) *reinterpret_cast<f32x4_t*>(keep + key) = v;
       }
       const float t[1] = {w.top(s)};
       w.follow(t, u);
@@ -96,8 +103,91 @@ __device__ __forceinline__ void stats_body(const vrs_weights_args& a) {
   }
 }
 
-// A row's reference and 1 / sum over the parts of its keys.
-__device__ __forceinline__ float2 joined(const vrs_weights_args& a, const Log2& u, int64_t id, int keys) {
+// Streaming tiles of 64 rows (keys for the statistics, queries for the sums) in
+// LDS, twice: a thread holds the next tile's chunks in registers while this one is
+// in use, so that one barrier a tile is enough.
+template <typename T, int D>
+struct Stream {
+  using G = typename Elt<T>::group;
+  static constexpr int CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T), IT = 64 * CH / 256, TILE = 64 * D;
+  u32x4_t held[IT];
+  __device__ __forceinline__ static int row(int i) { return (i * 256 + (int)threadIdx.x) / CH; }
+  __device__ __forceinline__ static int elt(int i) { return (i * 256 + (int)threadIdx.x) % CH * PER; }
+  __device__ __forceinline__ void put(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = row(i);
+      *reinterpret_cast<u32x4_t*>(tile + r * D + (((i * 256 + (int)threadIdx.x) % CH) ^ Lds<T, D>::kswz(r)) * PER) = held[i];
+    }
+  }
+};
+
+// Stage 1, many rows: a workgroup of 4 waves takes 128 rows, which the keys pass by.
+// 4096 causal queries, 32 heads on 8 of 128: see the host's choice.
+template <typename T, int D>
+__device__ __forceinline__ void stats_body(const vrs_weights_args& a) {
+  using S = Stream<T, D>;
+  __shared__ __attribute__((aligned(16))) T tile[2][S::TILE];
+  const int wave = threadIdx.x >> 6;
+  const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv, part = rest % a.parts;
+  const int group = a.heads / a.kv;
+  const TilePlace at = place_tile<128>(Sequences{a.s}, group, rest / a.parts);
+  if (at.tile < 0) return;
+  const SeqSpan sp = at.sp;
+  const int64_t rows = (int64_t)sp.q_len * group;
+  const int tiles = (int)((rows + 127) / 128);
+  if (at.tile >= tiles) return;
+  const int64_t r0 = (int64_t)(tiles - 1 - at.tile) * 128;       // late rows (causal: the most keys) first
+  const Log2 u(a.c);
+  Wave<T, D, 1> w;
+  w.init(u);
+  const int64_t r = r0 + wave * 32 + w.l32, pr = min(r, rows - 1);
+  const bool ok = r < rows;
+  const int j = (int)(pr / group), h = hk * group + (int)(pr - (int64_t)j * group);
+  const int64_t row = sp.q0 + j;
+  w.lim[0] = visible(sp, j, a.causal);
+  w.load_q(0, static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd, a.dim, ok);
+  int kb, ke;
+  part_of(visible(sp, (int)((min(r0 + 128, rows) - 1) / group), a.causal), part, a.parts, 64, kb, ke);
+  const int all = __builtin_amdgcn_readlane(w.lim[0], 0), mine = __builtin_amdgcn_readlane(w.lim[0], 31);
+  const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
+  S st;
+  auto load = [&](int kc) {              // keys past the sequence's last read 0 and are masked
+    const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((min(64, sp.k_lim - kc) - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
+#pragma unroll
+    for (int i = 0; i < S::IT; ++i)
+      st.held[i] = __builtin_amdgcn_raw_buffer_load_b128(
+          rk, S::elt(i) < a.dim ? (uint32_t)(S::row(i) * (int)a.k_ld + S::elt(i)) * (uint32_t)sizeof(T) : kOOB, 0, 0);
+  };
+  if (kb < ke) {
+    load(kb);
+    st.put(tile[0]);
+    if (kb + 64 < ke) load(kb + 64);
+    __syncthreads();
+    for (int kc = kb, buf = 0; kc < ke; kc += 64, buf ^= 1) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int at0 = kc + n * 32;
+        if (at0 >= mine) break;
+        f32x16_t s[1];
+        w.scores(tile[buf], n * 32, s);
+        if (at0 + 32 > all) w.mask(0, s[0], at0);
+        const float t[1] = {w.top(s[0])};
+        w.follow(t, u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w.l[0] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], w.unit[0], -w.R[0]));
+      }
+      if (kc + 64 < ke) st.put(tile[buf ^ 1]);
+      if (kc + 128 < ke) load(kc + 128);
+      __syncthreads();
+    }
+  }
+  const float lt = sum32(w.l[0]);
+  if (w.hh == 0 && ok) a.rl[((int64_t)part * a.s.q_rows + row) * a.heads + h] = make_float2(w.R[0], lt);
+}
+
+// A row's reference and sum over the parts of its keys.
+__device__ __forceinline__ float2 joined(const vrs_weights_args& a, const Log2& u, int64_t id) {
   const int64_t step = (int64_t)a.s.q_rows * a.heads;
   float mx = kNone, l = 0.f;
   for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.rl[p * step + id].x);
@@ -105,15 +195,14 @@ __device__ __forceinline__ float2 joined(const vrs_weights_args& a, const Log2& 
     const float2 rl = a.rl[p * step + id];
     l += u.factor(rl.x, mx) * rl.y;
   }
-  return make_float2(mx, share(l, keys));
+  return make_float2(mx, l);
 }
 
-// Stage 2 from the scores: a thread takes a key and passes over the rows.
+// Stage 2 from the scores: a thread takes 4 keys, 256 apart, and passes over the rows.
 template <typename T>
 __device__ __forceinline__ void sum_body(const vrs_weights_args& a) {
-  constexpr int RB = 64;
-  __shared__ float sR[RB], sinv[RB], sunit[RB];
-  __shared__ int slim[RB];
+  constexpr int RB = 32, KT = 4;
+  __shared__ f32x4_t stat[RB];                // reference, 1 / sum, unit, keys seen (as bits)
   const int hk = blockIdx.x % a.kv;
   const SeqSpan sp = seq_span(a.s, blockIdx.x / a.kv);
   const int G_ = a.heads / a.kv;
@@ -121,66 +210,92 @@ __device__ __forceinline__ void sum_body(const vrs_weights_args& a) {
   const Log2 u(a.c);
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   float* acc = a.acc + sp.k0 * a.acc_ld + hk * a.acc_hd;
-  for (int64_t k0 = (int64_t)blockIdx.y * 256; k0 < sp.k_lim; k0 += (int64_t)gridDim.y * 256) {
-    const int key = (int)k0 + threadIdx.x;
-    float sum = 0.f;
+  for (int64_t k0 = (int64_t)blockIdx.y * 256 * KT; k0 < sp.k_lim; k0 += (int64_t)gridDim.y * 256 * KT) {
+    const int64_t key = k0 + threadIdx.x;
+    float sum[KT], old[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      sum[t] = 0.f;
+      old[t] = a.decay != 0.f && key + t * 256 < sp.k_lim ? acc[(key + t * 256) * a.acc_ld] : 0.f;
+    }
     for (int r0 = 0; r0 < rows; r0 += RB) {
       __syncthreads();
       const int r = r0 + threadIdx.x;
       if (threadIdx.x < RB && r < rows) {
         const int j = r / G_;
-        const int64_t id = ((int64_t)sp.q0 + j) * a.heads + hk * G_ + (r - j * G_);
         const int lim = visible(sp, j, a.causal);
-        const float2 rl = joined(a, u, id, lim);
-        sR[threadIdx.x] = rl.x;
-        sinv[threadIdx.x] = rl.y;
-        sunit[threadIdx.x] = u.unit(rl.x);
-        slim[threadIdx.x] = lim;
+        const float2 rl = joined(a, u, ((int64_t)sp.q0 + j) * a.heads + hk * G_ + (r - j * G_));
+        stat[threadIdx.x] = (f32x4_t){rl.x, share(rl.y, lim), u.unit(rl.x), __int_as_float(lim)};
       }
       __syncthreads();
-      if (key < sp.k_lim) {
-        for (int i = 0; i < min(RB, rows - r0); ++i) {
-          if (key >= slim[i]) continue;
+      const int n = min(RB, rows - r0);
+      if (k0 + 256 * KT <= a.s_ld) {
+        for (int i = 0; i < n; ++i) {
+          const int j = (r0 + i) / G_, h = hk * G_ + (r0 + i - j * G_);
+          const float* s = a.scores + (((int64_t)sp.q0 + j) * a.heads + h) * a.s_ld + key;
+          const f32x4_t c = stat[i];
+          float x[KT];
+#pragma unroll
+          for (int t = 0; t < KT; ++t) x[t] = s[t * 256];
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t], c[2], -c[0])) * c[1];
+            sum[t] += key + t * 256 < __float_as_int(c[3]) ? p : 0.f;
+          }
+        }
+      } else {
+        for (int i = 0; i < n; ++i) {
           const int j = (r0 + i) / G_, h = hk * G_ + (r0 + i - j * G_);
           const int64_t row = (int64_t)sp.q0 + j;
-          float s;
-          if (key < a.s_ld) {
-            s = a.scores[(row * a.heads + h) * a.s_ld + key];
-          } else {                         // more keys than were counted on
-            const T* q = static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd;
-            const T* k = kp + (int64_t)key * a.k_ld;
-            s = 0.f;
-            for (int d = 0; d < a.dim; ++d) s = __builtin_fmaf(Elt<T>::to_f(q[d]), Elt<T>::to_f(k[d]), s);
+          const f32x4_t c = stat[i];
+          for (int t = 0; t < KT; ++t) {
+            const int64_t at = key + t * 256;
+            if (at >= __float_as_int(c[3])) break;
+            float x = 0.f;
+            if (at < a.s_ld) {
+              x = a.scores[(row * a.heads + h) * a.s_ld + at];
+            } else {                         // more keys than were counted on
+              const T* q = static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd;
+              const T* k = kp + at * a.k_ld;
+              for (int d = 0; d < a.dim; ++d) x = __builtin_fmaf(Elt<T>::to_f(q[d]), Elt<T>::to_f(k[d]), x);
+            }
+            sum[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[2], -c[0])) * c[1];
           }
-          sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s, sunit[i], -sR[i])) * sinv[i];
         }
       }
     }
-    if (key < sp.k_lim) {
-      float* to = acc + (int64_t)key * a.acc_ld;
-      *to = (a.decay == 0.f ? 0.f : a.decay * *to) + sum;
-    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+      if (key + t * 256 < sp.k_lim) acc[(key + t * 256) * a.acc_ld] = a.decay * old[t] + sum[t];
   }
 }
 
-// Stage 2 with the products again: a wave holds 32 keys, and the rows that see
-// them pass by in tiles of 32.
+// Stage 2 with the products again: a workgroup of 4 waves holds 128 keys, and a part
+// of the rows that see them passes by in tiles of 64.
 template <typename T, int D>
 __device__ __forceinline__ void keys_body(const vrs_weights_args& a) {
   using E = Elt<T>;
   using G = typename E::group;
-  const int hk = blockIdx.x % a.kv, wave = threadIdx.x >> 6, l32 = threadIdx.x & 31, hh = (threadIdx.x >> 5) & 1;
-  const SeqSpan sp = ranked_seq(Sequences{a.s}, blockIdx.x / a.kv);
-  const int G_ = a.heads / a.kv;
-  const int64_t rows = (int64_t)sp.q_len * G_;
+  using S = Stream<T, D>;
+  __shared__ __attribute__((aligned(16))) T tile[2][S::TILE];
+  __shared__ f32x4_t stat[2][64];             // reference, 1 / sum, unit, keys seen (as bits) of the tile's rows
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = threadIdx.x & 31, hh = (threadIdx.x >> 5) & 1;
+  const int hk = blockIdx.x % a.kv, pair = blockIdx.x % (a.s.n * a.kv), part = blockIdx.x / (a.s.n * a.kv);
+  const SeqSpan sp = seq_span(a.s, pair / a.kv);
+  const int group = a.heads / a.kv;
+  const float inv_group = 1.f / (float)group;
+  const int64_t rows = (int64_t)sp.q_len * group;
   const Log2 u(a.c);
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
   float* acc = a.acc + sp.k0 * a.acc_ld + hk * a.acc_hd;
-  for (int64_t k0 = (int64_t)blockIdx.y * 128 + wave * 32; k0 < sp.k_lim; k0 += (int64_t)gridDim.y * 128) {
-    const int kc = (int)k0;
+  for (int64_t k0 = (int64_t)blockIdx.y * 128; k0 < sp.k_lim; k0 += (int64_t)gridDim.y * 128) {
+    // key tiles past those counted on have no place in the workspace: one workgroup takes all their rows
+    const bool counted = k0 < (int64_t)a.s_ld;
+    const int parts = counted ? a.key_parts : 1;
+    if (part >= parts) return;
+    const int kc = (int)k0 + wave * 32, n = min(32, max(sp.k_lim - kc, 1));
     G kr[D / 16];
-    const int n = min(32, sp.k_lim - kc);
-    const auto rk = make_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
+    const auto rk = make_rsrc(kp + (int64_t)min(kc, sp.k_lim - 1) * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const int d = i * 16 + hh * 8;
@@ -189,53 +304,152 @@ __device__ __forceinline__ void keys_body(const vrs_weights_args& a) {
     float sum[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-    // rows from the first that sees key kc on
-    const int64_t skip = a.causal ? max((int64_t)0, (int64_t)kc - ((int64_t)sp.k_len - sp.q_len)) * G_ : 0;
-    for (int64_t r0 = skip / 32 * 32; r0 < rows; r0 += 32) {
-      const int64_t pr = min(r0 + l32, rows - 1);
-      const bool ok = r0 + l32 < rows;
-      const int j = (int)(pr / G_), h = hk * G_ + (int)(pr - (int64_t)j * G_);
-      const int64_t row = sp.q0 + j;
-      const int lim = ok ? visible(sp, j, a.causal) : 0;
-      const T* q = static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd;
-      const float2 rl = joined(a, u, row * a.heads + h, lim);
-      const float unit = u.unit(rl.x);
-      f32x16_t s;
+    // tiles from the first that has a row which sees key k0 on, shared out among the parts
+    const int64_t skip = a.causal ? max((int64_t)0, k0 - ((int64_t)sp.k_len - sp.q_len)) * group : 0;
+    // (divisions of 64 bits run on vector registers: what they give is made scalar again)
+    const int t0 = __builtin_amdgcn_readfirstlane((int)(min(skip, rows) / 64)), t1 = (int)((rows + 63) >> 6);
+    const int tb = __builtin_amdgcn_readfirstlane(t0 + (int)((int64_t)(t1 - t0) * part / parts));
+    const int te = __builtin_amdgcn_readfirstlane(t0 + (int)((int64_t)(t1 - t0) * (part + 1) / parts));
+    S st;
+    // The next tile to load: its first query and that one's first head, and where a thread's chunks and its row of
+    // the statistics lie from there.  Where 64 rows are whole queries these stay and the first query alone moves.
+    int at = tb;
+    int j0 = __builtin_amdgcn_readfirstlane((int)((int64_t)tb * 64 / group)), rem = (int)((int64_t)tb * 64 - (int64_t)j0 * group), sj, sh;
+    uint32_t off[S::IT];
+    auto places = [&]() {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const int d = i * 16 + hh * 8;
-        s = mfma32_k16(kr[i], d < a.dim ? E::load(q + d) : E::zero(), s);
+      for (int i = 0; i < S::IT; ++i) {
+        int h;
+        const int j = fdivmod(rem + S::row(i), group, inv_group, h);
+        off[i] = S::elt(i) < a.dim ? (uint32_t)(j * (int)a.q_ld + h * (int)a.q_hd + S::elt(i)) * (uint32_t)sizeof(T) : kOOB;
       }
+      sj = fdivmod(rem + (int)(threadIdx.x & 63), group, inv_group, sh);
+    };
+    places();
+    const int step = 64 / group, left = 64 % group;
+    float2 rl;                                // a row's statistics, as they are stored
+    int lim;
+    auto load = [&]() {
+      const auto rq = make_rsrc(static_cast<const T*>(a.q) + ((int64_t)sp.q0 + j0) * a.q_ld + (int64_t)hk * group * a.q_hd, 0x7fffffff);
+      const int here = (int)min(rows - (int64_t)at * 64, (int64_t)64);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = kc + (r >> 2) * 8 + hh * 4 + (r & 3);
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], unit, -rl.x)) * rl.y;
-        sum[r] += key < lim ? p : 0.f;
+      for (int i = 0; i < S::IT; ++i)
+        st.held[i] = __builtin_amdgcn_raw_buffer_load_b128(rq, S::row(i) < here ? off[i] : kOOB, 0, 0);
+      if (threadIdx.x < 64) {
+        lim = 0;
+        rl = make_float2(0.f, 1.f);
+        if ((int)threadIdx.x < here) {
+          lim = visible(sp, j0 + sj, a.causal);
+          const int64_t id = ((int64_t)sp.q0 + j0 + sj) * a.heads + hk * group + sh;
+          rl = a.parts == 1 ? a.rl[id] : joined(a, u, id);
+        }
       }
+      ++at;
+      j0 += step;
+      rem += left;
+      if (left) {
+        if (rem >= group) rem -= group, ++j0;
+        places();
+      }
+    };
+    auto put = [&](int buf) {
+      st.put(tile[buf]);
+      if (threadIdx.x < 64) stat[buf][threadIdx.x] = (f32x4_t){rl.x, share(rl.y, lim), u.unit(rl.x), __int_as_float(lim)};
+    };
+    __syncthreads();                          // the last keys' tiles are read
+    if (tb < te) {
+      load();
+      put(0);
+      if (tb + 1 < te) load();
+      __syncthreads();
+      int buf = 0;
+      int t = tb;
+      // Tiles up to `end`.  Two bodies in one loop would move the sums between registers at each tile.
+      auto pass = [&](auto masked, int end) {
+        for (; t < end; ++t, buf ^= 1) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            f32x16_t s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
+            const int q = m * 32 + l32, z = Lds<T, D>::kswz(q);
+            const T* base = tile[buf] + q * D;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              G qf;
+              if constexpr (sizeof(T) == 2) {
+                qf.v = *reinterpret_cast<const u32x4_t*>(base + ((2 * i + hh) ^ z) * S::PER);
+              } else {
+                qf.lo = *reinterpret_cast<const u32x4_t*>(base + ((4 * i + 2 * hh) ^ z) * S::PER);
+                qf.hi = *reinterpret_cast<const u32x4_t*>(base + ((4 * i + 2 * hh + 1) ^ z) * S::PER);
+              }
+              s = mfma32_k16(kr[i], qf, s);
+            }
+            const f32x4_t c = stat[buf][q];
+            const int room = __float_as_int(c[3]) - kc - hh * 4;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c[2], -c[0]));
+              if constexpr (decltype(masked)::value) sum[r] += (r >> 2) * 8 + (r & 3) < room ? e * c[1] : 0.f;
+              else sum[r] = __builtin_fmaf(e, c[1], sum[r]);
+            }
+          }
+          if (t + 1 < te) put(buf ^ 1);
+          if (t + 2 < te) load();
+          __syncthreads();
+        }
+      };
+      // from which tile on every row sees all of the workgroup's keys, up to the last tile that is whole
+      const int64_t from = a.causal ? min(k0 + 128, (int64_t)sp.k_lim) - 1 - ((int64_t)sp.k_len - sp.q_len) : 0;
+      const int full0 = (int)(min(max(from, (int64_t)0) * group + 63, rows) >> 6), full1 = min((int)(rows >> 6), te);
+      pass(std::true_type{}, min(full0, te));
+      pass(std::false_type{}, full1);
+      pass(std::true_type{}, te);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
 #pragma unroll
       for (int m = 1; m < 32; m <<= 1) sum[r] += __shfl_xor(sum[r], m);
-      const int key = kc + (r >> 2) * 8 + hh * 4 + (r & 3);
-      if (l32 == 0 && key < sp.k_lim) {
-        float* to = acc + (int64_t)key * a.acc_ld;
-        *to = (a.decay == 0.f ? 0.f : a.decay * *to) + sum[r];
+    }
+    if (l32 == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = kc + (r >> 2) * 8 + hh * 4 + (r & 3);
+        if (key >= sp.k_lim) continue;
+        if (parts > 1) {
+          a.scores[((int64_t)part * a.s.n * a.kv + pair) * a.s_ld + key] = sum[r];
+        } else {
+          float* to = acc + (int64_t)key * a.acc_ld;
+          *to = (a.decay == 0.f ? 0.f : a.decay * *to) + sum[r];
+        }
       }
     }
   }
 }
+
+// The parts of the rows, joined in order.
+__device__ __forceinline__ void join_body(const vrs_weights_args& a) {
+  const int pair = blockIdx.x, hk = pair % a.kv;
+  const SeqSpan sp = seq_span(a.s, pair / a.kv);
+  const int64_t key = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  if (key >= sp.k_lim || key >= a.s_ld) return;
+  float* to = a.acc + (sp.k0 + key) * a.acc_ld + hk * a.acc_hd;
+  const float old = a.decay == 0.f ? 0.f : a.decay * *to;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < a.key_parts; ++p) sum += a.scores[((int64_t)p * a.s.n * a.kv + pair) * a.s_ld + key];
+  *to = old + sum;
+}
 }  // namespace
 
-#define VRS_WEIGHTS(TN, T, D)                                                                                                 \
-  extern "C" __global__ __launch_bounds__(256, 2) void vrs_weights_scores_##TN##_d##D(vrs_weights_args a) { stats_body<T, D, true>(a); } \
-  extern "C" __global__ __launch_bounds__(256, 2) void vrs_weights_stats_##TN##_d##D(vrs_weights_args a) { stats_body<T, D, false>(a); } \
-  extern "C" __global__ __launch_bounds__(256, 2) void vrs_weights_keys_##TN##_d##D(vrs_weights_args a) { keys_body<T, D>(a); }
-VRS_WEIGHTS(bf16, bf16_t, 64)
-VRS_WEIGHTS(bf16, bf16_t, 128)
-VRS_WEIGHTS(f32, float, 64)
-VRS_WEIGHTS(f32, float, 128)
+#define VRS_WEIGHTS(TN, T, D, WPS)                                                                                                 \
+  extern "C" __global__ __launch_bounds__(256, 2) void vrs_weights_scores_##TN##_d##D(vrs_weights_args a) { scores_body<T, D>(a); } \
+  extern "C" __global__ __launch_bounds__(256, 2) void vrs_weights_stats_##TN##_d##D(vrs_weights_args a) { stats_body<T, D>(a); } \
+  extern "C" __global__ __launch_bounds__(256, WPS) void vrs_weights_keys_##TN##_d##D(vrs_weights_args a) { keys_body<T, D>(a); }
+VRS_WEIGHTS(bf16, bf16_t, 64, 3)
+VRS_WEIGHTS(bf16, bf16_t, 128, 3)
+VRS_WEIGHTS(f32, float, 64, 2)
+VRS_WEIGHTS(f32, float, 128, 1)
 extern "C" __global__ __launch_bounds__(256) void vrs_weights_sum_bf16(vrs_weights_args a) { sum_body<bf16_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_weights_sum_f32(vrs_weights_args a) { sum_body<float>(a); }
+extern "C" __global__ __launch_bounds__(256) void vrs_weights_join(vrs_weights_args a) { join_body(a); }
