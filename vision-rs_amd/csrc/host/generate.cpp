@@ -428,12 +428,18 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
   a.budget = d->budget; a.first = d->first; a.recent = d->recent;
   a.cols = (int32_t)(d->head_dim / per);
   const int64_t pairs = (int64_t)d->n * d->kv_heads;
-  a.slices = (int32_t)std::clamp<int64_t>(512 / pairs, 1, std::max<int64_t>(1, a.cols * b / 64));
+  // Workgroups of the move: two to a CU.  Slices of 128 bytes of a row (half a cache line costs its whole), of 32
+  // where workgroups would be few; blocks of rows where nothing moves in place.
+  const bool in_place = (k_out == k && k) || (v_out == v && v);
+  const int64_t want = up(512, 2 * pairs), row = (int64_t)d->head_dim * (int64_t)es;
+  a.slices = (int32_t)std::clamp<int64_t>(want, 1, std::max<int64_t>(1, row / (want > 4 && in_place ? 32 : 128)));
+  a.slices = std::min(std::max(a.slices, (int32_t)up(a.cols, 256)), a.cols);      // (a thread to a vector of a slice)
+  const int64_t blocks = in_place ? 1 : std::clamp<int64_t>(want / a.slices, 1, std::max<int64_t>(1, d->budget / 32));
   if (pairs * a.slices >= (1ll << 32) / 1024) return fail(VRS_EBADSHAPE, "%s: grid too large", me);
   if ((rc = launch(ctx, "vrs_evict_choose", dim3((unsigned)pairs), dim3(1024), 0, &a, stream))) return rc;
   char name[64];
   snprintf(name, sizeof name, "vrs_evict_move_b%d", b);
-  return launch(ctx, name, dim3((unsigned)(pairs * a.slices), 2), dim3(256), 0, &a, stream);
+  return launch(ctx, name, dim3((unsigned)(pairs * a.slices), 2, (unsigned)std::min<int64_t>(blocks, 65535)), dim3(256), 0, &a, stream);
 }
 
 }  // extern "C"

@@ -26,33 +26,64 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return x != x ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
+// Sum over the 16 lanes of a row, and over the lanes up to each.
+__device__ __forceinline__ int row_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);      // row_ror 8, 4, 2, 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true);
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true);
+}
+__device__ __forceinline__ int row_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: 0 comes in
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+}
+
 // The choice.  The threshold is the largest T that at least m of the keys that
-// compete reach, found two bits at a time by counting.
-constexpr int kT = 1024, kHeld = 16;        // threads; keys of a thread in registers
+// compete reach, found two bits at a time by counting (a wave counts 64 keys with
+// a comparison and a scalar popcount, and lane i of each wave reads wave i's
+// counts), until one is reached by m keys and no more.
+constexpr int kT = 1024, kHeld = 16, kW = kT / 64;       // threads; keys of a thread in registers; waves
 __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
-  __shared__ int cnt[2][3][kT / 64];
-  __shared__ uint2 pre[2][kT / 64];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  __shared__ __attribute__((aligned(16))) int cnt[2][kW][4];
+  __shared__ int2 pre[2][kW];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int h = blockIdx.x % a.kv, seq = blockIdx.x / a.kv;
   const Keys s = keys_of(a, seq);
   const int n = s.n, keep = min(n, a.budget);
   int* kept = a.kept + ((int64_t)seq * a.kv + h) * a.budget;
   const float* acc = a.acc + s.k0 * a.acc_ld + h * a.acc_hd;
   float* acco = a.acco + s.o0 * a.acco_ld + h * a.acco_hd;
-  const int last = max(n - a.recent, 0);                       // from here on all stay
+  const int first = min(a.first, n), last = max(n - a.recent, first);     // those between compete
   const int rounds = (n + kT - 1) / kT;
   const bool all = n <= a.budget;
   auto value = [&](int i) { return acc[(int64_t)i * a.acc_ld]; };
-  uint32_t held[kHeld];
-#pragma unroll
-  for (int r = 0; r < kHeld; ++r) {
-    const int i = r * kT + tid;
-    held[r] = !all && i >= a.first && i < last ? order_of(value(i)) : 0;   // (0: the order of no number)
-  }
-  const int m = keep - min(a.first, n) - (n - max(last, min(a.first, n)));    // of those that compete
+  float next = tid < n ? value(tid) : 0.f;
+  const int m = all ? 0 : keep - first - (n - last);           // of those that compete
   uint32_t T = 0;
-  if (!all && m > 0) {
-    for (int b = 30, turn = 0; b >= 0; b -= 2, turn ^= 1) {
+  int above = 0;                                               // keys above T
+  bool sharp = m == 0;                                         // those above T are m
+  if (m == 0) T = 0xffffffffu;
+  if (m > 0) {
+    uint32_t held[kHeld];
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      const int i = r * kT + tid;
+      held[r] = i >= first && i < last ? order_of(value(i)) : 0;          // (0: the order of no number)
+    }
+    int turn = 0;
+    auto total = [&](int c1, int c2, int c3, int (&c)[3]) {
+      if (lane == 0) *reinterpret_cast<int4*>(cnt[turn][wave]) = make_int4(c1, c2, c3, 0);
+      __syncthreads();
+      const int4 w = *reinterpret_cast<const int4*>(cnt[turn][lane & (kW - 1)]);
+      c[0] = __builtin_amdgcn_readfirstlane(row_sum(w.x));
+      c[1] = __builtin_amdgcn_readfirstlane(row_sum(w.y));
+      c[2] = __builtin_amdgcn_readfirstlane(row_sum(w.z));
+      turn ^= 1;
+    };
+    int c[3];
+    for (int b = 30; b >= 0 && !sharp; b -= 2) {
       const uint32_t t1 = T | 1u << b, t2 = T | 2u << b, t3 = T | 3u << b;
       int c1 = 0, c2 = 0, c3 = 0;
       auto count = [&](uint32_t o) {
@@ -65,58 +96,52 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
         if (r < rounds) count(held[r]);
       for (int r = kHeld; r < rounds; ++r) {
         const int i = r * kT + tid;
-        count(i >= a.first && i < last ? order_of(value(i)) : 0);
+        count(i >= first && i < last ? order_of(value(i)) : 0);
       }
-      if (lane == 0) cnt[turn][0][wave] = c1, cnt[turn][1][wave] = c2, cnt[turn][2][wave] = c3;
-      __syncthreads();
-      c1 = c2 = c3 = 0;
+      total(c1, c2, c3, c);
+      const int reach = c[2] >= m ? c[2] : c[1] >= m ? c[1] : c[0];
+      T = c[2] >= m ? t3 : c[1] >= m ? t2 : c[0] >= m ? t1 : T;
+      sharp = reach == m;
+    }
+    if (sharp) {
+      --T;                                                     // what is above that is what reaches T
+    } else {
+      int c1 = 0;
 #pragma unroll
-      for (int w = 0; w < kT / 64; ++w) c1 += cnt[turn][0][w], c2 += cnt[turn][1][w], c3 += cnt[turn][2][w];
-      T = c3 >= m ? t3 : c2 >= m ? t2 : c1 >= m ? t1 : T;
+      for (int r = 0; r < kHeld; ++r)
+        if (r < rounds) c1 += __builtin_popcountll(__ballot(held[r] > T));
+      for (int r = kHeld; r < rounds; ++r) {
+        const int i = r * kT + tid;
+        c1 += __builtin_popcountll(__ballot(i >= first && i < last && order_of(value(i)) > T));
+      }
+      total(c1, 0, 0, c);
+      above = c[0];
     }
   }
-  // how many equal ones stay: what the larger ones leave
-  int above = 0;
-  if (!all && m > 0) {
-    int c = 0;
-#pragma unroll
-    for (int r = 0; r < kHeld; ++r)
-      if (r < rounds) c += __builtin_popcountll(__ballot(held[r] > T));
-    for (int r = kHeld; r < rounds; ++r) {
-      const int i = r * kT + tid;
-      c += __builtin_popcountll(__ballot(i >= a.first && i < last && order_of(value(i)) > T));
-    }
-    __syncthreads();
-    if (lane == 0) cnt[0][0][wave] = c;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kT / 64; ++w) above += cnt[0][0][w];
-  }
-  const uint32_t equal = (uint32_t)max(m - above, 0);
+  const int equal = sharp ? 0 : m - above;                     // the earliest of those equal to T stay too
   // places in order: those that stay anyway and those equal to T before each
-  uint32_t sure0 = 0, eq0 = 0;
+  int sure0 = 0, eq0 = 0;
   for (int r = 0; r < rounds; ++r) {
     const int i = r * kT + tid;
-    const float x = i < n ? value(i) : 0.f;
+    const float x = next;
+    if (i + kT < n) next = value(i + kT);                      // (lies behind all that is written before)
     const uint32_t o = order_of(x);
-    const bool in = i < n, competes = in && i >= a.first && i < last;
-    const bool sure = in && (all || !competes || (m > 0 && o > T)), eq = competes && !all && m > 0 && o == T;
+    const bool in = i < n, competes = i >= first && i < last;
+    const bool sure = in && (all || !competes || o > T), eq = competes && equal > 0 && o == T;
     const uint64_t ms = __ballot(sure), me = __ballot(eq);
-    if (lane == 0) pre[r & 1][wave] = make_uint2(__builtin_popcountll(ms), __builtin_popcountll(me));
+    if (lane == 0) pre[r & 1][wave] = make_int2(__builtin_popcountll(ms), __builtin_popcountll(me));
+    asm volatile("" ::"v"(x));
     __syncthreads();                                           // also: the round's values are read
-    uint32_t sb = sure0, eb = eq0;
-#pragma unroll
-    for (int w = 0; w < kT / 64; ++w) {
-      const uint2 c = pre[r & 1][w];
-      if (w < wave) sb += c.x, eb += c.y;
-      sure0 += c.x, eq0 += c.y;
-    }
+    const int2 c = pre[r & 1][lane & (kW - 1)];
+    const int ss = row_scan(c.x), es = row_scan(c.y);          // up to each wave
     const uint64_t below = (1ull << lane) - 1;
-    sb += __builtin_popcountll(ms & below);
-    eb += __builtin_popcountll(me & below);
+    const int sb = sure0 + __builtin_amdgcn_readlane(ss, wave) - __builtin_popcountll(ms) + __builtin_popcountll(ms & below);
+    const int eb = eq0 + __builtin_amdgcn_readlane(es, wave) - __builtin_popcountll(me) + __builtin_popcountll(me & below);
+    sure0 += __builtin_amdgcn_readlane(ss, kW - 1);
+    eq0 += __builtin_amdgcn_readlane(es, kW - 1);
     if (sure || (eq && eb < equal)) {
-      const uint32_t to = sb + min(eb, equal);
-      if (to < (uint32_t)keep) {
+      const int to = sb + min(eb, equal);
+      if (to < keep) {
         kept[to] = i;
         if (s.o0 >= 0 && s.o0 + to < a.o_rows) acco[(int64_t)to * a.acco_ld] = x;
       }
@@ -126,9 +151,10 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
 }
 
 // The move: a workgroup takes a slice of the vectors of one head's rows, of K or of
-// V, and passes over the kept places in order.  A kept key never moves up, so in
-// place a tile's rows may be written once they are read: everything read later
-// lies behind them.
+// V, and passes over the kept places in order (where neither is moved in place,
+// over a block of them).  A kept key never moves up, so in place a tile's rows may
+// be written once they are read: everything read later lies behind them, and may
+// be on its way already.
 template <typename V>
 __device__ __forceinline__ void move_body(const vrs_evict_args& a) {
   constexpr int U = 8, NT = 256;
@@ -137,50 +163,65 @@ __device__ __forceinline__ void move_body(const vrs_evict_args& a) {
   const bool second = blockIdx.y == 1;
   const int64_t k0 = a.k_start[seq], o0 = a.o_start ? a.o_start[seq] : k0;
   const int* kept = a.kept + ((int64_t)seq * a.kv + h) * a.budget;
-  const int c0 = (int)((int64_t)a.cols * slice / a.slices), c1 = (int)((int64_t)a.cols * (slice + 1) / a.slices), w = c1 - c0;
+  const int c0 = (int)((int64_t)a.cols * slice / a.slices), w = (int)((int64_t)a.cols * (slice + 1) / a.slices) - c0;
   // offsets are in vectors
   const int64_t ld = second ? a.v_ld : a.k_ld, hd = second ? a.v_hd : a.k_hd;
   const int64_t old_ = second ? a.vo_ld : a.ko_ld, ohd = second ? a.vo_hd : a.ko_hd;
-  const V* src = static_cast<const V*>(second ? a.v : a.k) + k0 * ld + h * hd + c0;
-  V* dst = static_cast<V*>(second ? a.vo : a.ko) + o0 * old_ + h * ohd + c0;
+  const V* const src = static_cast<const V*>(second ? a.v : a.k) + k0 * ld + h * hd + c0;
+  V* const dst = static_cast<V*>(second ? a.vo : a.ko) + o0 * old_ + h * ohd + c0;
   const bool in_place = static_cast<const void*>(src) == static_cast<const void*>(dst);
   const int room = o0 < 0 || o0 >= a.o_rows ? 0 : (int)min((int64_t)a.budget, a.o_rows - o0);
-  int total = 0;
-  for (int64_t e0 = 0;; e0 += U * NT) {
-    V x[U];
-    int to[U];
-    bool more = false;
+  // w threads to a row (w <= NT), NT / w rows at a time
+  const int rpp = NT / w, tr = tid / w, tc = tid - tr * w;
+  const int b0 = (int)((int64_t)a.budget * blockIdx.z / gridDim.z), b1 = (int)((int64_t)a.budget * (blockIdx.z + 1) / gridDim.z);
+  struct Tile { V x[U]; int from[U]; };      // from: the kept places, then those of them that move
+  auto places = [&](Tile& t, int r0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t e = e0 + u * NT + tid;
-      const int64_t row = e / w;
-      const int c = (int)(e - row * w);
-      const int from = row < a.budget ? kept[row] : -1;
-      to[u] = -1;
-      if (from >= 0) {
-        more = true;
-        if (row < room && !(in_place && from == row)) {
-          x[u] = src[(int64_t)from * ld + c];
-          to[u] = (int)row;
-        }
-      }
+      const int row = r0 + u * rpp + tr;
+      t.from[u] = tr < rpp && row < b1 ? kept[row] : -1;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!__syncthreads_or(more)) break;                        // the tile is read
+  };
+  auto load = [&](Tile& t, int r0) {         // whether the tile has kept places
+    bool any = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t e = e0 + u * NT + tid;
-      if (to[u] >= 0) dst[(int64_t)to[u] * old_ + (e - e / w * w)] = x[u];
+      const int row = r0 + u * rpp + tr;
+      any |= t.from[u] >= 0;
+      if (row >= room || (in_place && t.from[u] == row)) t.from[u] = -1;       // no room, or there already
+      if (t.from[u] >= 0) t.x[u] = src[(int64_t)t.from[u] * ld + tc];
     }
+    return any;
+  };
+  // one tile is loaded, the places of the next are known
+  Tile t, n;
+  places(t, b0);
+  places(n, b0 + U * rpp);
+  bool any = load(t, b0);
+  for (int r0 = b0; r0 < b1; r0 += U * rpp) {
+    const bool more = load(n, r0 + U * rpp);
+    Tile n2;
+    places(n2, r0 + 2 * U * rpp);
+#pragma unroll
+    for (int u = 0; u < U; ++u) asm volatile("" ::"v"(t.x[u]));
+    if (!__syncthreads_or(any)) break;       // the tile is read
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t.from[u] >= 0) dst[(int64_t)(r0 + u * rpp + tr) * old_ + tc] = t.x[u];
+    t = n;
+    n = n2;
+    any = more;
   }
-  if (!second && slice == 0 && h == 0 && a.len_out) {
-    for (int j = tid; j < a.budget; j += NT) total += kept[j] >= 0;
-    __shared__ int sum;
-    if (tid == 0) sum = 0;
-    __syncthreads();
-    atomicAdd(&sum, total);
-    __syncthreads();
-    if (tid == 0) a.len_out[seq] = sum;
+  if (!second && slice == 0 && h == 0 && blockIdx.z == 0 && a.len_out && tid < 64) {
+    int lo = 0, len = a.budget;                                            // the kept ones come first
+    while (len > 1) {
+      const int step = (len + 63) >> 6, i = tid * step;
+      const uint64_t is = __ballot(i < len && kept[lo + i] >= 0);
+      const int hit = is ? 63 - __builtin_clzll(is) : 0;
+      lo += hit * step;
+      len = min(step, len - hit * step);
+    }
+    if (tid == 0) a.len_out[seq] = lo + (kept[lo] >= 0);
   }
 }
 }  // namespace
