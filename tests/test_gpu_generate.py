@@ -202,6 +202,18 @@ def test_prefix_attention_scores_of_minus_infinity(dtype):
     assert got[3].isnan().all() and torch.all(got[4] == 0)
 
 
+def test_prefix_attention_over_its_queries():
+    """out may be q; few and many sequences, tokens and prompts."""
+    import torch
+    for case in ("tokens", "prompts", "many", "group", ([1] * 3, [700, 900, 40], [0, 3], [3000]), ([1] * 90, [9] * 90, [0, 45, 90], [400, 2000])):
+        b = build(case)
+        q, k, v, _ = prefix_inputs(b, "bf16", 32, 4, 128)
+        want = ctx().prefix_attention(q, k, v, b["seqs"], b["prefixes"], out=q.clone())
+        ref, tol = prefix_ref(b, q, k, v, True, 128 ** -0.5, q, "bf16")
+        inside(want, ref, tol)
+        assert torch.equal(ctx().prefix_attention(q, k, v, b["seqs"], b["prefixes"], out=q), want)
+
+
 def test_prefix_attention_far_scores():
     """Prefix and own keys whose scores lie far from each other: the larger take all."""
     for dtype in ("bf16", "f32"):

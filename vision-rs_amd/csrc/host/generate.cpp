@@ -38,7 +38,8 @@ int check_prefixes(const vrs_prefixes* p, const char* me) {
 // Kernels and parts of the prefixes' keys and of the own ones.
 struct PrefixPlan {
   bool pre_few, own_few;
-  int pre_parts, own_parts;
+  bool finish;                      // the own keys' launch finishes; else all parts are joined by a third kernel
+  int pre_parts, own_parts, part_len;
   int64_t pre_rows, own_rows;       // few: row tiles of the longest; else ids of row tiles
 };
 PrefixPlan plan_prefix(const vrs_attention_desc* d, const vrs_seqs* s, const vrs_prefixes* x) {
@@ -47,21 +48,25 @@ PrefixPlan plan_prefix(const vrs_attention_desc* d, const vrs_seqs* s, const vrs
   const int64_t mq = std::max<int64_t>(1, s->max_q > 0 ? std::min(s->max_q, d->q_rows) : up(d->q_rows, n));
   const int64_t mk = s->max_k > 0 ? std::min(s->max_k, d->k_rows) : up(d->k_rows, n);
   const int64_t mr = std::max<int64_t>(1, x->max_rows > 0 ? std::min(x->max_rows, d->q_rows) : up(d->q_rows, g));
-  const int64_t mp = x->max_k > 0 ? std::min(x->max_k, d->k_rows) : up(d->k_rows, g);
+  const int64_t mp = std::max<int64_t>(1, x->max_k > 0 ? std::min(x->max_k, d->k_rows) : up(d->k_rows, g));
   PrefixPlan p;
   p.pre_few = mr * group <= 32;
   p.own_few = mq * group <= 32;
   auto tiles = [&](int64_t count, int64_t rows) { return std::min(d->q_rows * group / 128 + count, count * up(rows * group, 128)); };
   const int64_t pre = (p.pre_few ? g * up(mr * group, 32) : tiles(g, mr)) * d->kv_heads;
   const int64_t own = (p.own_few ? n * up(mq * group, 32) : tiles(n, mq)) * d->kv_heads;
-  p.pre_parts = (int)std::clamp<int64_t>(std::min(up(512, pre), mp / (p.pre_few ? 192 : 128)), 1, 64);
+  // parts of a prefix, all of one length but the last: 512 workgroups where there are 128 keys for each
+  const int64_t parts = std::clamp<int64_t>(std::min(up(512, pre), mp / 128), 1, 64);
+  p.part_len = (int)(up(up(mp, parts), 32) * 32);
+  p.pre_parts = (int)up(mp, p.part_len);
   p.own_parts = (int)std::clamp<int64_t>(std::min(512 / own, mk / 192), 1, 16);
+  p.finish = !p.own_few && p.own_parts == 1;
   p.pre_rows = p.pre_few ? up(mr * group, 32) : d->q_rows * group / 128 + g;
   p.own_rows = p.own_few ? up(mq * group, 32) : d->q_rows * group / 128 + n;
   return p;
 }
 size_t prefix_bytes(const vrs_attention_desc* d, const PrefixPlan& p) {
-  return (size_t)(p.pre_parts + p.own_parts) * d->q_rows * d->heads * (d->head_dim + 2) * 4;
+  return (size_t)(p.pre_parts + (p.finish ? 0 : p.own_parts)) * d->q_rows * d->heads * (d->head_dim + 2) * 4;
 }
 
 }  // namespace
@@ -96,36 +101,37 @@ int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_se
   a.q_ld = d->q_ld; a.q_hd = d->q_hd; a.k_ld = d->k_ld; a.k_hd = d->k_hd;
   a.v_ld = d->v_ld; a.v_hd = d->v_hd; a.o_ld = d->o_ld; a.o_hd = d->o_hd;
   a.heads = d->heads; a.kv = d->kv_heads; a.dim = d->head_dim; a.causal = d->causal != 0;
-  a.parts = p.pre_parts + p.own_parts;
+  a.parts = p.pre_parts + (p.finish ? 0 : p.own_parts);
   a.c = (float)((d->scale > 0.f ? (double)d->scale : 1.0 / std::sqrt((double)d->head_dim)) * 1.4426950408889634);
   a.part_o = static_cast<float*>(workspace);
   a.part_rl = reinterpret_cast<float2*>(a.part_o + (int64_t)a.parts * d->q_rows * d->heads * d->head_dim);
   x.first = prefixes->first; x.p_start = prefixes->k_start; x.p_len = prefixes->k_len; x.groups = prefixes->n;
-  x.pre_parts = p.pre_parts; x.own_parts = p.own_parts;
+  x.pre_parts = p.pre_parts; x.own_parts = p.own_parts; x.part_len = p.part_len; x.finish = p.finish;
   const int64_t pre = (int64_t)d->kv_heads * p.pre_parts * (p.pre_few ? (int64_t)prefixes->n : p.pre_rows);
   const int64_t own = (int64_t)d->kv_heads * p.own_parts * (p.own_few ? (int64_t)seqs->n : p.own_rows);
-  const int64_t joins = up((int64_t)d->q_rows * d->heads * (d->head_dim / 4), 256);
-  if (p.pre_rows >= (1 << 16) * 256ll || p.own_rows >= (1 << 16) * 256ll || pre + own >= (1ll << 32) / 512 || joins >= (1ll << 32) / 256)
+  const int64_t per_row = up((int64_t)d->heads * (d->head_dim / 4), 256);
+  if (p.pre_rows >= (1 << 16) * 256ll || p.own_rows >= (1 << 16) * 256ll || pre + own >= (1ll << 32) / 512 ||
+      d->q_rows >= (1 << 24) || per_row > 65535)
     return fail(VRS_EBADSHAPE, "%s: grid too large", me);
   const int D = d->head_dim <= 64 ? 64 : 128;
   char name[64];
-  auto go = [&](bool few, int64_t pre_blocks, int64_t own_blocks) {
+  // (row tiles past the grid's are taken in turn)
+  x.pre_rows = (int32_t)std::min<int64_t>(p.pre_rows, 65535); x.own_rows = (int32_t)std::min<int64_t>(p.own_rows, 65535);
+  auto go = [&](const char* kind, int64_t pre_blocks, int64_t own_blocks) {
     x.pre_blocks = (int32_t)pre_blocks;
-    // (row tiles past the grid's are taken in turn)
-    x.pre_rows = (int32_t)std::min<int64_t>(p.pre_rows, 65535); x.own_rows = (int32_t)std::min<int64_t>(p.own_rows, 65535);
-    const int y = !few ? 1 : std::max(pre_blocks ? x.pre_rows : 1, own_blocks ? x.own_rows : 1);
-    snprintf(name, sizeof name, "vrs_prefix_%s_%s_d%d", few ? "few" : "prompt", dsuffix(d->dtype), D);
+    const int y = std::max(pre_blocks && p.pre_few ? x.pre_rows : 1, own_blocks && p.own_few ? x.own_rows : 1);
+    snprintf(name, sizeof name, "vrs_prefix_%s_%s_d%d", kind, dsuffix(d->dtype), D);
     return launch(ctx, name, dim3((unsigned)(pre_blocks + own_blocks), (unsigned)y), dim3(256), 0, &x, stream);
   };
-  if (p.pre_few == p.own_few) {
-    rc = go(p.pre_few, pre, own);
+  if (p.own_few) {
+    rc = go(p.pre_few ? "few" : "mixed", pre, own);
   } else {
-    rc = go(p.pre_few, pre, 0);
-    if (!rc) rc = go(p.own_few, 0, own);
+    rc = go(p.pre_few ? "few" : "prompt", pre, 0);
+    if (!rc) rc = go("own", 0, own);
   }
-  if (rc) return rc;
+  if (rc || p.finish) return rc;
   snprintf(name, sizeof name, "vrs_prefix_join_%s", dsuffix(d->dtype));
-  return launch(ctx, name, dim3((unsigned)joins), dim3(256), 0, &x, stream);
+  return launch(ctx, name, dim3((unsigned)d->q_rows, (unsigned)per_row), dim3(256), 0, &x, stream);
 }
 
 }  // extern "C"

@@ -394,6 +394,8 @@ typedef struct {
   const int32_t* p_len;    /* [groups] */
   int32_t groups;
   int32_t pre_parts, own_parts;
+  int32_t part_len;        /* keys of a prefix to a part; the last part takes what is left */
+  int32_t finish;          /* the own keys' launch joins the prefix's parts and finishes */
   int32_t pre_blocks;      /* workgroups of the launch that take prefixes (in x; the others own keys) */
   int32_t pre_rows, own_rows;   /* few rows: row tiles of either kind (in y) */
 } vrs_prefix_args;

@@ -33,7 +33,7 @@ __device__ __forceinline__ void prompt_kernel(const vrs_attention_args& a) {
   const int part = rest % a.parts;
   const TilePlace at = place_tile<32 * NW * QT>(Sequences{a.s}, a.heads / a.kv, rest / a.parts);
   if (at.tile < 0) return;
-  prompt_body<T, D, KT, QT, NW>(a, {at.sp, hk, at.tile, 0, part, a.parts, part, a.causal, a.parts == 1});
+  prompt_body<T, D, KT, QT, NW>(a, {at.sp, hk, at.tile, 0, part, a.parts, part, a.causal, a.parts == 1, 0, 0, 0});
 }
 // Few queries: no two workgroups share keys: in the order of launch, round the XCDs, the sequences with
 // the most keys first.
@@ -42,7 +42,7 @@ __device__ __forceinline__ void few_kernel(const vrs_attention_args& a) {
   const int hk = blockIdx.x % a.kv, rest = blockIdx.x / a.kv;
   const int part = rest % a.parts;
   few_body<T, D, NW>(a, {ranked_seq(Sequences{a.s}, rest / a.parts), hk, (int)blockIdx.y, (int)gridDim.y, part, a.parts, part,
-                         a.causal, a.parts == 1});
+                         a.causal, a.parts == 1, 0, 0, 0});
 }
 
 // ---------------------------------------------------------------------------

@@ -13,7 +13,23 @@ struct AttentionJob {
   int out_part;         // which part of the workspace; direct: results go to `out`, finished
   int causal;
   bool direct;
+  int part_len;         // keys of a part (the last one takes what is left); 0: parts of one length
+  int joined;           // prompts: finished results take in so many parts of the workspace, of so many keys in all
+  int joined_keys;
 };
+// Keys [kb, ke) of a job's part of `keys`.
+__device__ __forceinline__ void keys_of(const AttentionJob& job, int keys, int unit, int& kb, int& ke) {
+  if (job.part_len == 0) return part_of(keys, job.part, job.parts, unit, kb, ke);
+  kb = (int)min((int64_t)job.part * job.part_len, (int64_t)keys);
+  ke = job.part == job.parts - 1 ? keys : (int)min((int64_t)(job.part + 1) * job.part_len, (int64_t)keys);
+}
+
+// The prompts' K and V tiles; one object for all bodies of a kernel that name it.
+template <typename T, int D, int KT>
+__device__ __forceinline__ T* prompt_lds() {
+  __shared__ __attribute__((aligned(16))) T smem[3 * 2 * KT * D];
+  return smem;
+}
 
 // ---------------------------------------------------------------------------
 // Prompts: a workgroup of 4 waves takes 128 * QT rows, the queries of all heads
@@ -53,7 +69,6 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
   constexpr int CH = Lds<T, D>::CH, PER = 16 / (int)sizeof(T);
   constexpr int IT = KT * CH / NT;                 // chunks a thread stages of K, and of V
   constexpr int TILE = KT * D;
-  __shared__ __attribute__((aligned(16))) T smem[3 * 2 * TILE];    // three times K, V
   __shared__ int odd_tile[3];     // first key of the tile that a buffer holds, if it had values not finite
   const int tid = threadIdx.x, wave = tid >> 6;
   const int hk = job.hk;
@@ -81,7 +96,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
     w.load_q(q, static_cast<const T*>(a.q) + qrow[q] * a.q_ld + head[q] * a.q_hd, a.dim, ok[q]);
   }
   int kb, ke;
-  part_of(visible(sp, (int)((min(r0 + BM, rows) - 1) / group), job.causal), job.part, job.parts, KT, kb, ke);
+  keys_of(job, visible(sp, (int)((min(r0 + BM, rows) - 1) / group), job.causal), KT, kb, ke);
   const int all = visible(sp, (int)(r0 / group), job.causal);   // keys that every row of the workgroup sees
   const int mine = __builtin_amdgcn_readlane(w.lim[QT - 1], 31);   // keys that some row of the wave sees
 
@@ -98,7 +113,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
     ko[i] = kc < a.dim ? (uint32_t)(row * (int)a.k_ld + kc) * (uint32_t)sizeof(T) : kOOB;
     vo[i] = vc < a.dim ? (uint32_t)(row * (int)a.v_ld + vc) * (uint32_t)sizeof(T) : kOOB;
   }
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem + wave * 1024);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)prompt_lds<T, D, KT>() + wave * 1024);
   auto load = [&](int buf, int kc) {
     const int n = min(KT, sp.k_lim - kc);
     const i32x4_hw rk = lds_rsrc(kp + (int64_t)kc * a.k_ld, (int)(((n - 1) * a.k_ld + a.dim) * (int)sizeof(T)));
@@ -114,7 +129,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      u32x4_t* at = reinterpret_cast<u32x4_t*>(smem + (buf * 2 + 1) * TILE) + (i * NW + wave) * 64 + (tid & 63);
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(prompt_lds<T, D, KT>() + (buf * 2 + 1) * TILE) + (i * NW + wave) * 64 + (tid & 63);
       u32x4_t u = *at;
       if (clean<T>(u)) {
         *at = u;
@@ -144,13 +159,13 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
         t[q] = w.top(s[q]);
       }
     };
-    w.scores(smem, 0, s);
+    w.scores(prompt_lds<T, D, KT>(), 0, s);
     look(kb + 32 > all, kb);
     // TAIL: some row does not see the whole of this or the next tile, or no tile follows
     auto tile = [&](auto tail, int buf, bool more) {
       constexpr bool TAIL = decltype(tail)::value;
       const int nbuf = buf == 2 ? 0 : buf + 1;
-      const T* sK = smem + buf * 2 * TILE;
+      const T* sK = prompt_lds<T, D, KT>() + buf * 2 * TILE;
       if (TAIL && kc + KT > all) clean_tile(buf, kc);
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
@@ -163,7 +178,7 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
         f32x16_t s1[QT];
         const bool ahead = !TAIL || ((!last || more) && kc + (n + 1) * 32 < mine);
         __builtin_amdgcn_s_setprio(1);
-        if (ahead) w.scores(last ? smem + nbuf * 2 * TILE : sK, last ? 0 : (n + 1) * 32, s1);
+        if (ahead) w.scores(last ? prompt_lds<T, D, KT>() + nbuf * 2 * TILE : sK, last ? 0 : (n + 1) * 32, s1);
         if (live) {
           typename Wave<T, D, QT>::P p[QT];
 #pragma unroll
@@ -189,6 +204,14 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
     }
     for (int buf = 0; kc < ke; buf = buf == 2 ? 0 : buf + 1) tile(std::true_type{}, buf, kc + KT < ke);
   }
+  if (job.joined) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+      const int64_t i = qrow[q] * a.heads + head[q];
+      w.take_parts(q, a.part_o + i * a.dim, a.part_rl + i, (int64_t)a.s.q_rows * a.heads, job.joined, a.dim, u);
+      w.lim[q] = (int)min((int64_t)w.lim[q] + job.joined_keys, (int64_t)0x7fffffff);
+    }
+  }
 #pragma unroll
   for (int q = 0; q < QT; ++q) {
     if (job.direct) {
@@ -209,7 +232,9 @@ __device__ __forceinline__ void prompt_body(const vrs_attention_args& a, const A
 // row to a lane), V through a wave's own LDS tile for the transposed reads,
 // the next tile's loads in flight meanwhile.  64 tokens over 500 .. 8000 keys,
 // 32 heads on 8 of 128, 1.14 GB: 233 us, 4.9 TB/s.
-template <typename T, int D, int NW>
+// SHARED: in the LDS of the prompts' body, for a kernel that has both.  It holds the
+// O of two waves, so that the upper two are added to the lower two first.
+template <typename T, int D, int NW, bool SHARED = false>
 __device__ __forceinline__ void few_body(const vrs_attention_args& a, const AttentionJob& job) {
   using E = Elt<T>;
   using G = typename E::group;
@@ -217,15 +242,23 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a, const Atte
   constexpr int IT = 32 * CH / 64;                 // V chunks of a lane
   constexpr int OL = D + 4;                        // O row in LDS (float32)
   constexpr int V_BYTES = NW * 32 * D * (int)sizeof(T), O_BYTES = NW * 32 * OL * 4;
-  __shared__ __attribute__((aligned(16))) char mem[V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
+  static_assert(!SHARED || (NW == 4 && (V_BYTES > O_BYTES / 2 ? V_BYTES : O_BYTES / 2) <= 6 * 32 * D * (int)sizeof(T)), "");
+  __shared__ __attribute__((aligned(16))) char mem[SHARED ? 16 : V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
   __shared__ float sR[NW][32], sl[NW][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int hk = job.hk;
   const SeqSpan sp = job.sp;
   const int G_ = a.heads / a.kv;
   const int64_t rows = (int64_t)sp.q_len * G_;
-  T* sV = reinterpret_cast<T*>(mem) + wave * 32 * D;
-  float* sO = reinterpret_cast<float*>(mem);
+  T* sV;
+  float* sO;
+  if constexpr (SHARED) {
+    sV = prompt_lds<T, D, 32>() + wave * 32 * D;
+    sO = reinterpret_cast<float*>(prompt_lds<T, D, 32>());
+  } else {
+    sV = reinterpret_cast<T*>(mem) + wave * 32 * D;
+    sO = reinterpret_cast<float*>(mem);
+  }
 
   const Log2 u(a.c);
   // row tiles of the sequence, one workgroup each (and more than were counted on, in turn)
@@ -241,7 +274,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a, const Atte
     w.load_q(0, static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd, a.dim, ok);
     const int lim_min = __builtin_amdgcn_readfirstlane(lim), lim_max = __builtin_amdgcn_readlane(lim, 31);
     int kb, ke;
-    part_of(lim_max, job.part, job.parts, 32, kb, ke);
+    keys_of(job, lim_max, 32, kb, ke);
 
     const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.k_ld + (int64_t)hk * a.k_hd;
     const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.v_ld + (int64_t)hk * a.v_hd;
@@ -299,18 +332,42 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a, const Atte
       __builtin_amdgcn_wave_barrier();
     }
     // join the waves: the largest reference, sums and O scaled to it
-    const float lt = sum32(w.l[0]);
+    float lt = sum32(w.l[0]);
+    constexpr int NJ = SHARED ? 2 : NW;    // of so many waves
+    auto put = [&](int at) {
+      if (w.hh == 0) {
+        sR[at][w.l32] = w.R[0];
+        sl[at][w.l32] = lt;
+      }
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4_t*>(&sO[(at * 32 + w.l32) * OL + d * 32 + g * 8 + w.hh * 4]) =
+              (f32x4_t){w.o[0][d][4 * g], w.o[0][d][4 * g + 1], w.o[0][d][4 * g + 2], w.o[0][d][4 * g + 3]};
+    };
     __syncthreads();                       // every wave is done with its V tile
-    if (w.hh == 0) {
-      sR[wave][w.l32] = w.R[0];
-      sl[wave][w.l32] = lt;
+    if constexpr (SHARED) {
+      if (wave >= 2) put(wave - 2);
+      __syncthreads();
+      if (wave < 2) {
+        const float other = sR[wave][w.l32], mx = fmaxf(w.R[0], other);
+        const float mine = u.factor(w.R[0], mx), its = u.factor(other, mx);
+        lt = mine * lt + its * sl[wave][w.l32];
+        w.R[0] = mx;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&sO[(wave * 32 + w.l32) * OL + d * 32 + g * 8 + w.hh * 4]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w.o[0][d][4 * g + k] = mine * w.o[0][d][4 * g + k] + its * v[k];
+          }
+        put(wave);                         // where it has read, and no other wave has
+      }
+    } else {
+      put(wave);
     }
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4_t*>(&sO[(wave * 32 + w.l32) * OL + d * 32 + g * 8 + w.hh * 4]) =
-            (f32x4_t){w.o[0][d][4 * g], w.o[0][d][4 * g + 1], w.o[0][d][4 * g + 2], w.o[0][d][4 * g + 3]};
     __syncthreads();
     // 2 NW threads to a row, 4 elements at a time
     const int rr = threadIdx.x / (2 * NW), e0 = threadIdx.x % (2 * NW) * 4;
@@ -319,10 +376,10 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a, const Atte
       const int64_t orow = sp.q0 + jj;
       float mx = sR[0][rr];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sR[i][rr]);
-      float f[NW], lsum = 0.f;
+      for (int i = 1; i < NJ; ++i) mx = fmaxf(mx, sR[i][rr]);
+      float f[NJ], lsum = 0.f;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) {       // a wave without keys has l = 0, O = 0
+      for (int i = 0; i < NJ; ++i) {       // a wave without keys has l = 0, O = 0
         f[i] = u.factor(sR[i][rr], mx);
         lsum += f[i] * sl[i][rr];
       }
@@ -333,7 +390,7 @@ __device__ __forceinline__ void few_body(const vrs_attention_args& a, const Atte
       for (int e = e0; e < a.dim; e += 8 * NW) {
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NW; ++i) v += f[i] * *reinterpret_cast<const f32x4_t*>(&sO[(i * 32 + rr) * OL + e]);
+        for (int i = 0; i < NJ; ++i) v += f[i] * *reinterpret_cast<const f32x4_t*>(&sO[(i * 32 + rr) * OL + e]);
         v *= inv;
         if (!job.direct) {
           *reinterpret_cast<f32x4_t*>(a.part_o + at * a.dim + e) = v;

@@ -310,6 +310,36 @@ struct Wave {
     }
   }
 
+  // adds parts of a workspace, `step` (row, head) apart, to the query's O, reference and sum
+  __device__ __forceinline__ void take_parts(int q, const float* po, const float2* prl, int64_t step, int parts, int dim,
+                                             const Log2& u) {
+    float mx = R[q];
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) mx = fmaxf(mx, prl[i * step].x);
+    const float mine = u.factor(R[q], mx);
+    R[q] = mx;
+    unit[q] = u.unit(mx);
+    l[q] *= mine;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) o[q][d] *= mine;
+#pragma unroll 1
+    for (int i = 0; i < parts; ++i) {
+      const float2 rl = prl[i * step];
+      const float f = u.factor(rl.x, mx);
+      if (hh == 0) l[q] += f * rl.y;         // (the halves of the wave add up their sums)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int e = d * 32 + g * 8 + hh * 4;
+          f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+          if (e < dim) v = *reinterpret_cast<const f32x4_t*>(po + i * step * dim + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[q][d][4 * g + k] += f * v[k];
+        }
+    }
+  }
+
   // the unfinished query to a workspace: O (float32), reference, sum
   __device__ __forceinline__ void store_part(int q, float* po, float2* prl, int dim, bool ok) const {
     const float lt = sum32(l[q]);
