@@ -399,6 +399,16 @@ def test_beam_select_of_masks_at_the_end_of_the_range(dtype):
     check_select(x, s, 12)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_beam_select_of_beams_with_like_scores(dtype):
+    """Many beams and chunks of which any may hold the best: far more entries reach the first threshold than are kept."""
+    import torch
+    for beams, vocab, k in ((26, 60405, 26), (64, 30000, 128), (40, 9000, 60)):
+        x, s = logits_of(2, beams, vocab, dtype, seed=beams, scale=2.0), scores_of(2, beams) * 1e-3
+        check_select(x, s, k)
+        check_select(x.round(), torch.zeros_like(s), k)
+
+
 def test_beam_select_equal_beams():
     """The same logits and score in every beam: equal candidates by the lowest beam."""
     x = logits_of(2, 1, 3000, "f32", seed=9).expand(2, 6, 3000).contiguous()

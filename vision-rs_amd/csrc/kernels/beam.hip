@@ -197,8 +197,10 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
   __shared__ uint8_t kind[64];                 // 0: nothing but -infinity, 1: its lists, 2: the end token alone
   __shared__ __attribute__((aligned(16))) uint64_t co[kCand];
   __shared__ __attribute__((aligned(16))) uint32_t cat[kCand];
+  __shared__ uint64_t ko[kCand];
+  __shared__ uint32_t kat[kCand];
   __shared__ __attribute__((aligned(16))) uint32_t smax[kT];
-  __shared__ int count;
+  __shared__ int count, kept;
   __shared__ uint32_t sth;
   __shared__ uint64_t so[kWaves];
   __shared__ uint32_t sat[kWaves];
@@ -243,16 +245,18 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
       kind[i] = !(s - s == 0.f) ? 0 : done ? 2 : !(l > 0.0 && l < INFINITY && m > -INFINITY && m < INFINITY) ? 0 : 1;
     }
   }
-  if (tid == 0) count = 0, sth = 0;
+  if (tid == 0) count = 0, kept = 0, sth = 0;
   __syncthreads();
+  const float inv_chunks = 1.f / (float)a.chunks;
   // an entry's order (0: none) and flat place
   auto valued = [&](int l, int j, uint2 e, uint64_t& o, uint32_t& at) {
-    const int i = l / a.chunks, k = kind[i];
+    int c;
+    const int i = fdivmod(l, a.chunks, inv_chunks, c), k = kind[i];
     o = 0;
     if (k == 1 && e.y != 0xffffffffu) {
       o = order64(score[i] + ((double)__uint_as_float(e.x) - lse[i]));
       at = (uint32_t)(i * a.vocab) + e.y;
-    } else if (k == 2 && j == 0 && l == i * a.chunks) {
+    } else if (k == 2 && j == 0 && c == 0) {
       o = order64(score[i]);
       at = (uint32_t)(i * a.vocab + a.eos);
     }
@@ -279,32 +283,86 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
   }
   if (above < a.k && reach >= a.k) sth = top;
   __syncthreads();
-  const uint32_t T0 = max(sth, 1u);
-  auto take = [&](uint64_t o, uint32_t at) {
-    if ((uint32_t)(o >> 32) < T0) return false;
-    const int p = atomicAdd(&count, 1);
-    if (p < kCand) co[p] = o, cat[p] = at;
-    return true;
-  };
-  bool more = l0 < lists;
+  uint32_t T0 = max(sth, 1u);
+  // what reaches T0: a thread's entries eight at a time, on their way together
+  auto collect = [&]() {
+    auto take = [&](uint64_t o, uint32_t at) {
+      if ((uint32_t)(o >> 32) < T0) return false;
+      const int p = atomicAdd(&count, 1);
+      if (p < kCand) co[p] = o, cat[p] = at;
+      return true;
+    };
+    for (int l = l0; l < lists; l += kT >> lg) {
+      bool more = true;
+      int j = j0;
+      if (l == l0) {
 #pragma unroll
-  for (int i = 0; i < kEarly; ++i) {
-    uint64_t o = 0;
-    uint32_t at = 0;
-    if (more) valued(l0, j0 + i * per, early[i], o, at);
-    more = more && take(o, at);
-  }
-  for (int l = l0; l < lists; l += kT >> lg) {
-    if (l == l0 && !more) continue;
-    for (int j = j0 + (l == l0 ? kEarly * per : 0); j < a.k; j += per) {
-      uint64_t o;
-      uint32_t at = 0;
-      entry(l, j, o, at);
-      if (!take(o, at)) break;
+        for (int i = 0; i < kEarly; ++i, j += per) {
+          uint64_t o = 0;
+          uint32_t at = 0;
+          if (more) valued(l0, j, early[i], o, at);
+          more = more && take(o, at);
+        }
+      }
+      for (; more && j < a.k; j += 8 * per) {
+        uint2 e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = j + i * per < a.k ? base[(int64_t)l * a.k + j + i * per] : make_uint2(0, 0xffffffffu);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint64_t o = 0;
+          uint32_t at = 0;
+          if (more) valued(l, j + i * per, e[i], o, at);
+          more = more && take(o, at);
+        }
+      }
+    }
+    __syncthreads();
+    return count;
+  };
+  int have = collect();
+  // The k-th largest (in the upper bits) of those that LDS holds bounds that of all.
+  auto bound = [&]() {
+    uint32_t mine[kCand / kT], t = 0;
+#pragma unroll
+    for (int i = 0; i < kCand / kT; ++i) mine[i] = i * kT + tid < have ? (uint32_t)(co[i * kT + tid] >> 32) : 0;
+    for (int bit = 31; bit >= 6; --bit) {
+      const uint32_t trial = t | 1u << bit;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < kCand / kT; ++i) c += __builtin_popcountll(__ballot(mine[i] >= trial));
+      if (lane == 0) smax[(bit & 1) * kWaves + wave] = c;
+      __syncthreads();
+      const u32x4_t n = reinterpret_cast<const u32x4_t*>(smax)[bit & 1];
+      if ((int)(n[0] + n[1] + n[2] + n[3]) >= a.k) t = trial;
+    }
+    return t;
+  };
+  if (have > kCand) {                          // beams of like scores
+    const uint32_t T1 = bound();
+    if (T1 > T0) {
+      T0 = T1;
+      __syncthreads();                         // the count is read
+      if (tid == 0) count = 0;
+      __syncthreads();
+      have = collect();
     }
   }
-  __syncthreads();
-  const int have = count;
+  // Ranks cost their number squared: those that cannot be among the k leave first.
+  uint64_t* ro = co;
+  uint32_t* rat = cat;
+  int ranked = min(have, kCand);
+  if (have > 2 * a.k + 32 && have <= kCand) {
+    const uint32_t T1 = bound();
+    for (int i = tid; i < have; i += kT) {
+      if ((uint32_t)(co[i] >> 32) < T1) continue;
+      const int p = atomicAdd(&kept, 1);
+      ko[p] = co[i], kat[p] = cat[i];
+    }
+    __syncthreads();
+    ro = ko, rat = kat;
+    ranked = kept;
+  }
   auto put = [&](int k, uint64_t o, uint32_t at) {
     const uint64_t bits = o ^ (((int64_t)o >> 63) ? 0x8000000000000000ull : ~0ull);
     a.out_scores[(int64_t)b * a.k + k] = (float)__builtin_bit_cast(double, bits);
@@ -313,12 +371,12 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
   };
   int got = min(have, a.k);
   if (have <= kCand) {
-    for (int i = tid; i < have; i += kT) {
-      const uint64_t o = co[i];
-      const uint32_t at = cat[i];
+    for (int i = tid; i < ranked; i += kT) {
+      const uint64_t o = ro[i];
+      const uint32_t at = rat[i];
       int r = 0;
 #pragma unroll 8
-      for (int j = 0; j < have; ++j) r += co[j] > o || (co[j] == o && cat[j] < at);
+      for (int j = 0; j < ranked; ++j) r += ro[j] > o || (ro[j] == o && rat[j] < at);
       if (r < a.k) put(r, o, at);
     }
   } else {
