@@ -38,6 +38,37 @@ __device__ __forceinline__ uint32_t reached(uint32_t o, int r) {
   return t;
 }
 
+// Over the lanes of a wave by DPP: shifts inside rows of 16, then rows into the next; lane 63 has all.
+template <int C, int ROWS>
+__device__ __forceinline__ float dpp(float old, float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(old), __float_as_uint(x), C, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp<0x111, 0xf>(x, x));
+  x = fmaxf(x, dpp<0x112, 0xf>(x, x));
+  x = fmaxf(x, dpp<0x114, 0xf>(x, x));
+  x = fmaxf(x, dpp<0x118, 0xf>(x, x));
+  x = fmaxf(x, dpp<0x142, 0xa>(x, x));
+  x = fmaxf(x, dpp<0x143, 0xc>(x, x));
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+template <int C, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)b, C, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(b >> 32), C, ROWS, 0xf, false);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// lane 63's is the sum
+__device__ __forceinline__ double wave_sum(double x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  return dpp_add<0x143, 0xc>(x);
+}
+
 // Maximum over the workgroup of (order, -place): the lowest place of the largest.
 __device__ __forceinline__ void best_of(uint64_t& o, uint32_t& at, uint64_t (&so)[kWaves], uint32_t (&sat)[kWaves]) {
 #pragma unroll
@@ -55,16 +86,16 @@ __device__ __forceinline__ void best_of(uint64_t& o, uint32_t& at, uint64_t (&so
 }
 
 // ---------------------------------------------------------------------------
-// A chunk of one row: VT vectors of 16 bytes to a thread.  The sum is of 2^((x - m) L), L = log2 e rounded to
-// float32, and lse = m + log2(sum) / L with the same L, so that its rounding (1.3e-8) counts times the entropy only.
-// (One FMA of x L - m L would serve, but not at the ends of the range, where masks lie.)  A NaN or +infinity makes
-// the sum NaN.
+// A chunk of one row: VT vectors of 16 bytes to a thread.  The sum is of 2^(x L - R), L = log2 e rounded to float32
+// and R = m L rounded, one FMA and one v_exp to a logit, and lse = (R + log2 sum) / L, so that R's rounding falls out
+// and L's (1.3e-8) counts times the entropy only.  A NaN or +infinity makes the sum NaN.
 constexpr float kL = 1.44269502f;
 template <typename T, int VT>
 __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   constexpr int V = 16 / (int)sizeof(T), N = VT * V;
-  __shared__ __attribute__((aligned(16))) uint2 cand[kCand];
-  __shared__ int count;
+  constexpr int kEach = kCand / kWaves;
+  __shared__ __attribute__((aligned(16))) uint64_t cand[kWaves][kEach];
+  __shared__ int count[kWaves];
   __shared__ float swm[kWaves];
   __shared__ double sws[kWaves];
   __shared__ uint32_t sth[kWaves], salone[kWaves];
@@ -114,59 +145,59 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   const uint32_t top = m == -INFINITY ? 0 : order32(m);
   const uint32_t each = reached(top, (a.k + kWaves - 1) / kWaves);
   const uint32_t alone = n < N * kT && a.k <= 64 ? reached(top, a.k) : 0;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  m = wave_max(m);
   if (lane == 0) swm[wave] = m, sth[wave] = each, salone[wave] = alone;
-  if (tid == 0) count = 0;
   __syncthreads();
   m = fmaxf(fmaxf(swm[0], swm[1]), fmaxf(swm[2], swm[3]));
   uint32_t T0 = min(min(sth[0], sth[1]), min(sth[2], sth[3]));
   T0 = max(T0, max(max(salone[0], salone[1]), max(salone[2], salone[3])));
   const float Tf = T0 ? __uint_as_float(T0 ^ ((int32_t)T0 < 0 ? 0x80000000u : 0xffffffffu)) : -3.40282347e38f;
-  // candidates (none is -infinity or NaN): a wave's places by one addition, then what each ballot holds
+  // candidates (none is -infinity or NaN), each wave's in its own part of the list
   int mine = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) mine += __builtin_popcountll(__ballot(v[i] >= Tf));
-  int base = 0;
-  if (lane == 0 && mine) base = atomicAdd(&count, mine);
+  for (int i = 0; i < N; ++i) {
+    const bool in = v[i] >= Tf;
+    const uint64_t mask = __ballot(in);
+    if (mask == 0) continue;
+    const int p = mine + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (in && p < kEach) cand[wave][p] = (uint64_t)order32(v[i]) << 32 | ~token(i);
+    mine += __builtin_popcountll(mask);
+  }
+  if (lane == 0) count[wave] = mine;
   const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
+  if (fabsf(ref) < 1e30f) {
+    const float R = ref * kL;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * kL);
-  double total = sum;
+    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[i], kL, -R));
+  } else {                                     // where masks lie at the ends of the range
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1) total += __shfl_xor(total, k);
-  if (lane == 0) sws[wave] = total;
-  base = __builtin_amdgcn_readfirstlane(base);
-  if (mine) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint64_t mask = __ballot(v[i] >= Tf);
-      if (mask == 0) continue;
-      const int p = base + __builtin_popcountll(mask & ((1ull << lane) - 1));
-      if (v[i] >= Tf && p < kCand) cand[p] = make_uint2(order32(v[i]), token(i));
-      base += __builtin_popcountll(mask);
-    }
+    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * kL);
   }
+  const double total = wave_sum(sum);
+  if (lane == 63) sws[wave] = total;
   __syncthreads();
   const int64_t at = (int64_t)row * a.chunks + ch;
-  if (tid == 0) a.part[at] = make_double2((double)m * kL, sws[0] + sws[1] + sws[2] + sws[3]);
+  if (tid == 0)
+    a.part[at] = make_double2(fabsf(ref) < 1e30f && m > -INFINITY ? (double)(ref * kL) : (double)m * kL, sws[0] + sws[1] + sws[2] + sws[3]);
   uint2* list = a.list + at * a.k;
-  const int have = count;
-  auto logit = [](uint32_t o) { return o ^ (((int32_t)o >> 31) ? 0x80000000u : 0xffffffffu); };
-  if (have <= kCand) {
-    for (int i = tid; i < have; i += kT) {
-      const uint2 me = cand[i];
-      int rank = 0;
-      for (int j = 0; j < have; j += 8) {
+  int have = 0, most = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const u32x4_t c = reinterpret_cast<const u32x4_t*>(cand + j)[e];
-          rank += c[0] > me.x || (c[0] == me.x && c[1] < me.y);
-          rank += c[2] > me.x || (c[2] == me.x && c[3] < me.y);
+  for (int w = 0; w < kWaves; ++w) have += count[w], most = max(most, count[w]);
+  auto logit = [](uint32_t o) { return o ^ (((int32_t)o >> 31) ? 0x80000000u : 0xffffffffu); };
+  if (most <= kEach) {
+    for (int i = lane; i < mine; i += 64) {
+      const uint64_t me = cand[wave][i];       // larger logits, then smaller tokens, are larger numbers
+      int rank = 0;
+#pragma unroll 1
+      for (int w = 0; w < kWaves; ++w) {
+        const int n8 = count[w];
+        for (int j = 0; j < n8; j += 8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) rank += cand[w][j + e] > me;
         }
       }
-      if (rank < a.k) list[rank] = make_uint2(logit(me.x), me.y);
+      if (rank < a.k) list[rank] = make_uint2(logit((uint32_t)(me >> 32)), ~(uint32_t)me);
     }
     if (tid < a.k && tid >= have) list[tid] = make_uint2(0, 0xffffffffu);
   } else {
