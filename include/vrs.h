@@ -552,7 +552,7 @@ typedef struct {
  * alignment, the rounding and the workspace are vrs_attention's, and so is the
  * result: a query that sees no key gets 0.  A prefix is read once for up to 128
  * rows (queries times heads of a key head) of its group instead of once for each
- * sequence. */
+ * sequence.  Fewer than 2^24 rows of q. */
 size_t vrs_prefix_attention_workspace_size(const vrs_attention_desc* d, const vrs_seqs* seqs,
                                            const vrs_prefixes* prefixes);
 int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_seqs* seqs, const vrs_prefixes* prefixes,
@@ -572,7 +572,7 @@ int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_se
  * +infinity, or nothing else than -infinity.
  * logits: rows (beams of all requests, one after another) of contiguous elements,
  * ld elements apart, of any alignment of their elements.  k <= 128 and
- * <= beams * vocab, beams <= 64, beams * vocab < 2^31.
+ * <= beams * vocab, beams <= 64, beams * vocab < 2^31, up to 65535 rows.
  * workspace: 16-byte aligned, vrs_beam_select_workspace_size bytes; a call uses it
  * until its kernels end. */
 typedef struct {
@@ -594,7 +594,7 @@ int vrs_beam_select(vrs_ctx* ctx, const vrs_beam_desc* d, const void* logits, co
  * beam's slot alone.  Slots are numbered request * beams + beam.  Caches (rows of
  * keys), lengths (one row of 4 bytes) and tokens are such states alike.  Offsets are
  * in bytes; no two rows may overlap; fastest where all are multiples of 16.
- * beams <= 64. */
+ * beams <= 64, batch and layers <= 65535. */
 typedef struct {
   int32_t batch, beams, layers, rows;
   int64_t row_bytes, row_ld, slot_ld, layer_ld;
@@ -610,8 +610,9 @@ int vrs_beam_reorder(vrs_ctx* ctx, const vrs_reorder_desc* d, const int32_t* par
  * sees).  acc: float32, of key row r and key head g at acc[r * acc_ld + g * acc_hd];
  * sequences must not share key rows.  decay 0 does not read acc.
  * Scores, weights and sums are float32 and each sum has a fixed order.  head_dim,
- * alignment, strides and workspace as in vrs_attention, but that the heads of a key
- * head and 65 rows of q lie within 2^29 elements. */
+ * alignment, strides and workspace (for a few rows to a key head 4 bytes for each
+ * score, up to max_k of a row) as in vrs_attention, but that the heads of a key head
+ * and 65 rows of q lie within 2^29 elements. */
 typedef struct {
   int32_t q_rows, k_rows;
   int32_t heads, kv_heads, head_dim, dtype;   /* VRS_BF16 or VRS_F32 */

@@ -330,7 +330,18 @@ def scores_of(batch, beams, seed=0):
     return -torch.rand(batch, beams, generator=g, device="cuda").mul(5).cumsum(1)
 
 
-SELECT = [(1, 1, 1, 1), (1, 1, 5, 5), (2, 3, 7, 10), (1, 4, 2048, 4), (1, 4, 2049, 8), (3, 2, 8191, 64), (1, 1, 50001, 128),
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab,lo,hi", [(8192, 100, 1100), (8192, 8000, 8192), (20000, 5, 17), (3000, 2040, 2100), (60000, 0, 3000)])
+def test_beam_select_of_few_allowed_tokens(dtype, vocab, lo, hi):
+    """A run of tokens, the others at -infinity: waves with and without numbers, fewer than k in all."""
+    import torch
+    x = torch.full((2, 3, vocab), -math.inf, dtype=tdt(dtype), device="cuda")
+    x[..., lo:hi] = logits_of(2, 3, hi - lo, dtype, seed=lo)
+    for k in (1, 7, 64, 65, 128):
+        check_select(x, scores_of(2, 3), k)
+
+
+SELECT = [(1, 1, 255, 100), (2, 2, 849, 128), (1, 3, 300, 64), (1, 1, 1, 1), (1, 1, 5, 5), (2, 3, 7, 10), (1, 4, 2048, 4), (1, 4, 2049, 8), (3, 2, 8191, 64), (1, 1, 50001, 128),
           (2, 5, 30000, 10), (2, 64, 1000, 128), (1, 7, 8, 56), (64, 8, 9001, 16), (3, 1, 300, 1), (1, 2, 260000, 100), (33, 16, 8200, 32)]
 
 
@@ -906,3 +917,31 @@ def test_a_beam_search_over_an_evicted_prompt(dtype):
     reset()
     for got in replayed(step, states, reset):
         assert all(torch.equal(a, b0) for a, b0 in zip(got, after))
+
+
+def test_calls_on_two_streams_at_once():
+    """Each operator on two streams that are not the current one, with workspaces of their own: the bits of calls one
+    after another."""
+    import torch
+    b = build("group")
+    q, k, v, out = prefix_inputs(b, "bf16", 8, 2, 64)
+    x, s = logits_of(4, 8, 60000, "bf16", seed=2), scores_of(4, 8)
+    state0, parents = torch.randn(3, 32, 50, 64, device="cuda"), torch.randint(0, 8, (4, 8), device="cuda", dtype=torch.int32)
+    acc0 = torch.rand(2, b["k_rows"], device="cuda")
+    at, lens = i32(b["k_at"][:-1]), i32(b["k_len"])
+
+    def run(stream):
+        state, acc, kk, vv = state0.clone(), acc0.clone(), k.clone(), v.clone()
+        torch.cuda.synchronize()
+        got = [ctx().prefix_attention(q, k, v, b["seqs"], b["prefixes"], out=out.clone(), stream=stream),
+               *ctx().beam_select(x, s, 8, stream=stream), ctx().beam_reorder(state, parents, stream=stream),
+               ctx().attention_weights(q, k, b["seqs"], acc, stream=stream),
+               *ctx().cache_evict(kk, vv, acc0.clone(), at, lens, 2, stream=stream), kk, vv]
+        return got
+    want = run(None)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [run(t.cuda_stream) for t in streams]
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(bits(a), bits(c)) for a, c in zip(g, want))

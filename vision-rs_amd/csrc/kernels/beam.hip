@@ -106,51 +106,46 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   if (a.done && a.done[row]) return;           // such a beam goes on with the end token alone
   const int c0 = ch * a.chunk, n = min(a.chunk, a.vocab - c0);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.ld + c0;
-  u32x4_t raw[VT];
-  if (n == N * kT) {
+  // Vectors of a row that starts anywhere; in a short chunk an element a thread and turn, so that every wave has
+  // its share.
+  const bool whole = n == N * kT;
+  float v[N];
+  if (whole) {
+    u32x4_t raw[VT];
 #pragma unroll
-    for (int j = 0; j < VT; ++j) __builtin_memcpy(&raw[j], x + (j * kT + tid) * V, 16);      // rows start anywhere
-  } else {
-    constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;                    // -infinity
+    for (int j = 0; j < VT; ++j) __builtin_memcpy(&raw[j], x + (j * kT + tid) * V, 16);
 #pragma unroll
-    for (int j = 0; j < VT; ++j) {
-      const int e0 = (j * kT + tid) * V;
-      raw[j] = (u32x4_t){none, none, none, none};
-      if (e0 + V <= n) {
-        __builtin_memcpy(&raw[j], x + e0, 16);
-      } else if (e0 < n) {                     // the row ends in this vector
-        T last[V];
-        __builtin_memcpy(last, &raw[j], 16);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e0 + e < n) last[e] = x[e0 + e];
-        __builtin_memcpy(&raw[j], last, 16);
-      }
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i / 4][i % 4]);
+      else v[i] = __uint_as_float(i % 2 ? raw[i / 8][i % 8 / 2] & 0xffff0000u : raw[i / 8][i % 8 / 2] << 16);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Elt<T>::to_f(x[min(i * kT + tid, n - 1)]);      // (without branches: all on their way)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i * kT + tid < n ? v[i] : -INFINITY;
   }
   reinterpret_cast<u32x4_t*>(cand)[tid] = (u32x4_t){0, 0, 0, 0};    // the ranks below read whole eights
   reinterpret_cast<u32x4_t*>(cand)[kT + tid] = (u32x4_t){0, 0, 0, 0};
-  float v[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i / 4][i % 4]);
-    else v[i] = __uint_as_float(i % 2 ? raw[i / 8][i % 8 / 2] & 0xffff0000u : raw[i / 8][i % 8 / 2] << 16);
-  }
-  auto token = [&](int i) { return (uint32_t)(c0 + ((i / V) * kT + tid) * V + i % V); };
+  auto token = [&](int i) { return (uint32_t)(c0 + (whole ? ((i / V) * kT + tid) * V + i % V : i * kT + tid)); };
   float m = v[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);                   // (a NaN is passed over)
   if (!(m > -INFINITY)) m = -INFINITY;                              // (nothing else but NaN)
-  // what every wave has at least ceil(k / waves) numbers of, or one of them k (short chunks fill one wave only)
+  // what every wave has at least ceil(k / waves) numbers of
   const uint32_t top = m == -INFINITY ? 0 : order32(m);
   const uint32_t each = reached(top, (a.k + kWaves - 1) / kWaves);
-  const uint32_t alone = n < N * kT && a.k <= 64 ? reached(top, a.k) : 0;
   m = wave_max(m);
-  if (lane == 0) swm[wave] = m, sth[wave] = each, salone[wave] = alone;
+  if (lane == 0) swm[wave] = m, sth[wave] = each;
   __syncthreads();
   m = fmaxf(fmaxf(swm[0], swm[1]), fmaxf(swm[2], swm[3]));
   uint32_t T0 = min(min(sth[0], sth[1]), min(sth[2], sth[3]));
-  T0 = max(T0, max(max(salone[0], salone[1]), max(salone[2], salone[3])));
+  if (T0 == 0 && a.k <= 64) {                  // some wave has not so many (masked tokens): one that has k, if any
+    const uint32_t alone = reached(top, a.k);
+    if (lane == 0) salone[wave] = alone;
+    __syncthreads();
+    T0 = max(max(salone[0], salone[1]), max(salone[2], salone[3]));
+  }
   const float Tf = T0 ? __uint_as_float(T0 ^ ((int32_t)T0 < 0 ? 0x80000000u : 0xffffffffu)) : -3.40282347e38f;
   // candidates (none is -infinity or NaN), each wave's in its own part of the list
   int mine = 0;

@@ -190,7 +190,9 @@ __device__ __forceinline__ void stats_body(const vrs_weights_args& a) {
 __device__ __forceinline__ float2 joined(const vrs_weights_args& a, const Log2& u, int64_t id) {
   const int64_t step = (int64_t)a.s.q_rows * a.heads;
   float mx = kNone, l = 0.f;
+#pragma unroll 8
   for (int p = 0; p < a.parts; ++p) mx = fmaxf(mx, a.rl[p * step + id].x);
+#pragma unroll 8
   for (int p = 0; p < a.parts; ++p) {
     const float2 rl = a.rl[p * step + id];
     l += u.factor(rl.x, mx) * rl.y;
