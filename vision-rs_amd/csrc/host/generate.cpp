@@ -55,9 +55,9 @@ PrefixPlan plan_prefix(const vrs_attention_desc* d, const vrs_seqs* s, const vrs
   auto tiles = [&](int64_t count, int64_t rows) { return std::min(d->q_rows * group / 128 + count, count * up(rows * group, 128)); };
   const int64_t pre = (p.pre_few ? g * up(mr * group, 32) : tiles(g, mr)) * d->kv_heads;
   const int64_t own = (p.own_few ? n * up(mq * group, 32) : tiles(n, mq)) * d->kv_heads;
-  // parts of a prefix, all of one length but the last: 512 workgroups where there are 128 keys for each
-  const int64_t parts = std::clamp<int64_t>(std::min(up(512, pre), mp / 128), 1, 64);
-  p.part_len = (int)(up(up(mp, parts), 32) * 32);
+  // parts of a prefix, all of one length but the last: 512 workgroups as long as there are 128 keys for each
+  const int64_t parts = std::clamp<int64_t>(std::min(up(512, pre), up(mp, 128)), 1, 64);
+  p.part_len = (int)(up(up(mp, parts), p.pre_few ? 128 : 32) * (p.pre_few ? 128 : 32));     // (few rows: a tile to each wave)
   p.pre_parts = (int)up(mp, p.part_len);
   p.own_parts = (int)std::clamp<int64_t>(std::min(512 / own, mk / 192), 1, 16);
   p.finish = !p.own_few && p.own_parts == 1;
@@ -442,8 +442,11 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
   a.slices = std::min(std::max(a.slices, (int32_t)up(a.cols, 256)), a.cols);      // (a thread to a vector of a slice)
   const int64_t blocks = in_place ? 1 : std::clamp<int64_t>(want / a.slices, 1, std::max<int64_t>(1, d->budget / 32));
   if (pairs * a.slices >= (1ll << 32) / 1024) return fail(VRS_EBADSHAPE, "%s: grid too large", me);
-  if ((rc = launch(ctx, "vrs_evict_choose", dim3((unsigned)pairs), dim3(1024), 0, &a, stream))) return rc;
+  // the choice holds 16 keys of a thread in registers, and waits for fewer waves where 256 threads are enough
+  const int threads = (d->max_k > 0 ? d->max_k : d->k_rows / d->n) <= 4096 ? 256 : 1024;
   char name[64];
+  snprintf(name, sizeof name, "vrs_evict_choose_t%d", threads);
+  if ((rc = launch(ctx, name, dim3((unsigned)pairs), dim3(threads), 0, &a, stream))) return rc;
   snprintf(name, sizeof name, "vrs_evict_move_b%d", b);
   return launch(ctx, name, dim3((unsigned)(pairs * a.slices), 2, (unsigned)std::min<int64_t>(blocks, 65535)), dim3(256), 0, &a, stream);
 }

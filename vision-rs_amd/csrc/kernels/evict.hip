@@ -26,26 +26,35 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return x != x ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-// Sum over the 16 lanes of a row, and over the lanes up to each.
+// Sum over W lanes of a row of 16 whose lanes repeat after W, and over the lanes up to each of the first W.
+template <int W>
 __device__ __forceinline__ int row_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);      // row_ror 8, 4, 2, 1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true);
+  if constexpr (W == 16) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);    // row_ror 8, 4, 2, 1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true);
+  }
   x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true);
   return x + __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true);
 }
+template <int W>
 __device__ __forceinline__ int row_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8: 0 comes in
   x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  return x + __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  if constexpr (W == 16) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  }
+  return x;
 }
 
 // The choice.  The threshold is the largest T that at least m of the keys that
 // compete reach, found two bits at a time by counting (a wave counts 64 keys with
 // a comparison and a scalar popcount, and lane i of each wave reads wave i's
 // counts), until one is reached by m keys and no more.
-constexpr int kT = 1024, kHeld = 16, kW = kT / 64;       // threads; keys of a thread in registers; waves
+constexpr int kHeld = 16;                                // keys of a thread in registers
+template <int kT>                                        // threads: 256 or 1024
 __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
+  constexpr int kW = kT / 64;
   __shared__ __attribute__((aligned(16))) int cnt[2][kW][4];
   __shared__ int2 pre[2][kW];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -77,9 +86,9 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
       if (lane == 0) *reinterpret_cast<int4*>(cnt[turn][wave]) = make_int4(c1, c2, c3, 0);
       __syncthreads();
       const int4 w = *reinterpret_cast<const int4*>(cnt[turn][lane & (kW - 1)]);
-      c[0] = __builtin_amdgcn_readfirstlane(row_sum(w.x));
-      c[1] = __builtin_amdgcn_readfirstlane(row_sum(w.y));
-      c[2] = __builtin_amdgcn_readfirstlane(row_sum(w.z));
+      c[0] = __builtin_amdgcn_readfirstlane(row_sum<kW>(w.x));
+      c[1] = __builtin_amdgcn_readfirstlane(row_sum<kW>(w.y));
+      c[2] = __builtin_amdgcn_readfirstlane(row_sum<kW>(w.z));
       turn ^= 1;
     };
     int c[3];
@@ -133,7 +142,7 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
     asm volatile("" ::"v"(x));
     __syncthreads();                                           // also: the round's values are read
     const int2 c = pre[r & 1][lane & (kW - 1)];
-    const int ss = row_scan(c.x), es = row_scan(c.y);          // up to each wave
+    const int ss = row_scan<kW>(c.x), es = row_scan<kW>(c.y);          // up to each wave
     const uint64_t below = (1ull << lane) - 1;
     const int sb = sure0 + __builtin_amdgcn_readlane(ss, wave) - __builtin_popcountll(ms) + __builtin_popcountll(ms & below);
     const int eb = eq0 + __builtin_amdgcn_readlane(es, wave) - __builtin_popcountll(me) + __builtin_popcountll(me & below);
@@ -226,7 +235,8 @@ __device__ __forceinline__ void move_body(const vrs_evict_args& a) {
 }
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(1024) void vrs_evict_choose(vrs_evict_args a) { choose_body(a); }
+extern "C" __global__ __launch_bounds__(256) void vrs_evict_choose_t256(vrs_evict_args a) { choose_body<256>(a); }
+extern "C" __global__ __launch_bounds__(1024) void vrs_evict_choose_t1024(vrs_evict_args a) { choose_body<1024>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_evict_move_b16(vrs_evict_args a) { move_body<u32x4_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_evict_move_b4(vrs_evict_args a) { move_body<uint32_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_evict_move_b2(vrs_evict_args a) { move_body<uint16_t>(a); }
