@@ -55,8 +55,9 @@ PrefixPlan plan_prefix(const vrs_attention_desc* d, const vrs_seqs* s, const vrs
   auto tiles = [&](int64_t count, int64_t rows) { return std::min(d->q_rows * group / 128 + count, count * up(rows * group, 128)); };
   const int64_t pre = (p.pre_few ? g * up(mr * group, 32) : tiles(g, mr)) * d->kv_heads;
   const int64_t own = (p.own_few ? n * up(mq * group, 32) : tiles(n, mq)) * d->kv_heads;
-  // parts of a prefix, all of one length but the last: 512 workgroups as long as there are 128 keys for each
-  const int64_t parts = std::clamp<int64_t>(std::min(up(512, pre), up(mp, 128)), 1, 64);
+  // Parts of a prefix, all of one length but the last: 384 workgroups as long as there are 128 keys for each (64
+  // tokens on four prefixes of 1500 .. 6000 keys: 256 52.1 us, 384 51.4, 512 52.8, 768 53.3).
+  const int64_t parts = std::clamp<int64_t>(std::min(up(384, pre), up(mp, 128)), 1, 64);
   p.part_len = (int)(up(up(mp, parts), p.pre_few ? 128 : 32) * (p.pre_few ? 128 : 32));     // (few rows: a tile to each wave)
   p.pre_parts = (int)up(mp, p.part_len);
   p.own_parts = (int)std::clamp<int64_t>(std::min(512 / own, mk / 192), 1, 16);

@@ -43,8 +43,9 @@ __device__ __forceinline__ int parts_of(const vrs_prefix_args& p, int keys) {
   return min(p.pre_parts, max(1, (int)(((int64_t)keys + p.part_len - 1) / p.part_len)));
 }
 
-// One launch for prefixes (the first pre_blocks workgroups, whose keys are the most) and own keys, all parts going
-// to the workspace, or one for each, the second finishing what the first left there.
+// One launch for prefixes and own keys, all parts going to the workspace and to the join, or, where the own keys'
+// rows are many (their parts would be most of the traffic), one for each, the second finishing what the first left
+// (24 questions of 30 .. 200 tokens about 9000 keys: 505 + 33 us, 540 + 39 with the own keys in the first launch).
 template <typename F>
 __device__ __forceinline__ void job_of(const vrs_prefix_args& p, bool pre, int id, F place) {
   const vrs_attention_args& a = p.a;
@@ -107,12 +108,14 @@ __device__ __forceinline__ void few_kernel(const vrs_prefix_args& p) {
   const bool pre = (int)blockIdx.x < p.pre_blocks;
   few_job<T, D, false>(p, pre, blockIdx.x - (pre ? 0 : p.pre_blocks));
 }
-// Many rows to a prefix, few to a sequence: both kinds at once, the one bound by its instructions and the other by
-// memory.  64 tokens on four prefixes: see the figures at the top.
+// Many rows to a prefix, few to a sequence: both kinds in one launch, the few first, which are bound by memory and
+// unequal (64 tokens on four prefixes of 1500 .. 6000 keys, 20 .. 700 own, 32 heads on 8 of 128: 40 us, 42 with
+// the prefixes first, 28 + 18 in two launches; the join takes 7).
 template <typename T, int D>
 __device__ __forceinline__ void mixed_kernel(const vrs_prefix_args& p) {
-  if ((int)blockIdx.x >= p.pre_blocks) few_job<T, D, true>(p, false, blockIdx.x - p.pre_blocks);
-  else if (blockIdx.y == 0) prompt_job<T, D, true>(p, blockIdx.x);
+  const int own = gridDim.x - p.pre_blocks;
+  if ((int)blockIdx.x < own) few_job<T, D, true>(p, false, blockIdx.x);
+  else if (blockIdx.y == 0) prompt_job<T, D, true>(p, blockIdx.x - own);
 }
 
 // Joins the parts: a workgroup takes a row, a thread 4 elements of a head.
