@@ -8,9 +8,16 @@
 //
 // The k largest of a workgroup's numbers: the r-th largest of a wave's lane maxima,
 // r = k / waves, is reached by k numbers at least, and by few more where their order
-// is that of a vocabulary.  Those that reach it go to LDS and each counts how many
-// beat it, which is its place.  Where they are too many (equal or sorted logits) the
-// workgroup takes its maximum k times instead.
+// is that of a vocabulary (k 16: some 40 of 8192).  Those that reach it go to LDS and
+// each counts how many beat it, which is its place.  Where they are too many (equal
+// or sorted logits) the workgroup takes its maximum k times instead.
+//
+// 32 requests of 8 beams over 128000 tokens in bfloat16, a quarter of them at their
+// end (49 MB): 17 .. 18.6 us for the chunks, 2.8 TB/s, and 10.4 for the join.  46
+// registers, so that 8 workgroups share a CU: with the next chunk's loads ahead it is
+// 118 and 22 us.  Vector instructions take 45 % of the cycles (per logit: widening,
+// maximum, FMA, v_exp at four times an instruction's cycles, addition, two
+// comparisons), waits for the loads and two barriers the rest.
 #include "common.h"
 
 namespace {
@@ -453,7 +460,8 @@ __device__ __forceinline__ void join_body(const vrs_beam_args& a) {
 // ---------------------------------------------------------------------------
 // state[b][i] = old state[b][parent[b][i]] in place.  A thread takes one vector of a
 // row for all beams of a request: it reads those that others go on from, and then
-// writes them to where they go; no other thread touches that vector.
+// writes them to where they go; no other thread touches that vector.  16 requests of 8
+// beams, 60 .. 300 rows of 4 KiB in 16 layers, 1.5 GB: 300 .. 321 us, 4.8 .. 5.1 TB/s.
 template <typename V, int B>
 __device__ __forceinline__ void reorder_body(const vrs_reorder_args& a) {
   const int lane = threadIdx.x & 63, b = blockIdx.y;

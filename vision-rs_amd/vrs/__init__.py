@@ -10,7 +10,9 @@ Layer/op names mirror the reference crate: conv / conv_bn / dwconv /
 conv_plain (blocks/conv.rs), c3k2, c3k2_psa (blocks/c3k2.rs), c2psa and
 psa_attention (blocks/c2psa.rs), sppf (blocks/sppf.rs), detect
 (blocks/detect.rs), yolo26 (yolo26/mod.rs).  rms_norm, rope and attention are
-the operators around the products of a transformer layer.
+the operators around the products of a transformer layer; prefix_attention,
+beam_select, beam_reorder, attention_weights and cache_evict those of programs
+that generate from a cache.
 """
 from __future__ import annotations
 
