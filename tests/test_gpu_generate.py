@@ -185,6 +185,25 @@ def test_prefix_attention_values_that_are_not_finite(dtype, case):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_keys_at_their_queries_rows(dtype):
+    """Sequences without k_start and k_len: own keys lie at the queries' rows, prefixes behind them."""
+    import torch
+    for q_len, first, prefix in (([1, 1, 1], [0, 3], [50]), ([40, 130, 7], [0, 1, 3], [33, 200])):
+        starts = [2 + sum(q_len[:i]) for i in range(len(q_len) + 1)]
+        rows = starts[-1] + 3
+        p_at = [rows + 1 + sum(prefix[:i]) for i in range(len(prefix))]
+        b = dict(starts=starts, rows=rows, k_len=q_len, k_at=starts[:-1], p_at=p_at, prefix=prefix, k_rows=p_at[-1] + prefix[-1] + 2,
+                 group=[next(g for g in range(len(prefix)) if first[g] <= i < first[g + 1]) for i in range(len(q_len))])
+        seqs = vrs.seqs(i32(starts), max_q=max(q_len), max_k=max(q_len))
+        q, k, v, out = prefix_inputs(b, dtype, 4, 2, 64)
+        ref, tol = prefix_ref(b, q, k, v, True, 0.125, out, dtype)
+        inside(ctx().prefix_attention(q, k, v, seqs, vrs.prefixes(i32(first), i32(p_at), i32(prefix)), out=out), ref, tol)
+        acc = torch.rand(2, b["k_rows"], device="cuda")
+        ref, tol = weights_ref(q, k, acc, starts, q_len, starts[:-1], True, 0.125, 0.5)
+        inside(ctx().attention_weights(q, k, seqs, acc, decay=0.5), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_prefix_attention_scores_of_minus_infinity(dtype):
     """A query all of whose keys score -infinity is NaN, one that sees no key 0, and one run of such keys weighs nothing."""
     import torch
@@ -633,6 +652,15 @@ def test_attention_weights_hints_choose_kernels_only():
         for max_q, max_k in ((0, 0), (1, 1), (1, 0), (1, 10), (5, 4000), (1 << 30, 1 << 30), (64, 1)):
             s.max_q, s.max_k = max_q, max_k
             inside(ctx().attention_weights(q, k, s, acc.clone()), ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv", [(7, 1), (66, 1), (12, 4), (40, 8)])
+def test_attention_weights_groups_of_any_size(dtype, heads, kv):
+    """Row tiles that end inside a query, groups larger than a tile; parts of rows and of keys."""
+    check_weights(([130, 3, 40], [0, 500, 7]), dtype, heads, kv, 64, True)
+    check_weights(([33], [3000]), dtype, heads, kv, 72, True, seed=heads)
+    check_weights(([600, 500], [0, 0]), dtype, heads, kv, 32, False, seed=kv)
 
 
 def test_attention_weights_large_and_far_scores():
