@@ -636,7 +636,7 @@ int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seq
  * kept [n][kv_heads][budget] receives the places of the kept keys (-1 behind them),
  * len_out [n] (may be k_len; NULL: not stored) min(k_len, budget).  k_start, k_len,
  * out_start are DEVICE arrays; what they say outside the buffers is cut off.
- * Sequences must not share rows.  k_rows up to 2^31 - 1024, budget up to 2^31 - 2^20.
+ * Sequences must not share rows.  k_rows and budget up to 2^31 - 2^20.
  * k and v: any alignment of their elements, fastest at 16 bytes.  acc as in
  * vrs_attention_weights.  max_k: the most keys of a sequence, 0 if unknown (for speed
  * alone).  Keys keep the rotary positions that they have: give vrs_rope positions of

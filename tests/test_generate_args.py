@@ -150,7 +150,7 @@ def evict(ctx, at=FAKE, lens=2 * FAKE, o_start=None, k=3 * FAKE, v=4 * FAKE, acc
     (-2, dict(head_dim=5000)), (-1, dict(budget=0)), (-1, dict(first=-1)), (-1, dict(recent=-1)), (-1, dict(first=5, recent=4)),
     (-1, dict(max_k=-1)), (-2, dict(k_ld=-1)), (-2, dict(ko=7 * FAKE, ko_ld=32)), (-2, dict(ko=7 * FAKE, ko_hd=32)), (-2, dict(ko_ld=256)),
     (-2, dict(vo_hd=128, vo_ld=256)), (-2, dict(acco_hd=80)), (-2, dict(o_start=9 * FAKE)), (-2, dict(ao=8 * FAKE, acco_ld=0)),
-    (-1, dict(vo=3 * FAKE)), (-1, dict(ko=4 * FAKE)), (-1, dict(len_out=FAKE)), (-1, dict(len_out=6 * FAKE)), (-3, dict(k_rows=(1 << 31) - 512)), (-3, dict(budget=(1 << 31) - 1)),
+    (-1, dict(vo=3 * FAKE)), (-1, dict(ko=4 * FAKE)), (-1, dict(len_out=FAKE)), (-1, dict(len_out=6 * FAKE)), (-3, dict(k_rows=(1 << 31) - 512)), (-3, dict(k_rows=(1 << 31) - 2000)), (-3, dict(budget=(1 << 31) - 1)),
 ])
 def test_cache_evict_refuses(ctx, code, kw):
     rc, msg = evict(ctx, **kw)

@@ -401,7 +401,7 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
     if (s < 0 || s >> 40) return fail(VRS_EBADSHAPE, "%s: stride %lld", me, (long long)s);
   if (d->n == 0) return VRS_OK;
   // the kernels' numbers of keys and of kept places run on to the end of the tiles ahead
-  if (d->k_rows > 0x7fffffff - 1023 || d->budget > 0x7fffffff - (1 << 20))
+  if (std::max(d->k_rows, d->budget) > 0x7fffffff - (1 << 20))
     return fail(VRS_EUNSUPPORTED, "%s: %d key rows, a budget of %d", me, d->k_rows, d->budget);
   const size_t es = elt_size(d->dtype);
   if ((rc = check_ptr(k_start, 4, me, "k_start")) || (rc = check_ptr(k_len, 4, me, "k_len")) || (rc = check_ptr(kept, 4, me, "kept")) ||

@@ -55,11 +55,12 @@ __device__ __forceinline__ int row_scan(int x) {
 // a comparison and a scalar popcount, and lane i of each wave reads wave i's
 // counts), until one is reached by m keys and no more.
 constexpr int kHeld = 16;                                // keys of a thread in registers
+constexpr int kAtOnce = 4;                               // rounds of keys that are placed together
 template <int kT>                                        // threads: 256 or 1024
 __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
   constexpr int kW = kT / 64;
   __shared__ __attribute__((aligned(16))) int cnt[2][kW][4];
-  __shared__ int2 pre[2][kW];
+  __shared__ int2 pre[2][kAtOnce][kW];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int h = blockIdx.x % a.kv, seq = blockIdx.x / a.kv;
   const Keys s = keys_of(a, seq);
@@ -71,7 +72,9 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
   const int rounds = (n + kT - 1) / kT;
   const bool all = n <= a.budget;
   auto value = [&](int i) { return acc[(int64_t)i * a.acc_ld]; };
-  float next = tid < n ? value(tid) : 0.f;
+  float next[kAtOnce];
+#pragma unroll
+  for (int r = 0; r < kAtOnce; ++r) next[r] = r * kT + tid < n ? value(r * kT + tid) : 0.f;
   const int m = all ? 0 : keep - first - (n - last);           // of those that compete
   uint32_t T = 0;
   int above = 0;                                               // keys above T
@@ -131,31 +134,44 @@ __device__ __forceinline__ void choose_body(const vrs_evict_args& a) {
     }
   }
   const int equal = sharp ? 0 : m - above;                     // the earliest of those equal to T stay too
-  // places in order: those that stay anyway and those equal to T before each
+  // places in order: those that stay anyway and those equal to T before each, kAtOnce rounds to a barrier
   int sure0 = 0, eq0 = 0;
-  for (int r = 0; r < rounds; ++r) {
-    const int i = r * kT + tid;
-    const float x = next;
-    if (i + kT < n) next = value(i + kT);                      // (lies behind all that is written before)
-    const uint32_t o = order_of(x);
-    const bool in = i < n, competes = i >= first && i < last;
-    const bool sure = in && (all || !competes || o > T), eq = competes && equal > 0 && o == T;
-    const uint64_t ms = __ballot(sure), me = __ballot(eq);
-    if (lane == 0) pre[r & 1][wave] = make_int2(__builtin_popcountll(ms), __builtin_popcountll(me));
-    asm volatile("" ::"v"(x));
-    __syncthreads();                                           // also: the round's values are read
-    const int2 c = pre[r & 1][lane & (kW - 1)];
-    const int ss = row_scan<kW>(c.x), es = row_scan<kW>(c.y);          // up to each wave
-    const uint64_t below = (1ull << lane) - 1;
-    const int sb = sure0 + __builtin_amdgcn_readlane(ss, wave) - __builtin_popcountll(ms) + __builtin_popcountll(ms & below);
-    const int eb = eq0 + __builtin_amdgcn_readlane(es, wave) - __builtin_popcountll(me) + __builtin_popcountll(me & below);
-    sure0 += __builtin_amdgcn_readlane(ss, kW - 1);
-    eq0 += __builtin_amdgcn_readlane(es, kW - 1);
-    if (sure || (eq && eb < equal)) {
-      const int to = sb + min(eb, equal);
-      if (to < keep) {
-        kept[to] = i;
-        if (s.o0 >= 0 && s.o0 + to < a.o_rows) acco[(int64_t)to * a.acco_ld] = x;
+  for (int r0 = 0, turn = 0; r0 < rounds; r0 += kAtOnce, turn ^= 1) {
+    float x[kAtOnce];
+    uint64_t ms[kAtOnce], me[kAtOnce];
+#pragma unroll
+    for (int r = 0; r < kAtOnce; ++r) x[r] = next[r];
+#pragma unroll
+    for (int r = 0; r < kAtOnce; ++r) {
+      const int i = (r0 + kAtOnce + r) * kT + tid;
+      if (i < n) next[r] = value(i);                           // (lies behind all that is written before)
+    }
+#pragma unroll
+    for (int r = 0; r < kAtOnce; ++r) {
+      const int i = (r0 + r) * kT + tid;
+      const uint32_t o = order_of(x[r]);
+      const bool competes = i >= first && i < last;
+      ms[r] = __ballot(i < n && (all || !competes || o > T));
+      me[r] = __ballot(competes && equal > 0 && o == T);
+      if (lane == 0) pre[turn][r][wave] = make_int2(__builtin_popcountll(ms[r]), __builtin_popcountll(me[r]));
+      asm volatile("" ::"v"(x[r]));
+    }
+    __syncthreads();                                           // also: the rounds' values are read
+    const int2 c = pre[turn][lane >> 4][lane & (kW - 1)];      // a row of 16 lanes for each round
+    const int ss = row_scan<kW>(c.x), es = row_scan<kW>(c.y);  // up to each wave
+    const uint64_t bit = 1ull << lane;
+#pragma unroll
+    for (int r = 0; r < kAtOnce; ++r) {
+      const int sb = sure0 + __builtin_amdgcn_readlane(ss, 16 * r + wave) - __builtin_popcountll(ms[r]) + __builtin_popcountll(ms[r] & (bit - 1));
+      const int eb = eq0 + __builtin_amdgcn_readlane(es, 16 * r + wave) - __builtin_popcountll(me[r]) + __builtin_popcountll(me[r] & (bit - 1));
+      sure0 += __builtin_amdgcn_readlane(ss, 16 * r + kW - 1);
+      eq0 += __builtin_amdgcn_readlane(es, 16 * r + kW - 1);
+      if ((ms[r] & bit) || ((me[r] & bit) && eb < equal)) {
+        const int to = sb + min(eb, equal);
+        if (to < keep) {
+          kept[to] = (r0 + r) * kT + tid;
+          if (s.o0 >= 0 && s.o0 + to < a.o_rows) acco[(int64_t)to * a.acco_ld] = x[r];
+        }
       }
     }
   }
