@@ -4,7 +4,7 @@
 //
 // Two launches: the choice (a workgroup for each sequence and key head), then the
 // move of K and V along the list of kept places.  16 caches of 2500 .. 8000 keys, 8
-// heads of 128 in bfloat16, cut to 2048 where they lie (274 MB): 25 us, bound by the
+// heads of 128 in bfloat16, cut to 2048 where they lie (274 MB): 23 us, bound by the
 // rounds of counting in 128 workgroups, and 54, 4.9 TB/s (75 without the next tile's
 // rows on their way; slices of 64 bytes of a row, half a cache line, 90).
 #include "common.h"
