@@ -430,6 +430,30 @@ def test_beam_select_of_masks_at_the_end_of_the_range(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("far", [1e5, 2e6, 1e8, 1e9, 4e9, 1e10, 1e11, 1e20, 9e29])
+@pytest.mark.parametrize("batch,beams,vocab", [(2, 3, 5000), (75, 4, 17000)])
+def test_beam_select_of_masks_far_from_zero(dtype, far, batch, beams, vocab):
+    """Chunks of nothing but tokens masked by a large negative number, beams of nothing else, tokens forced by a large
+    positive one: the sums' terms are in range wherever the chunk's largest logit lies."""
+    import torch
+    x, s = logits_of(batch, beams, vocab, dtype, seed=11), scores_of(batch, beams, seed=12)
+    x[0, 0, vocab // 3:] = -far                  # whole chunks beside ordinary logits
+    x[0, 1] = -far                               # nothing else
+    x[0, 2, 9:] = -far
+    x[1, 0, vocab - 5] = far                     # forced: the only one of its beam that counts
+    x[1, 1] = far
+    x[1, 2, ::2] = -far
+    for k in (1, 8, 128):
+        ref = select_ref(x, s, k)
+        got = ctx().beam_select(x, s, k)
+        torch.cuda.synchronize()
+        assert torch.equal(got[1].cpu(), ref[1]) and torch.equal(got[2].cpu(), ref[2])
+        # as check_select, and lse in 64 bits on either side: two roundings here and one there, each by 2^-53 of it
+        lse = torch.logsumexp(x.double().cpu(), 2).abs().gather(1, ref[1].long())
+        inside(got[0].cpu(), ref[0], ref[0].abs().nan_to_num(0, 0, 0) * F * 1.01 + 34 * F * 4 + lse * 2.0 ** -51)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_beam_select_of_beams_with_like_scores(dtype):
     """Many beams and chunks of which any may hold the best: far more entries reach the first threshold than are kept."""
     import torch

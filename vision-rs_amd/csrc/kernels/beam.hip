@@ -95,8 +95,12 @@ __device__ __forceinline__ void best_of(uint64_t& o, uint32_t& at, uint64_t (&so
 // ---------------------------------------------------------------------------
 // A chunk of one row: VT vectors of 16 bytes to a thread.  The sum is of 2^(x L - R), L = log2 e rounded to float32
 // and R = m L rounded, one FMA and one v_exp to a logit, and lse = (R + log2 sum) / L, so that R's rounding falls out
-// and L's (1.3e-8) counts times the entropy only.  A NaN or +infinity makes the sum NaN.
+// and L's (1.3e-8) counts times the entropy only.  R is off by up to 2^-24 of itself, which the largest logit's term
+// has in its exponent (a chunk masked by -1e10 would leave the range of 2^x): from |m| = 2^20 on the terms are
+// 2^((x - m) L), of a difference that is exact where it counts, and R = m L in 64 bits.  A NaN or +infinity makes the
+// sum NaN.
 constexpr float kL = 1.44269502f;
+constexpr float kNear = 1048576.f;
 template <typename T, int VT>
 __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   constexpr int V = 16 / (int)sizeof(T), N = VT * V;
@@ -167,12 +171,13 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   }
   if (lane == 0) count[wave] = mine;
   const float ref = m == -INFINITY ? 0.f : m;
+  const bool near = fabsf(ref) < kNear;
   float sum = 0.f;
-  if (fabsf(ref) < 1e30f) {
+  if (near) {
     const float R = ref * kL;
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[i], kL, -R));
-  } else {                                     // where masks lie at the ends of the range
+  } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * kL);
   }
@@ -181,7 +186,7 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   __syncthreads();
   const int64_t at = (int64_t)row * a.chunks + ch;
   if (tid == 0)
-    a.part[at] = make_double2(fabsf(ref) < 1e30f && m > -INFINITY ? (double)(ref * kL) : (double)m * kL, sws[0] + sws[1] + sws[2] + sws[3]);
+    a.part[at] = make_double2(near && m > -INFINITY ? (double)(ref * kL) : (double)m * kL, sws[0] + sws[1] + sws[2] + sws[3]);
   uint2* list = a.list + at * a.k;
   int have = 0, most = 0;
 #pragma unroll
