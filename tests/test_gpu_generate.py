@@ -997,3 +997,37 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(bits(a), bits(c)) for a, c in zip(g, want))
+
+
+def test_calls_that_overlap_on_two_streams():
+    """Two streams that run the operators at once, each in another order and with inputs and workspaces of its own: the
+    bits of calls one after another.  All inputs are there before the first call, and nothing waits until the last."""
+    import torch
+    b = build(([1] * 48, [200 + i for i in range(48)], [0, 24, 48], [3000, 1700]))
+    q, k, v, out = prefix_inputs(b, "bf16", 32, 8, 128)
+    x, s = logits_of(8, 8, 60000, "bf16", seed=2), scores_of(8, 8)
+    state0, parents = torch.randn(6, 64, 50, 128, device="cuda"), torch.randint(0, 8, (8, 8), device="cuda", dtype=torch.int32)
+    acc0 = torch.rand(8, b["k_rows"], device="cuda")
+    at, lens = i32(b["k_at"][:-1]), i32(b["k_len"])
+
+    def jobs(stream):
+        state, acc, kk, vv, aa, o = state0.clone(), acc0.clone(), k.clone(), v.clone(), acc0.clone(), out.clone()
+        c = ctx()
+        return [lambda: [c.prefix_attention(q, k, v, b["seqs"], b["prefixes"], out=o, stream=stream)],
+                lambda: [*c.beam_select(x, s, 8, stream=stream)],
+                lambda: [c.beam_reorder(state, parents, stream=stream)],
+                lambda: [c.attention_weights(q, k, b["seqs"], acc, stream=stream)],
+                lambda: [*c.cache_evict(kk, vv, aa, at, lens, 150, first=4, recent=20, stream=stream), kk, vv, aa]]
+    want = [call() for call in jobs(None)]
+    streams, turns = [torch.cuda.Stream() for _ in range(2)], 5
+    calls = [[jobs(t.cuda_stream) for t in streams] for _ in range(turns)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in calls:
+        for i in range(len(want)):
+            for j, mine in enumerate(turn):
+                n = (i + 2 * j) % len(want)
+                got.append((n, mine[n]()))
+    torch.cuda.synchronize()
+    for n, outs in got:
+        assert all(torch.equal(bits(a), bits(c)) for a, c in zip(outs, want[n])), n
