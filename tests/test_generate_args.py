@@ -161,6 +161,14 @@ def test_cache_evict_of_nothing_is_nothing(ctx):
     assert evict(ctx, n=0, at=None, k=None, kept=None)[0] == 0
 
 
+def test_cache_evict_addresses_of_empty_buffers_are_of_no_account(ctx):
+    """Neither their alignment nor their strides choose a kernel; the calls end at the grid's limit, before a launch."""
+    for kw in (dict(k_rows=0, k=3 * FAKE + 2, ko=7 * FAKE, vo=8 * FAKE, ao=9 * FAKE), dict(k_rows=0, v=4 * FAKE + 1, ko=7 * FAKE, vo=8 * FAKE, ao=9 * FAKE),
+               dict(out_rows=0, ko=7 * FAKE + 2, vo=8 * FAKE, ao=9 * FAKE), dict(k_rows=0, out_rows=0, k=FAKE + 1, ko=FAKE + 1)):
+        rc, msg = evict(ctx, dtype=vrs.F32, n=1 << 21, **kw)
+        assert rc == -2 and "grid too large" in msg, (rc, msg, kw)
+
+
 # ---- the binding ---------------------------------------------------------------------------------
 
 

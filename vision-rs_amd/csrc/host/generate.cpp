@@ -427,10 +427,10 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
 
   auto fits = [&](int64_t bytes) {
     const int64_t n = bytes / (int64_t)es;
-    bool ok = d->head_dim % n == 0;
-    for (const void* p : {k, v, (const void*)k_out, (const void*)v_out}) ok = ok && aligned(p, bytes);
-    for (int64_t s : {d->k_ld, d->k_hd, d->v_ld, d->v_hd, d->ko_ld, d->ko_hd, d->vo_ld, d->vo_hd}) ok = ok && s % n == 0;
-    return ok;
+    auto of = [&](const void* p, int64_t ld, int64_t hd) { return aligned(p, bytes) && ld % n == 0 && hd % n == 0; };
+    // (an empty buffer may have any address)
+    return d->head_dim % n == 0 && (d->k_rows == 0 || (of(k, d->k_ld, d->k_hd) && of(v, d->v_ld, d->v_hd))) &&
+           (d->out_rows == 0 || (of(k_out, d->ko_ld, d->ko_hd) && of(v_out, d->vo_ld, d->vo_hd)));
   };
   const int b = fits(16) ? 16 : fits(4) ? 4 : 2;
   const int64_t per = b / (int64_t)es;
