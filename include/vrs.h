@@ -572,7 +572,8 @@ int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_se
  * +infinity, or nothing else than -infinity.
  * logits: rows (beams of all requests, one after another) of contiguous elements,
  * ld elements apart, of any alignment of their elements.  k <= 128 and
- * <= beams * vocab, beams <= 64, beams * vocab < 2^31, up to 65535 rows.
+ * <= beams * vocab, beams <= 64, beams * vocab < 2^31, up to 65535 rows.  The outputs
+ * are arrays of their own.
  * workspace: 16-byte aligned, vrs_beam_select_workspace_size bytes; a call uses it
  * until its kernels end. */
 typedef struct {
@@ -593,7 +594,8 @@ int vrs_beam_select(vrs_ctx* ctx, const vrs_beam_desc* d, const void* logits, co
  * of a receiving slot stay as they were.  A parent outside 0 .. beams - 1 leaves its
  * beam's slot alone.  Slots are numbered request * beams + beam.  Caches (rows of
  * keys), lengths (one row of 4 bytes) and tokens are such states alike.  Offsets are
- * in bytes; no two rows may overlap; fastest where all are multiples of 16.
+ * in bytes; no two rows may overlap; fastest where all are multiples of 16.  parents
+ * and len lie outside the state.
  * beams <= 64, batch and layers <= 65535. */
 typedef struct {
   int32_t batch, beams, layers, rows;
@@ -636,7 +638,8 @@ int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seq
  * kept [n][kv_heads][budget] receives the places of the kept keys (-1 behind them),
  * len_out [n] (may be k_len; NULL: not stored) min(k_len, budget).  k_start, k_len,
  * out_start are DEVICE arrays; what they say outside the buffers is cut off.
- * Sequences must not share rows.  k_rows and budget up to 2^31 - 2^20.
+ * Sequences must not share rows; kept, len_out and acc_out are arrays of their own
+ * otherwise.  k_rows and budget up to 2^31 - 2^20.
  * k and v: any alignment of their elements, fastest at 16 bytes.  acc as in
  * vrs_attention_weights.  max_k: the most keys of a sequence, 0 if unknown (for speed
  * alone).  Keys keep the rotary positions that they have: give vrs_rope positions of

@@ -169,6 +169,28 @@ def test_cache_evict_addresses_of_empty_buffers_are_of_no_account(ctx):
         assert rc == -2 and "grid too large" in msg, (rc, msg, kw)
 
 
+def test_outputs_that_are_other_arrays_are_refused(ctx):
+    """The kernels read what they would write: starts of keys, parents, lengths, logits."""
+    for kw in (dict(outs=(3 * FAKE, FAKE, 5 * FAKE)), dict(outs=(3 * FAKE, 4 * FAKE, FAKE)), dict(outs=(3 * FAKE, 2 * FAKE, 5 * FAKE)),
+               dict(outs=(3 * FAKE, 4 * FAKE, 2 * FAKE)), dict(done=5 * FAKE), dict(done=4 * FAKE), dict(done=3 * FAKE)):
+        rc, msg = select(ctx, **kw)
+        assert rc == -1 and "vrs_beam_select: an output" in msg, (rc, msg, kw)
+    for kw in (dict(parents=2 * FAKE), dict(lens=2 * FAKE)):
+        rc, msg = reorder(ctx, **kw)
+        assert rc == -1 and "vrs_beam_reorder: the state" in msg, (rc, msg, kw)
+    for kept in (FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, 5 * FAKE, 9 * FAKE):
+        for kw in ({}, dict(o_start=9 * FAKE, ko=7 * FAKE, vo=8 * FAKE, ao=10 * FAKE)):
+            if kept != 9 * FAKE or kw:
+                rc, msg = evict(ctx, kept=kept, **kw)
+                assert rc == -1 and "vrs_cache_evict: kept is" in msg, (rc, msg, kept, kw)
+    for len_out in (3 * FAKE, 5 * FAKE, 7 * FAKE):
+        rc, msg = evict(ctx, len_out=len_out, ko=7 * FAKE, vo=8 * FAKE, ao=10 * FAKE)
+        assert rc == -1 and "vrs_cache_evict: len_out is" in msg, (rc, msg, len_out)
+    for kw in (dict(ao=3 * FAKE), dict(ao=4 * FAKE), dict(ko=7 * FAKE, ao=7 * FAKE), dict(ko=5 * FAKE, ao=7 * FAKE)):
+        rc, msg = evict(ctx, **kw)
+        assert rc == -1 and "vrs_cache_evict: acc is" in msg, (rc, msg, kw)
+
+
 # ---- the binding ---------------------------------------------------------------------------------
 
 

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "layers.h"
 
@@ -14,6 +15,11 @@ using namespace vrs;
 namespace {
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether p, if not null, is one of the others.
+bool one_of(const void* p, std::initializer_list<const void*> others) {
+  return p && std::find(others.begin(), others.end(), p) != others.end();
+}
 
 int check_workspace(const void* ws, size_t have, size_t need, const char* me) {
   if (!need) return VRS_OK;
@@ -208,8 +214,8 @@ int vrs_beam_select(vrs_ctx* ctx, const vrs_beam_desc* d, const void* logits, co
       (rc = check_ptr(out_scores, 4, me, "out_scores")) || (rc = check_ptr(out_parents, 4, me, "out_parents")) ||
       (rc = check_ptr(out_tokens, 4, me, "out_tokens")))
     return rc;
-  if (out_scores == scores || (const void*)out_scores == logits || (void*)out_parents == (void*)out_tokens ||
-      (void*)out_scores == (void*)out_parents || (void*)out_scores == (void*)out_tokens)
+  if (one_of(out_scores, {logits, scores, done, out_parents, out_tokens}) || one_of(out_parents, {logits, scores, done, out_tokens}) ||
+      one_of(out_tokens, {logits, scores, done}))
     return fail(VRS_EINVAL, "%s: an output is another buffer", me);
   const BeamPlan p = plan_beam(d);
   if ((rc = check_workspace(workspace, workspace_bytes, beam_bytes(d, p), me))) return rc;
@@ -244,6 +250,7 @@ int vrs_beam_reorder(vrs_ctx* ctx, const vrs_reorder_desc* d, const int32_t* par
   if ((rc = check_ptr(parents, 4, me, "parents")) || (len && (rc = check_ptr(len, 4, me, "len"))) ||
       (rc = check_ptr(state, 1, me, "state")))
     return rc;
+  if (one_of(state, {parents, len})) return fail(VRS_EINVAL, "%s: the state is parents or len", me);
   if (!rows_apart(d->row_bytes, {d->rows, (int64_t)d->batch * d->beams, d->layers}, {d->row_ld, d->slot_ld, d->layer_ld}))
     return fail(VRS_EBADSHAPE, "%s: strides fold rows onto each other", me);
   if (d->batch > 65535 || d->layers > 65535) return fail(VRS_EUNSUPPORTED, "%s: %d requests, %d layers (up to 65535)", me, d->batch, d->layers);
@@ -423,7 +430,12 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
   };
   if (folds(d->ko_ld, d->ko_hd, d->head_dim) || folds(d->vo_ld, d->vo_hd, d->head_dim) || folds(d->acco_ld, d->acco_hd, 1))
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
-  if (len_out && (len_out == k_start || len_out == out_start || len_out == kept)) return fail(VRS_EINVAL, "%s: len_out is another array", me);
+  const void *k_in = d->k_rows ? k : nullptr, *v_in = d->k_rows ? v : nullptr, *acc_in = d->k_rows ? acc : nullptr;
+  const void *k_to = d->out_rows ? k_out : nullptr, *v_to = d->out_rows ? v_out : nullptr, *acc_to = d->out_rows ? acc_out : nullptr;
+  if (one_of(len_out, {k_start, out_start, kept, k_in, v_in, acc_in, k_to, v_to, acc_to}))
+    return fail(VRS_EINVAL, "%s: len_out is another array", me);
+  if (one_of(kept, {k_start, k_len, out_start, k_in, v_in, acc_in, k_to, v_to, acc_to})) return fail(VRS_EINVAL, "%s: kept is another array", me);
+  if (one_of(acc_to, {k_in, v_in, k_to, v_to}) || one_of(acc_in, {k_to, v_to})) return fail(VRS_EINVAL, "%s: acc is another buffer", me);
 
   auto fits = [&](int64_t bytes) {
     const int64_t n = bytes / (int64_t)es;
