@@ -432,9 +432,9 @@ int vrs_cache_evict(vrs_ctx* ctx, const vrs_evict_desc* d, const int32_t* k_star
     return fail(VRS_EBADSHAPE, "%s: output strides fold rows or heads onto each other", me);
   const void *k_in = d->k_rows ? k : nullptr, *v_in = d->k_rows ? v : nullptr, *acc_in = d->k_rows ? acc : nullptr;
   const void *k_to = d->out_rows ? k_out : nullptr, *v_to = d->out_rows ? v_out : nullptr, *acc_to = d->out_rows ? acc_out : nullptr;
+  if (one_of(kept, {k_start, k_len, out_start, k_in, v_in, acc_in, k_to, v_to, acc_to})) return fail(VRS_EINVAL, "%s: kept is another array", me);
   if (one_of(len_out, {k_start, out_start, kept, k_in, v_in, acc_in, k_to, v_to, acc_to}))
     return fail(VRS_EINVAL, "%s: len_out is another array", me);
-  if (one_of(kept, {k_start, k_len, out_start, k_in, v_in, acc_in, k_to, v_to, acc_to})) return fail(VRS_EINVAL, "%s: kept is another array", me);
   if (one_of(acc_to, {k_in, v_in, k_to, v_to}) || one_of(acc_in, {k_to, v_to})) return fail(VRS_EINVAL, "%s: acc is another buffer", me);
 
   auto fits = [&](int64_t bytes) {
