@@ -249,7 +249,7 @@ __device__ __forceinline__ void sum_body(const vrs_weights_args& a) {
             sum[t] += key + t * 256 < __float_as_int(c[3]) ? p : 0.f;
           }
         }
-      } else {
+      } else {      // more keys than were counted on: a key tile has all its scores or none (s_ld is whole tiles)
         for (int i = 0; i < n; ++i) {
           const int j = (r0 + i) / G_, h = hk * G_ + (r0 + i - j * G_);
           const int64_t row = (int64_t)sp.q0 + j;
@@ -257,14 +257,10 @@ __device__ __forceinline__ void sum_body(const vrs_weights_args& a) {
           for (int t = 0; t < KT; ++t) {
             const int64_t at = key + t * 256;
             if (at >= __float_as_int(c[3])) break;
+            const T* q = static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd;
+            const T* k = kp + at * a.k_ld;
             float x = 0.f;
-            if (at < a.s_ld) {
-              x = a.scores[(row * a.heads + h) * a.s_ld + at];
-            } else {                         // more keys than were counted on
-              const T* q = static_cast<const T*>(a.q) + row * a.q_ld + h * a.q_hd;
-              const T* k = kp + at * a.k_ld;
-              for (int d = 0; d < a.dim; ++d) x = __builtin_fmaf(Elt<T>::to_f(q[d]), Elt<T>::to_f(k[d]), x);
-            }
+            for (int d = 0; d < a.dim; ++d) x = __builtin_fmaf(Elt<T>::to_f(q[d]), Elt<T>::to_f(k[d]), x);
             sum[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[2], -c[0])) * c[1];
           }
         }
