@@ -718,6 +718,32 @@ def test_attention_weights_strides_workspace_and_graph():
             assert torch.equal(got.t()[1:], want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_weights_of_rows_whose_keys_are_in_parts(dtype):
+    """A workspace full of NaN, rows of no sequence, replays that follow the lengths."""
+    import torch
+    case = ([40, 0, 70, 1], [3000, 9, 500, 200])
+    starts, rows, k_len, k_at, s = weights_case(case)
+    q, k = randn(rows, 4, 64, dtype=dtype, seed=1, scale=2), randn(k_at[-1] + 4, 2, 64, dtype=dtype, seed=2)
+    acc0 = torch.rand(2, k_at[-1] + 4, device="cuda")
+    d = vrs._WEIGHTS(rows, k.shape[0], 4, 2, 64, vrs.F32 if dtype == "f32" else vrs.BF16, 1, 0.0, 0.5, 256, 64, 128, 64, 1, k.shape[0])
+    ws = torch.full((vrs.lib().vrs_attention_weights_workspace_size(d, s.address) // 4,), math.nan, device="cuda").view(torch.uint8)
+    assert ws.numel() >= 2 * 8 * rows * 4                   # two parts at least
+    acc = acc0.clone()
+    call = lambda: ctx().attention_weights(q, k, s, acc, decay=0.5, workspace=ws)   # noqa: E731
+    ref, tol = weights_ref(q, k, acc0, starts, k_len, k_at, True, 0.125, 0.5)
+    call()
+    inside(acc, ref, tol)
+    want = acc.clone()
+    for (got,) in replayed(call, [acc], lambda: acc.copy_(acc0)):
+        assert torch.equal(got, want)
+    k_len[0] = 41                                           # the captured call would see these
+    s.tensors[2].copy_(i32(k_len))
+    ref, tol = weights_ref(q, k, acc0, starts, k_len, k_at, True, 0.125, 0.5)
+    for (got,) in replayed(call, [acc], lambda: acc.copy_(acc0)):
+        inside(got, ref, tol)
+
+
 def test_attention_weights_writes_no_key_outside():
     import torch
     buf = torch.full((1, 60), 7.0, device="cuda")

@@ -380,6 +380,10 @@ int vrs_attention_weights(vrs_ctx* ctx, const vrs_weights_desc* d, const vrs_seq
     const unsigned y = p.few ? (unsigned)std::min<int64_t>(p.row_tiles, 65535) : 1;
     rc = launch(ctx, name, dim3((unsigned)first, y), dim3(256), 0, &a, stream);
     if (rc) return rc;
+    // (q_rows * heads < 2^31, as the first launch's grid has it)
+    if (!p.few && p.parts > 1 &&
+        (rc = launch(ctx, "vrs_weights_rows", dim3((unsigned)up((int64_t)d->q_rows * d->heads, 256)), dim3(256), 0, &a, stream)))
+      return rc;
   }
   if (p.few) snprintf(name, sizeof name, "vrs_weights_sum_%s", dsuffix(d->dtype));
   else snprintf(name, sizeof name, "vrs_weights_keys_%s_d%d", dsuffix(d->dtype), D);

@@ -203,6 +203,16 @@ __device__ __forceinline__ float2 joined(const vrs_weights_args& a, const Log2& 
   return make_float2(mx, l);
 }
 
+// Between the stages, many rows whose keys are in parts: a thread joins a row's parts and leaves them as the first.
+// In stage 2 each tile of keys would do so again, with registers that its products need: 100 queries over 4000 keys,
+// 32 heads on 8 of 128, 16 parts: 60 us a call, 35 with this launch; a prompt of 4096, whose rows have one part: 14
+// registers of stage 2 spilled and 112 us, 2 and 100.
+__device__ __forceinline__ void rows_body(const vrs_weights_args& a) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (int64_t)a.s.q_rows * a.heads) return;
+  a.rl[id] = joined(a, Log2(a.c), id);
+}
+
 // Stage 2 from the scores: a thread takes 4 keys, 256 apart, and passes over the rows.
 // 64 tokens over 500 .. 8000 keys: 20 us (one key a thread: 37).
 template <typename T>
@@ -273,11 +283,11 @@ __device__ __forceinline__ void sum_body(const vrs_weights_args& a) {
 }
 
 // Stage 2 with the products again: a workgroup of 4 waves holds 128 keys, and a part
-// of the rows that see them passes by in tiles of 64.  The same prompt: 105 .. 112 us.
-// Rows straight from memory to each wave: 919 us; their offsets by 64-bit arithmetic
-// on vector registers, which makes the loads' buffer descriptors vectors too and puts
-// a loop around each load: 130.  Three waves to a SIMD (168 registers): two 123, four
-// 216 (they spill).
+// of the rows that see them passes by in tiles of 64.  The same prompt: 100 .. 113 us
+// (cards and their clocks differ).  Rows straight from memory to each wave: 919 us;
+// their offsets by 64-bit arithmetic on vector registers, which makes the loads'
+// buffer descriptors vectors too and puts a loop around each load: 130.  Three waves
+// to a SIMD (168 registers, 2 more spilled): two 125, four 178 (37 spilled).
 template <typename T, int D>
 __device__ __forceinline__ void keys_body(const vrs_weights_args& a) {
   using E = Elt<T>;
@@ -347,7 +357,7 @@ __device__ __forceinline__ void keys_body(const vrs_weights_args& a) {
         if ((int)threadIdx.x < here) {
           lim = visible(sp, j0 + sj, a.causal);
           const int64_t id = ((int64_t)sp.q0 + j0 + sj) * a.heads + hk * group + sh;
-          rl = a.parts == 1 ? a.rl[id] : joined(a, u, id);
+          rl = a.rl[id];                     // (of all parts: see rows_body)
         }
       }
       ++at;
@@ -458,4 +468,5 @@ VRS_WEIGHTS(f32, float, 64, 2)
 VRS_WEIGHTS(f32, float, 128, 1)
 extern "C" __global__ __launch_bounds__(256) void vrs_weights_sum_bf16(vrs_weights_args a) { sum_body<bf16_t>(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_weights_sum_f32(vrs_weights_args a) { sum_body<float>(a); }
+extern "C" __global__ __launch_bounds__(256) void vrs_weights_rows(vrs_weights_args a) { rows_body(a); }
 extern "C" __global__ __launch_bounds__(256) void vrs_weights_join(vrs_weights_args a) { join_body(a); }
