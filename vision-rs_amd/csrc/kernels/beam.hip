@@ -13,11 +13,13 @@
 // or sorted logits) the workgroup takes its maximum k times instead.
 //
 // 32 requests of 8 beams over 128000 tokens in bfloat16, a quarter of them at their
-// end (49 MB): 17 .. 18.6 us for the chunks, 2.8 TB/s, and 10.4 for the join.  46
-// registers, so that 8 workgroups share a CU: with the next chunk's loads ahead it is
-// 118 and 22 us.  Vector instructions take 45 % of the cycles (per logit: widening,
-// maximum, FMA, v_exp at four times an instruction's cycles, addition, two
-// comparisons), waits for the loads and two barriers the rest.
+// end (49 MB): 17 us for the chunks, 2.9 TB/s, and 10.2 for the join.  50 registers,
+// so that 8 workgroups share a CU: with the next chunk's loads ahead it was 118 and
+// 22 us.  A short chunk's elements one by one, all on their way at once, in place of
+// its vectors: 77 and 18.4 us, for the whole chunks too.  Vector instructions take
+// 45 % of the cycles (per logit: widening, maximum, FMA, v_exp at four times an
+// instruction's cycles, addition, two comparisons), waits for the loads and two
+// barriers the rest.
 #include "common.h"
 
 namespace {
@@ -117,28 +119,40 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   if (a.done && a.done[row]) return;           // such a beam goes on with the end token alone
   const int c0 = ch * a.chunk, n = min(a.chunk, a.vocab - c0);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.ld + c0;
-  // Vectors of a row that starts anywhere; in a short chunk an element a thread and turn, so that every wave has
-  // its share.
+  // Vectors of a row that starts anywhere; a short chunk's go round the waves, so that each has its share.
   const bool whole = n == N * kT;
-  float v[N];
+  const int place = whole ? tid : lane * kWaves + wave;
+  u32x4_t raw[VT];
   if (whole) {
-    u32x4_t raw[VT];
 #pragma unroll
-    for (int j = 0; j < VT; ++j) __builtin_memcpy(&raw[j], x + (j * kT + tid) * V, 16);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i / 4][i % 4]);
-      else v[i] = __uint_as_float(i % 2 ? raw[i / 8][i % 8 / 2] & 0xffff0000u : raw[i / 8][i % 8 / 2] << 16);
-    }
+    for (int j = 0; j < VT; ++j) __builtin_memcpy(&raw[j], x + (j * kT + place) * V, 16);
   } else {
+    constexpr uint32_t kNo = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;                    // -infinity
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = Elt<T>::to_f(x[min(i * kT + tid, n - 1)]);      // (without branches: all on their way)
+    for (int j = 0; j < VT; ++j) {
+      const int e0 = (j * kT + place) * V;
+      raw[j] = (u32x4_t){kNo, kNo, kNo, kNo};
+      if (e0 + V <= n) {
+        __builtin_memcpy(&raw[j], x + e0, 16);
+      } else if (e0 < n) {                     // the row ends in this vector
+        T last[V];
+        __builtin_memcpy(last, &raw[j], 16);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i * kT + tid < n ? v[i] : -INFINITY;
+        for (int e = 0; e < V; ++e)
+          if (e0 + e < n) last[e] = x[e0 + e];
+        __builtin_memcpy(&raw[j], last, 16);
+      }
+    }
+  }
+  float v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[i / 4][i % 4]);
+    else v[i] = __uint_as_float(i % 2 ? raw[i / 8][i % 8 / 2] & 0xffff0000u : raw[i / 8][i % 8 / 2] << 16);
   }
   reinterpret_cast<u32x4_t*>(cand)[tid] = (u32x4_t){0, 0, 0, 0};    // the ranks below read whole eights
   reinterpret_cast<u32x4_t*>(cand)[kT + tid] = (u32x4_t){0, 0, 0, 0};
-  auto token = [&](int i) { return (uint32_t)(c0 + (whole ? ((i / V) * kT + tid) * V + i % V : i * kT + tid)); };
+  auto token = [&](int i) { return (uint32_t)(c0 + ((i / V) * kT + place) * V + i % V); };
   float m = v[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);                   // (a NaN is passed over)
