@@ -119,8 +119,11 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   if (a.done && a.done[row]) return;           // such a beam goes on with the end token alone
   const int c0 = ch * a.chunk, n = min(a.chunk, a.vocab - c0);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.ld + c0;
-  // Vectors of a row that starts anywhere; a short chunk's go round the waves, so that each has its share.
-  const bool whole = n == N * kT;
+  // Vectors of a row that starts anywhere.  A short chunk's go round the waves, so that each has its share; one of
+  // fewer than k vectors is taken by elements, since each lane has but one number for the threshold (64 x 8 beams
+  // over 849 tokens, k 128: 87 us by vectors, 40 by elements).
+  constexpr int kThin = V * 128 / kT;          // elements of a thread at most (k <= 128)
+  const bool whole = n == N * kT, thin = !whole && n < V * a.k;
   const int place = whole ? tid : lane * kWaves + wave;
   u32x4_t raw[VT];
   if (whole) {
@@ -132,6 +135,7 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
     for (int j = 0; j < VT; ++j) {
       const int e0 = (j * kT + place) * V;
       raw[j] = (u32x4_t){kNo, kNo, kNo, kNo};
+      if (thin) continue;
       if (e0 + V <= n) {
         __builtin_memcpy(&raw[j], x + e0, 16);
       } else if (e0 < n) {                     // the row ends in this vector
@@ -143,6 +147,14 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
         __builtin_memcpy(&raw[j], last, 16);
       }
     }
+    if (thin) {
+      T own[V];
+      __builtin_memcpy(own, &raw[0], 16);
+#pragma unroll
+      for (int e = 0; e < kThin; ++e)
+        if (e * kT + tid < n) own[e] = x[e * kT + tid];
+      __builtin_memcpy(&raw[0], own, 16);
+    }
   }
   float v[N];
 #pragma unroll
@@ -152,7 +164,8 @@ __device__ __forceinline__ void part_body(const vrs_beam_args& a) {
   }
   reinterpret_cast<u32x4_t*>(cand)[tid] = (u32x4_t){0, 0, 0, 0};    // the ranks below read whole eights
   reinterpret_cast<u32x4_t*>(cand)[kT + tid] = (u32x4_t){0, 0, 0, 0};
-  auto token = [&](int i) { return (uint32_t)(c0 + ((i / V) * kT + place) * V + i % V); };
+  const int token0 = c0 + (thin ? tid : place * V);
+  auto token = [&](int i) { return (uint32_t)(token0 + (thin && i < kThin ? i * kT : (i / V) * kT * V + i % V)); };
   float m = v[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);                   // (a NaN is passed over)
