@@ -563,9 +563,9 @@ int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_se
  * candidates (beam i, token t),
  *   c = scores[i] + (logits[i][t] - lse_i),  lse_i = log sum_t exp(logits[i][t])
  * in falling order, equal ones by the lowest i * vocab + t; candidates of one beam
- * are in the order of their logits.  lse comes from float32 exponentials summed in
- * 64 bits and c is compared in 64 bits, out_scores rounds it once.  done (may be
- * NULL): a beam whose byte is not 0 is at its end and goes on with the token `eos`
+ * are in the order of their logits.  lse comes from float32 exponentials, up to 32 of
+ * them summed in float32 and these sums in 64 bits; lse and c are held and compared in
+ * 64 bits, out_scores rounds c once.  done (may be NULL): a beam whose byte is not 0 is at its end and goes on with the token `eos`
  * alone, c = scores[i].  A candidate whose c is not a number counts as -infinity:
  * tokens with a logit of -infinity, all others of a beam at its end, and every
  * token of a beam whose score is not finite or whose logits hold a NaN or
@@ -613,8 +613,10 @@ int vrs_beam_reorder(vrs_ctx* ctx, const vrs_reorder_desc* d, const int32_t* par
  * sequences must not share key rows.  decay 0 does not read acc.
  * Scores, weights and sums are float32 and each sum has a fixed order.  head_dim,
  * alignment, strides and workspace (for a few rows to a key head 4 bytes for each
- * score, up to max_k of a row) as in vrs_attention, but that the heads of a key head
- * and 65 rows of q lie within 2^29 elements. */
+ * score of max_k keys to a row, rounded up to 1024) as in vrs_attention, but that the
+ * heads of a key head and 65 rows of q lie within 2^29 elements.  There is no form for
+ * shared prefixes: what a prefix receives is had before it is shared, from the queries
+ * of its prompt. */
 typedef struct {
   int32_t q_rows, k_rows;
   int32_t heads, kv_heads, head_dim, dtype;   /* VRS_BF16 or VRS_F32 */
