@@ -565,11 +565,11 @@ int vrs_prefix_attention(vrs_ctx* ctx, const vrs_attention_desc* d, const vrs_se
  * in falling order, equal ones by the lowest i * vocab + t; candidates of one beam
  * are in the order of their logits.  lse comes from float32 exponentials, up to 32 of
  * them summed in float32 and these sums in 64 bits; lse and c are held and compared in
- * 64 bits, out_scores rounds c once.  done (may be NULL): a beam whose byte is not 0 is at its end and goes on with the token `eos`
- * alone, c = scores[i].  A candidate whose c is not a number counts as -infinity:
- * tokens with a logit of -infinity, all others of a beam at its end, and every
- * token of a beam whose score is not finite or whose logits hold a NaN or
- * +infinity, or nothing else than -infinity.
+ * 64 bits, out_scores rounds c once.  done (may be NULL): a beam whose byte is not 0
+ * is at its end and goes on with the token `eos` alone, c = scores[i].  A candidate
+ * whose c is not a number counts as -infinity: tokens with a logit of -infinity, all
+ * others of a beam at its end, and every token of a beam whose score is not finite or
+ * whose logits hold a NaN or +infinity, or nothing else than -infinity.
  * logits: rows (beams of all requests, one after another) of contiguous elements,
  * ld elements apart, of any alignment of their elements.  k <= 128 and
  * <= beams * vocab, beams <= 64, beams * vocab < 2^31, up to 65535 rows.  The outputs
