@@ -1057,3 +1057,70 @@ def test_calls_that_overlap_on_two_streams():
     torch.cuda.synchronize()
     for n, outs in got:
         assert all(torch.equal(bits(a), bits(c)) for a, c in zip(outs, want[n])), n
+
+
+@pytest.mark.parametrize("case", [([2] * 210, [3 + i % 40 for i in range(210)], [3 * i for i in range(71)], [5 * i for i in range(70)]),
+                                  ([40] * 70, [i % 9 for i in range(70)], [0, 1, 30, 70], [300, 0, 41])])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefix_attention_of_many_groups_of_many_rows(dtype, case):
+    """Over 64 groups, or sequences, whose row tiles are found by a search."""
+    check_prefix(case, dtype, 8, 1, 64)
+    check_prefix(case, dtype, 8, 1, 64, hint=False)
+
+
+# ---- sizes that pass 32 bits ------------------------------------------------------------------
+
+
+def test_caches_whose_offsets_pass_32_bits():
+    """Prefixes, own keys and evicted ones behind 2^31 elements and 2^32 bytes of a cache: the bits of the same call
+    where they lie at its begin."""
+    import torch
+    rows, kv, dim, far = 4_300_000, 4, 128, 4_299_000
+    near = 1000
+    k, v = (torch.zeros(rows, kv, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    acc = torch.zeros(kv, rows, device="cuda")
+    for seed, t in ((1, k), (2, v)):
+        t[:near] = randn(near, kv, dim, seed=seed)
+        t[far:far + near] = t[:near]
+    acc[:, :near] = torch.rand(kv, near, device="cuda")
+    acc[:, far:far + near] = acc[:, :near]
+    for q_len, n_own in (([1] * 6, 90), ([30] * 6, 90)):
+        starts = [sum(q_len[:i]) for i in range(7)]
+        q = randn(starts[-1], 8, dim, seed=3, scale=2)
+        got, sums = [], []
+        for at in (0, far):
+            s = vrs.seqs(i32(starts), i32([at + 300 + 100 * i for i in range(6)]), i32([n_own] * 6), max_q=max(q_len), max_k=n_own)
+            p = vrs.prefixes(i32([0, 6]), i32([at]), i32([290]), max_rows=starts[-1], max_k=290)
+            got.append(ctx().prefix_attention(q, k, v, s, p))
+            a = acc.clone()
+            ctx().attention_weights(q, k, s, a)
+            sums.append(a[:, at:at + near].clone())
+            assert torch.equal(a[:, near:far], acc[:, near:far])
+        assert got[0].abs().max() > 0 and torch.equal(*got) and torch.equal(*sums)
+    kept, left = ctx().cache_evict(k, v, acc, i32([5, far + 5]), i32([900, 900]), 300, first=4, recent=50)
+    assert torch.equal(kept[0], kept[1]) and left.tolist() == [300, 300]
+    for t in (k, v, acc.t()):
+        assert torch.equal(t[:near], t[far:far + near])
+
+
+def test_beam_states_and_logits_whose_offsets_pass_32_bits():
+    import torch
+    rows, row = 70, 1 << 20
+    state = torch.zeros(2, 32, rows, row, dtype=torch.uint8, device="cuda")             # 4.7 GB
+    state[:, ::8] = torch.randint(0, 255, (2, 4, rows, row), dtype=torch.uint8, device="cuda")
+    parents = torch.zeros(4, 8, dtype=torch.int32, device="cuda")
+    lens = torch.full((32,), 69, dtype=torch.int32, device="cuda")
+    ctx().beam_reorder(state, parents, lens=lens)
+    for i in range(32):
+        assert torch.equal(state[:, i, :69], state[:, i // 8 * 8, :69])
+        assert i % 8 == 0 or not state[:, i, 69].any()
+    del state
+    batch, vocab = 1100, 250000
+    x = torch.zeros(batch, 8, vocab, dtype=torch.bfloat16, device="cuda")               # 2.2e9 logits
+    x[-1] = logits_of(1, 8, vocab, "bf16", seed=4)[0]
+    s = scores_of(batch, 8)
+    got = ctx().beam_select(x, s, 8)
+    ref = select_ref(x[-1:], s[-1:], 8)
+    assert torch.equal(got[1][-1:].cpu(), ref[1]) and torch.equal(got[2][-1:].cpu(), ref[2])
+    inside(got[0][-1:].cpu(), ref[0], ref[0].abs() * F * 1.01 + 34 * F * 4)
+    assert not got[1][:-1].any() and torch.equal(got[2][:-1].cpu(), torch.arange(8, dtype=torch.int32).expand(batch - 1, 8))
