@@ -694,6 +694,28 @@ def test_attention_weights_large_and_far_scores():
         check_weights("tokens", dtype, scale=1e-4)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q_len,past", [([1, 1], [60, 700]), ([60, 3], [0, 40]), ([50], [2000])])
+def test_attention_weights_of_scores_far_from_zero(dtype, q_len, past):
+    """Scores of 2^34, exact in either type: those keys share each query's weight evenly, the others get none."""
+    import torch
+    starts, rows, k_len, k_at, s = weights_case((q_len, past))
+    q = torch.zeros(rows, 4, 64, dtype=tdt(dtype), device="cuda")
+    k = torch.zeros(k_at[-1] + 4, 2, 64, dtype=tdt(dtype), device="cuda")
+    q[..., 0] = 2.0 ** 17
+    acc = torch.zeros(2, k_at[-1] + 4, device="cuda")
+    ref = acc.double()
+    for i, (n, m) in enumerate(zip(k_len, q_len)):
+        large = [j for j in (0, 7, 33, 59, n - 1) if j < n]
+        k[[k_at[i] + j for j in large], :, 0] = 2.0 ** 17
+        for j in range(m):
+            seen = [x for x in set(large) if x <= n - m + j]
+            for x in seen:
+                ref[:, k_at[i] + x] += 2 / len(seen)           # two heads of a key head
+    ctx().attention_weights(q, k, s, acc, scale=1.0)
+    inside(acc, ref, ref * 200 * F)
+
+
 def test_attention_weights_strides_workspace_and_graph():
     """acc with the heads inside its rows, views, a workspace full of NaN, replays."""
     import torch
@@ -826,6 +848,18 @@ def test_cache_evict_long(inplace):
     """More keys than the choice holds in registers (16384)."""
     check_evict([16384, 16385, 40000], 9000, 4, 500, "bf16", 1, 8, inplace)
     check_evict([20000], 19999, 0, 0, "bf16", 1, 8, inplace)
+
+
+def test_cache_evict_hint_chooses_kernels_only():
+    import torch
+    for k_len, budget in (([9000, 20, 4097], 700), ([300, 90], 64)):
+        k_at, rows = [0, 9001, 9030][:len(k_len)], 14000
+        k, v, acc = randn(rows, 2, 64, seed=1), randn(rows, 2, 64, seed=2), torch.rand(2, rows, device="cuda")
+        ref = evict_ref(k, v, acc, k_at, k_len, budget, 2, 30, (k, v, acc), k_at)
+        for hint in (0, 1, 4096, 4097, (1 << 31) - 1):
+            outs = [t.clone() for t in (k, v, acc)]
+            kept, _ = ctx().cache_evict(*outs, i32(k_at), i32(k_len), budget, first=2, recent=30, max_k=hint)
+            assert all(torch.equal(a, b) for a, b in zip((*outs, kept), ref)), hint
 
 
 def test_cache_evict_equal_and_odd_values():
