@@ -1102,6 +1102,42 @@ def test_prefix_attention_of_many_groups_of_many_rows(dtype, case):
     check_prefix(case, dtype, 8, 1, 64, hint=False)
 
 
+def test_empty_batches_and_caches():
+    """No keys, no sequences, no requests, no layers: results of nothing, and nothing else is touched."""
+    import torch
+    e = lambda *shape, dt=torch.bfloat16: torch.empty(shape, dtype=dt, device="cuda")      # noqa: E731
+    q = randn(6, 4, 64, seed=1)
+    for q_start in ([0, 1, 2], [0, 2, 6], [0, 0, 0]):
+        for prefix in (([0, 2], [0], [5]), ([0, 0, 2], [0, 3], [0, 9]), ([0], [], [])):
+            out = torch.full((6, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+            s = vrs.seqs(i32(q_start), i32([0, 0]), i32([0, 4]))
+            ctx().prefix_attention(q, e(0, 2, 64), e(0, 2, 64), s, vrs.prefixes(*map(i32, prefix)), out=out)
+            assert not out[:q_start[-1]].any() and torch.all(out[q_start[-1]:] == 5)
+    s = vrs.seqs(i32([0]), i32([]), i32([]))
+    k = randn(9, 2, 64, seed=2)
+    acc = torch.full((2, 9), 3.0, device="cuda")
+    assert ctx().prefix_attention(q, k, k, s, vrs.prefixes(i32([0, 0]), i32([0]), i32([9]))).shape == q.shape
+    ctx().attention_weights(q, k, s, acc)
+    ctx().attention_weights(q, e(0, 2, 64), vrs.seqs(i32([0, 6]), i32([0]), i32([3])), e(2, 0, dt=torch.float32))
+    assert torch.all(acc == 3)
+    ctx().attention_weights(e(0, 4, 64), k, vrs.seqs(i32([0, 0]), i32([2]), i32([3])), acc, decay=0.5)
+    assert acc[0].tolist() == [3, 3, 1.5, 1.5, 1.5, 3, 3, 3, 3] and torch.equal(acc[0], acc[1])
+    assert [t.shape for t in ctx().beam_select(e(0, 3, 50), e(0, 3, dt=torch.float32), 4)] == [(0, 4)] * 3
+    parents = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for shape in ((0, 6, 4, 8), (2, 6, 0, 8), (2, 6, 4, 0)):
+        assert ctx().beam_reorder(e(*shape), parents).shape == shape
+    assert ctx().beam_reorder(e(2, 0, 4, 8), torch.zeros(0, 3, dtype=torch.int32, device="cuda")).shape == (2, 0, 4, 8)
+    kept, left = ctx().cache_evict(e(0, 2, 64), e(0, 2, 64), e(2, 0, dt=torch.float32), i32([0, 4]), i32([7, 0]), 5)
+    assert torch.all(kept == -1) and left.tolist() == [0, 0]
+    v = randn(9, 2, 64, seed=3)
+    k0, v0, a0 = k.clone(), v.clone(), acc.clone()
+    kept, left = ctx().cache_evict(k, v, acc, i32([]), i32([]), 5)
+    assert kept.numel() == 0 and left.numel() == 0
+    kept, left = ctx().cache_evict(k, v, acc, i32([1]), i32([8]), 3, k_out=e(0, 2, 64), v_out=e(0, 2, 64), acc_out=e(2, 0, dt=torch.float32))
+    assert left.tolist() == [3] and kept.shape == (1, 2, 3)
+    assert torch.equal(k, k0) and torch.equal(v, v0) and torch.equal(acc, a0)
+
+
 # ---- sizes that pass 32 bits ------------------------------------------------------------------
 
 
